@@ -55,6 +55,9 @@ extern "C" {
 #define VINFER_ST_NONFINITE 2u   /* a row has no finite maximum after processing */
 #define VINFER_ST_HIST_FULL 4u   /* vinfer_hist_append: a slot had no room for a new token */
 #define VINFER_ST_INTERNAL 8u    /* an internal consistency check failed */
+#define VINFER_ST_BAD_SCORE 16u  /* vinfer_beam_select: a beam's score is NaN or +inf */
+#define VINFER_ST_BAD_PARENT 32u /* vinfer_reorder_states: a parent that cannot be copied from */
+#define VINFER_ST_BAD_LIST 64u   /* vinfer_distill_*: an id or a log-probability out of range */
 
 /* args.flags */
 #define VINFER_FLAG_EXACT_ALL 1u /* resolve every row with the exact multi-pass search */
@@ -198,6 +201,128 @@ int vinfer_hist_reset(const int32_t* slot_list, int64_t n, int64_t slots, int32_
                       int32_t* hist_counts, int32_t* hist_len, int32_t cap, void* stream);
 int vinfer_sample_decode(const VinferSampleArgs* args, int32_t* hist_len, int32_t cap,
                          void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- beam search -----------------------------------------------------------------------------
+ * No counterpart in the reference, which decodes one sequence a request
+ * (src/vinfer/runtime/generate.py:105-146). One step over requests of W = `beams` rows each: beam w
+ * of request r holds an accumulated log-probability scores[r, w] and row r * W + w of the logits.
+ * A continuation's score is scores[r, w] + logits[token] - logsumexp(row).
+ *  - out_scores / out_beams / out_tokens [requests, n]: the n best continuations over the request's
+ *    beams and the vocabulary, in descending score, ties by beam, then token. Slots behind the last
+ *    candidate get -inf, -1, -1. A beam with score -inf is dead and its row is not read; a token
+ *    with logit -inf is no candidate.
+ *  - next_scores / parents / next_tokens [requests, W] (all three or none): the first W of the
+ *    candidates whose token is none of eos[0 .. n_eos), laid into the request's slots: the best
+ *    child of a beam stays in the beam's slot, the others fill the slots without a child in
+ *    ascending order. parents are slot numbers over all requests (r * W + beam), as
+ *    vinfer_reorder_states takes them. A slot without a child gets -inf, itself and -1. n >=
+ *    beams * (1 + n_eos) always finds every continuation. next_scores may be the scores array.
+ *  - A score that is NaN or +inf sets VINFER_ST_BAD_SCORE, a live row whose logits hold a NaN or
+ *    +inf or nothing above -inf VINFER_ST_NONFINITE; such a beam has no candidates.
+ * The order is that of exact scores: sums closer than 4e-6 are taken again in double.
+ * The workspace needs no initialisation, holds nothing between calls and serves one call at a
+ * time; 16-byte aligned. requests * beams <= VINFER_MAX_BATCH. */
+#define VINFER_BEAM_MAX_WIDTH 32
+#define VINFER_BEAM_MAX_N 128
+#define VINFER_BEAM_MAX_EOS 16
+typedef struct VinferBeamArgs {
+  const void* logits;      /* [requests * beams, ld] row-major; the first `vocab` columns are used */
+  int32_t dtype;           /* VINFER_DTYPE_F32 or VINFER_DTYPE_BF16 */
+  int32_t beams;           /* W */
+  int64_t requests;
+  int64_t vocab;
+  int64_t ld;              /* row stride, in elements (>= vocab) */
+  const float* scores;     /* [requests, beams] */
+  const int32_t* eos;      /* [n_eos] stop ids, device; may be NULL when n_eos is 0 */
+  int32_t n_eos;
+  int32_t n;               /* candidates listed for each request */
+  float* out_scores;       /* [requests, n] */
+  int32_t* out_beams;      /* [requests, n] */
+  int32_t* out_tokens;     /* [requests, n] */
+  float* next_scores;      /* [requests, beams], or NULL with the next two */
+  int32_t* parents;        /* [requests, beams] */
+  int32_t* next_tokens;    /* [requests, beams] */
+  int32_t* status;         /* optional, one device int32 */
+} VinferBeamArgs;
+size_t vinfer_beam_workspace_bytes(int64_t requests, int32_t beams, int64_t vocab, int32_t dtype,
+                                   int32_t n);
+int vinfer_beam_select(const VinferBeamArgs* args, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* ---- decode states that follow the beams -------------------------------------------------------
+ * The batched form of the state pool's copy from slot to slot (src/vinfer/state/pool.py): slot s of
+ * every state takes the contents of slot parents[s]. A state is described by its runs of
+ * contiguous bytes: slot s holds, for every index of the outer dimensions, run_bytes bytes at
+ * base + s * slot_stride + sum(index * outer_stride) (strides in bytes).
+ *  - In place (dst == src, in all states or in none): parents[s] == s leaves the slot alone; any
+ *    other parent must keep its own state (parents[parents[s]] == parents[s], as vinfer_beam_select
+ *    lays beams out), else the slot is left alone and VINFER_ST_BAD_PARENT set.
+ *  - Into another buffer (which must not overlap the source): every slot is copied, from any parent.
+ *  - lengths (device int32 [slots]) with len_unit_bytes > 0 copies only the first lengths[s]
+ *    positions (of len_unit_bytes each) of every run, with len_outer >= 0 only the first lengths[s]
+ *    indices of that outer dimension; positions behind them are neither read nor written.
+ * A parent outside [0, slots) leaves the slot alone and sets VINFER_ST_BAD_PARENT. `states` is a
+ * host array, read during the call. slots <= VINFER_STATE_MAX_SLOTS. */
+#define VINFER_STATE_MAX_OUTER 4
+#define VINFER_STATE_MAX_SLOTS 8192
+typedef struct VinferState {
+  const void* src;
+  void* dst;
+  int64_t src_slot_stride;
+  int64_t dst_slot_stride;
+  int64_t run_bytes;
+  int64_t len_unit_bytes;      /* bytes of one position within a run; 0: runs are copied whole */
+  int32_t len_outer;           /* the outer dimension that lengths cut; -1: none */
+  int32_t n_outer;
+  int64_t outer_size[VINFER_STATE_MAX_OUTER];
+  int64_t src_outer_stride[VINFER_STATE_MAX_OUTER];
+  int64_t dst_outer_stride[VINFER_STATE_MAX_OUTER];
+} VinferState;
+int vinfer_reorder_states(const VinferState* states, int32_t n_states, const int32_t* parents,
+                          int64_t slots, const int32_t* lengths, int32_t* status, void* stream);
+
+/* ---- distillation from a teacher's top log-probabilities -----------------------------------------
+ * The training side of vinfer_sample_top_logprobs: rows of a student's logits against the lists of
+ * token ids and log-probabilities that a teacher left (natural logarithms, at the temperature of
+ * the student's softmax). With q = softmax(logits / temperature) and p_j = exp(logprobs_j):
+ *   loss[row] = weight * ( sum_j p_j (ln p_j - ln q_j)  [ + p_t (ln p_t - ln q_t) with tail ] )
+ * tail == 0: the p_j are first divided by their sum. tail != 0: p_t = max(0, 1 - sum p_j) is matched
+ * with q_t, the student's mass outside the list. The loss carries no factor temperature^2.
+ * Entries with id < 0 are empty; an entry with log-probability -inf lists its token with mass 0; an
+ * id listed twice has the sum of its masses. A row of weight 0 is not read: loss and gradient 0;
+ * without tail, a list of no mass gives loss and gradient 0.
+ * An id >= vocab or a log-probability that is NaN or +inf sets VINFER_ST_BAD_LIST, logits without a
+ * finite log-sum VINFER_ST_NONFINITE; the row's loss and gradient are then NaN.
+ *  - vinfer_distill_loss: losses [rows]; row_stats (float [rows, 2], 8-byte aligned) and list_grads
+ *    (float [rows, k]) receive what the gradient needs, both or neither.
+ *  - vinfer_distill_grad: d(sum_r grad_out[r] * loss[r]) / dlogits, of the logits' type, rounded once
+ *    (grad_out NULL: ones). args as for the loss. grad may be the logits (then with their ld).
+ *  - vinfer_distill_step: both in one call, grad_out all ones. grad may be the logits.
+ * The workspace needs no initialisation and holds nothing between calls; 16-byte aligned. */
+#define VINFER_DISTILL_MAX_K 128
+#define VINFER_DISTILL_MAX_ROWS (1 << 22)
+typedef struct VinferDistillArgs {
+  const void* logits;      /* [rows, ld] row-major; the first `vocab` columns are used */
+  int32_t dtype;           /* VINFER_DTYPE_F32 or VINFER_DTYPE_BF16 */
+  int32_t k;               /* entries of each list */
+  int64_t rows;
+  int64_t vocab;
+  int64_t ld;              /* row stride, in elements (>= vocab) */
+  const int32_t* ids;      /* [rows, k] */
+  const float* logprobs;   /* [rows, k] */
+  const float* weights;    /* [rows], NULL: ones */
+  float temperature;       /* > 0 */
+  int32_t tail;
+  int32_t* status;         /* optional, one device int32 */
+} VinferDistillArgs;
+size_t vinfer_distill_workspace_bytes(int64_t rows, int64_t vocab, int32_t dtype, int32_t k);
+int vinfer_distill_loss(const VinferDistillArgs* args, float* loss, float* row_stats,
+                        float* list_grads, void* workspace, size_t workspace_bytes, void* stream);
+int vinfer_distill_grad(const VinferDistillArgs* args, const float* row_stats,
+                        const float* list_grads, const float* grad_out, void* grad,
+                        int64_t ld_grad, void* stream);
+int vinfer_distill_step(const VinferDistillArgs* args, float* loss, void* grad, int64_t ld_grad,
+                        void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -18,6 +18,7 @@ DTYPE_F32 = 0
 DTYPE_BF16 = 1
 OK, E_ARG, E_LIMIT, E_CUDA = 0, 1, 2, 3
 ST_BAD_PARAM, ST_NONFINITE, ST_HIST_FULL, ST_INTERNAL = 1, 2, 4, 8
+ST_BAD_SCORE, ST_BAD_PARENT, ST_BAD_LIST = 16, 32, 64
 FLAG_EXACT_ALL = 1
 MAX_VOCAB = 262144
 MAX_BATCH = 65535
@@ -25,6 +26,13 @@ STATIC_SCRATCH_BYTES = 32 << 20
 HIST_PAD_ID = 0x7FFFFFFF
 TOP_LOGPROBS_MAX = 32
 HIST_MAX_CAP = 1 << 20
+BEAM_MAX_WIDTH = 32
+BEAM_MAX_N = 128
+BEAM_MAX_EOS = 16
+STATE_MAX_OUTER = 4
+STATE_MAX_SLOTS = 8192
+DISTILL_MAX_K = 128
+DISTILL_MAX_ROWS = 1 << 22
 
 EXPORTS = (
     "vinfer_sampler_abi_version",
@@ -40,6 +48,13 @@ EXPORTS = (
     "vinfer_hist_append",
     "vinfer_hist_reset",
     "vinfer_sample_decode",
+    "vinfer_beam_workspace_bytes",
+    "vinfer_beam_select",
+    "vinfer_reorder_states",
+    "vinfer_distill_workspace_bytes",
+    "vinfer_distill_loss",
+    "vinfer_distill_grad",
+    "vinfer_distill_step",
 )
 
 _ERRORS = {E_ARG: "invalid argument", E_LIMIT: "limit exceeded", E_CUDA: "CUDA error"}
@@ -70,6 +85,67 @@ class SampleArgs(C.Structure):
         ("uniforms", C.c_void_p),
         ("out_ids", C.c_void_p),
         ("out_probs", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+
+class BeamArgs(C.Structure):
+    """Mirror of ``VinferBeamArgs``."""
+
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("beams", C.c_int32),
+        ("requests", C.c_int64),
+        ("vocab", C.c_int64),
+        ("ld", C.c_int64),
+        ("scores", C.c_void_p),
+        ("eos", C.c_void_p),
+        ("n_eos", C.c_int32),
+        ("n", C.c_int32),
+        ("out_scores", C.c_void_p),
+        ("out_beams", C.c_void_p),
+        ("out_tokens", C.c_void_p),
+        ("next_scores", C.c_void_p),
+        ("parents", C.c_void_p),
+        ("next_tokens", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+
+class State(C.Structure):
+    """Mirror of ``VinferState``."""
+
+    _fields_ = [
+        ("src", C.c_void_p),
+        ("dst", C.c_void_p),
+        ("src_slot_stride", C.c_int64),
+        ("dst_slot_stride", C.c_int64),
+        ("run_bytes", C.c_int64),
+        ("len_unit_bytes", C.c_int64),
+        ("len_outer", C.c_int32),
+        ("n_outer", C.c_int32),
+        ("outer_size", C.c_int64 * STATE_MAX_OUTER),
+        ("src_outer_stride", C.c_int64 * STATE_MAX_OUTER),
+        ("dst_outer_stride", C.c_int64 * STATE_MAX_OUTER),
+    ]
+
+
+class DistillArgs(C.Structure):
+    """Mirror of ``VinferDistillArgs``."""
+
+    _fields_ = [
+        ("logits", C.c_void_p),
+        ("dtype", C.c_int32),
+        ("k", C.c_int32),
+        ("rows", C.c_int64),
+        ("vocab", C.c_int64),
+        ("ld", C.c_int64),
+        ("ids", C.c_void_p),
+        ("logprobs", C.c_void_p),
+        ("weights", C.c_void_p),
+        ("temperature", C.c_float),
+        ("tail", C.c_int32),
         ("status", C.c_void_p),
     ]
 
@@ -121,6 +197,25 @@ def load() -> C.CDLL:
     lib.vinfer_hist_reset.restype = C.c_int
     lib.vinfer_hist_reset.argtypes = [C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p,
                                       C.c_void_p, C.c_int32, C.c_void_p]
+    lib.vinfer_beam_workspace_bytes.restype = C.c_size_t
+    lib.vinfer_beam_workspace_bytes.argtypes = [C.c_int64, C.c_int32, C.c_int64, C.c_int32,
+                                                C.c_int32]
+    lib.vinfer_beam_select.restype = C.c_int
+    lib.vinfer_beam_select.argtypes = [C.POINTER(BeamArgs), C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.vinfer_reorder_states.restype = C.c_int
+    lib.vinfer_reorder_states.argtypes = [C.POINTER(State), C.c_int32, C.c_void_p, C.c_int64,
+                                          C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.vinfer_distill_workspace_bytes.restype = C.c_size_t
+    lib.vinfer_distill_workspace_bytes.argtypes = [C.c_int64, C.c_int64, C.c_int32, C.c_int32]
+    lib.vinfer_distill_loss.restype = C.c_int
+    lib.vinfer_distill_loss.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.vinfer_distill_grad.restype = C.c_int
+    lib.vinfer_distill_grad.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p,
+                                        C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+    lib.vinfer_distill_step.restype = C.c_int
+    lib.vinfer_distill_step.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p, C.c_int64,
+                                        C.c_void_p, C.c_size_t, C.c_void_p]
     version = lib.vinfer_sampler_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"sampler library ABI {version}, expected {ABI_VERSION}")
@@ -143,4 +238,10 @@ def status_message(bits: int) -> str:
         names.append("a history slot was full (a token was not counted)")
     if bits & ST_INTERNAL:
         names.append("internal consistency check failed")
+    if bits & ST_BAD_SCORE:
+        names.append("a beam's score is NaN or +inf")
+    if bits & ST_BAD_PARENT:
+        names.append("a slot's parent is out of range or loses its own state")
+    if bits & ST_BAD_LIST:
+        names.append("a teacher's list holds an id or a log-probability out of range")
     return ", ".join(names) or "ok"

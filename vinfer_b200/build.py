@@ -18,8 +18,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libvinfer_sampler.so"
-SOURCES = [CSRC / "sampler.cu"]
-HEADERS = [INCLUDE / "vinfer_sampler.h"]
+SOURCES = [CSRC / name for name in ("sampler.cu", "beam.cu", "states.cu", "distill.cu")]
+HEADERS = [INCLUDE / "vinfer_sampler.h", CSRC / "rows.cuh"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -32,6 +32,7 @@ NVCC_FLAGS = [
     "-fPIC",
     "-Xptxas",
     "-warn-spills",
+    "-t4",  # the sources side by side
 ]
 
 

@@ -1,0 +1,658 @@
+// beam.cu — one step of beam search over rows of logits (sm_100a).
+//
+// A request has W beams; beam w holds the accumulated log-probability b_w and a row x_w of logits.
+// Its continuations score  s(w, t) = b_w + x_w[t] - lse(x_w);  the n best over beams and tokens
+// are listed (descending score, ties by beam, then token), and the best W of them that do not end
+// the sequence are laid into the request's slots.
+//
+//   * k_beam_rows streams each live row once, cut into parts (one CTA each): the part's softmax sum
+//     and its n best logits. Within a beam the scores' order is the logits' order, so no score is
+//     needed to list a part exactly. A dead beam (score -inf) costs a CTA that returns at once.
+//   * k_beam_pick, one CTA a request, launched as its programmatic dependent: a warp joins each
+//     beam's parts (sum and n best), then the beams' lists are ranked by score in double. Two
+//     beams' scores closer than NEAR could be ordered by the rounding of their sums, so the sums of
+//     such beams (rare) are taken again in double before the order stands.
+#include "rows.cuh"
+
+#include <algorithm>
+
+namespace {
+
+using namespace rows;
+
+constexpr int NT = 256, NW = NT / 32;
+constexpr int U = 8;              // 16-byte vectors a thread holds: 32 KiB a CTA and round
+constexpr int MAX_PARTS = 64;     // parts of a row
+constexpr int MAX_JOIN = 1024;    // entries of a beam's parts together (a warp joins them)
+constexpr int MAXN = VINFER_BEAM_MAX_N, MAXW = VINFER_BEAM_MAX_WIDTH;
+// Scores of different beams within this distance are compared with sums taken in double: about
+// ten times the error of a streamed log-sum (2^-20 from rounding the largest exponents, 2^-22
+// from ex2, both mostly averaged out over the row).
+constexpr double NEAR = 4e-6;
+
+static_assert(MAXN <= 128 && MAXW <= 32, "lists fit the picking kernel's shared memory");
+
+typedef unsigned long long u64;
+
+// A candidate of one row: ascending keys are descending logits, equal logits by ascending id.
+__device__ __forceinline__ u64 entry(float x, int id) {
+  return ((u64)(~okey(x)) << 32) | (uint32_t)id;
+}
+__device__ __forceinline__ float entry_x(u64 e) { return from_okey(~(uint32_t)(e >> 32)); }
+__device__ __forceinline__ int entry_id(u64 e) { return (int)(uint32_t)e; }
+
+struct PartHdr {
+  float m, s;  // softmax sum of the part, (m, s) at scale L2E
+  int cnt;     // listed entries, ascending
+  int pad;
+};
+
+struct RowsP {
+  const void* logits;
+  int64_t ld;
+  int V, n, parts;
+  const float* scores;
+  PartHdr* hdr;  // [rows, parts]
+  u64* list;     // [rows, parts, n]
+};
+
+// shared memory of k_beam_rows: the list under construction, then
+struct RowsS {
+  u64 best[MAXN];
+  float f[2 * NW];
+  float kth[NW];
+  int cnt, got;
+  uint32_t hist[256];
+  uint32_t bin, before;
+};
+__host__ __device__ inline int list_cap(int n, int A) { return U * A * n + 2 * n + 64; }
+
+// The n smallest of list[0, L) into best (any order); L > n. Radix select by bytes: keys are
+// unique, so it ends with exactly n.
+__device__ void select_best(const u64* list, int L, int n, RowsS& S) {
+  u64 prefix = 0, mask = 0;
+  int want = n;  // rank of the last kept key within the keys that share the prefix
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    S.hist[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < L; i += NT)
+      if ((list[i] & mask) == prefix) atomicAdd(&S.hist[(list[i] >> shift) & 255], 1u);
+    __syncthreads();
+    if (threadIdx.x < 32) {  // lane l holds bins [8l, 8l + 8)
+      uint32_t sum = 0;
+      for (int b = 0; b < 8; ++b) sum += S.hist[threadIdx.x * 8 + b];
+      uint32_t incl = sum;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(FULL, incl, o);
+        if ((int)threadIdx.x >= o) incl += t;
+      }
+      uint32_t run = incl - sum;
+      if (run < (uint32_t)want && (uint32_t)want <= incl) {
+        for (int b = 0; b < 8; ++b) {
+          const uint32_t h = S.hist[threadIdx.x * 8 + b];
+          if ((uint32_t)want <= run + h) {
+            S.bin = threadIdx.x * 8 + b;
+            S.before = run;
+            break;
+          }
+          run += h;
+        }
+      }
+    }
+    __syncthreads();
+    prefix |= (u64)S.bin << shift;
+    mask |= (u64)255 << shift;
+    want -= (int)S.before;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) S.got = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < L; i += NT)
+    if (list[i] <= prefix) {
+      const int at = atomicAdd(&S.got, 1);
+      if (at < MAXN) S.best[at] = list[i];
+    }
+  __syncthreads();
+}
+
+// The n-th largest of the block's lane maxima (exact: every lane counts the larger ones).
+// -inf when fewer than n lanes hold more than -inf.
+__device__ float nth_lane_max(float mx, int n, float* all, float* out) {
+  all[threadIdx.x] = mx;
+  if (threadIdx.x == 0) *out = neg_inf();
+  __syncthreads();
+  int larger = 0, equal_before = 0;
+  for (int i = 0; i < NT; ++i) {
+    larger += all[i] > mx;
+    equal_before += all[i] == mx && i < (int)threadIdx.x;
+  }
+  if (larger + equal_before == n - 1) *out = mx;
+  __syncthreads();
+  return *out;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
+  using V8 = Vec<T>;
+  constexpr int A = V8::A;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  u64* list = reinterpret_cast<u64*>(dyn);
+  __shared__ RowsS S;
+  const int row = blockIdx.x / P.parts, part = blockIdx.x - row * P.parts;
+  const float b = P.scores[row];
+  if (!(b > neg_inf() && b < -neg_inf())) return;  // dead, or refused by k_beam_pick
+  const Row<T> R(static_cast<const T*>(P.logits) + (int64_t)row * P.ld, P.V);
+  const int v0 = (int)((int64_t)R.nv * part / P.parts);
+  const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
+  const int n = P.n, cap = list_cap(n, A), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (tid == 0) S.cnt = 0;
+
+  float m = neg_inf(), s = 0.f;  // this thread's softmax sum
+  float bar = neg_inf();   // n listed or listable elements are >= bar, at lower ids than what follows
+  bool first = true;
+  int listed = 0;          // entries of the list when the round begins
+  for (int vb = v0; vb < v1; vb += NT * U) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = vb + u * NT + tid;
+      const uint32_t ni = V8::NEG_INF_WORD;
+      q[u] = v < v1 ? R.load(v) : make_uint4(ni, ni, ni, ni);
+    }
+    float mx = V8::max(q[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) mx = fmaxf(mx, V8::max(q[u]));
+    add_exps<T>(q, mx, L2E, m, s);
+
+    // The bar: a value that at least n lanes' maxima reach, so at least n elements do. The first
+    // round takes the smallest of the warps' k-th largest maxima (8k >= n); about 3n elements
+    // pass. Where that is -inf (short parts) or too many elements pass, the exact n-th maximum.
+    bool tight = false;
+    if (first) {
+      uint32_t key = okey(mx), top = 0;
+      for (int k = (n + NW - 1) / NW; k > 0; --k) {
+        top = __reduce_max_sync(FULL, key);
+        const unsigned who = __ballot_sync(FULL, key == top);
+        if (lane == __ffs(who) - 1) key = 0;
+      }
+      if (lane == 0) S.kth[w] = from_okey(top);
+      __syncthreads();
+      float t = S.kth[0];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) t = fminf(t, S.kth[i]);
+      bar = t;
+      if (!(t > neg_inf())) tight = true;
+    }
+    if (!tight) {
+      if (first ? mx >= bar : mx > bar) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float vm = V8::max(q[u]);
+          if (first ? vm >= bar : vm > bar) {
+            const int e0 = (vb + u * NT + tid) * A - R.off;
+            for (int j = 0; j < A; ++j) {
+              const float x = V8::get(q[u], j);
+              if ((first ? x >= bar : x > bar) && x > neg_inf()) {
+                const int at = atomicAdd(&S.cnt, 1);
+                if (at < cap) list[at] = entry(x, e0 + j);
+              }
+            }
+          }
+        }
+      }
+      __syncthreads();
+      tight = S.cnt > cap;
+    }
+    if (tight) {  // uniform: bounded and exact, whatever the data
+      __syncthreads();
+      int have = listed;
+      if (have > n) {
+        select_best(list, have, n, S);
+        for (int i = tid; i < n; i += NT) list[i] = S.best[i];
+        have = n;
+        __syncthreads();
+      }
+      // above the higher of the bar so far and this round's n-th lane maximum lie the elements
+      // of fewer than n lanes: at most (n - 1) * U * A
+      const float old = first ? neg_inf() : bar;
+      float* all = reinterpret_cast<float*>(S.hist);
+      const float nth = nth_lane_max(mx, n, all, S.f);
+      const float lo = fmaxf(old, nth);
+      if (tid == 0) S.cnt = have;
+      __syncthreads();
+      int eq_room = nth > old ? n : 0;  // equal elements count only where this round sets the bar
+      for (int u = 0; u < U; ++u) {
+        // q[u] by a dynamic index would live in local memory; the vector is read again
+        const int v = vb + u * NT + tid;
+        const uint32_t ni = V8::NEG_INF_WORD;
+        const uint4 r = v < v1 ? R.load(v) : make_uint4(ni, ni, ni, ni);
+        const int e0 = v * A - R.off;
+        int eq = 0;
+        for (int j = 0; j < A; ++j) {
+          const float x = V8::get(r, j);
+          if (x > lo) {
+            const int at = atomicAdd(&S.cnt, 1);
+            if (at < cap) list[at] = entry(x, e0 + j);
+          }
+          eq += x == lo && x > neg_inf();
+        }
+        if (eq_room > 0) {  // uniform: the lowest ids among the elements equal to the bar
+          int incl = eq;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(FULL, incl, o);
+            if (lane >= o) incl += t;
+          }
+          __syncthreads();
+          int* wsum = reinterpret_cast<int*>(S.kth);
+          if (lane == 31) wsum[w] = incl;
+          __syncthreads();
+          int base = incl - eq, total = 0;
+          for (int i = 0; i < NW; ++i) {
+            if (i < w) base += wsum[i];
+            total += wsum[i];
+          }
+          for (int j = 0; j < A && base < eq_room; ++j) {
+            const float x = V8::get(r, j);
+            if (x == lo && x > neg_inf()) {
+              const int at = atomicAdd(&S.cnt, 1);
+              if (at < cap) list[at] = entry(x, e0 + j);
+              ++base;
+            }
+          }
+          eq_room -= total;
+        }
+      }
+      __syncthreads();
+      bar = lo;
+    }
+    first = false;
+    listed = S.cnt;
+    __syncthreads();
+  }
+
+  // the part's n best, in order, and its sum
+  const int L = min(S.cnt, cap);
+  const u64* src = list;
+  int have = L;
+  if (L > 384) {
+    if (L > n) {
+      select_best(list, L, n, S);
+      src = S.best;
+      have = n;
+    }
+  }
+  const int64_t at = (int64_t)blockIdx.x;
+  u64* out = P.list + at * n;
+  for (int i = tid; i < have; i += NT) {
+    const u64 e = src[i];
+    int rank = 0;
+    for (int j = 0; j < have; ++j) rank += src[j] < e;
+    if (rank < n) out[rank] = e;
+  }
+  block_join<NW>(m, s, L2E, S.f);
+  if (tid == 0) {
+    PartHdr h;
+    h.m = m;
+    h.s = s;
+    h.cnt = min(have, n);
+    h.pad = 0;
+    P.hdr[at] = h;
+  }
+}
+
+struct PickP {
+  RowsP r;
+  int W, n_eos;
+  const int* eos;
+  float* out_scores;
+  int* out_beams;
+  int* out_tokens;
+  float* next_scores;
+  int* parents;
+  int* next_tokens;
+  int* status;
+};
+
+struct PickS {
+  double m[MAXW], lns[MAXW];  // log-sum of each beam's row: m + lns
+  float b[MAXW];        // beam scores
+  int cnt[MAXW];        // entries of each beam's list
+  int head[MAXN];       // ranked candidates: beam << 16 | place in its list
+  uint32_t flags;       // beams whose sums are taken again
+  int alive;            // surviving candidates
+  float kth[NW];
+  double red[NW];
+  int sel[MAXW];        // continuing candidates: their ranks
+  int nsel;
+};
+
+template <typename T>
+__device__ void row_sum_double(const RowsP& P, int row, double* red, double* m_out,
+                               double* lns_out) {
+  // strided by element, so equal rows get equal sums whatever their alignment
+  const T* x = static_cast<const T*>(P.logits) + (int64_t)row * P.ld;
+  float m = neg_inf();
+  for (int i = threadIdx.x; i < P.V; i += NT) m = fmaxf(m, Vec<T>::load(x + i));
+  m = warp_max(m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+  __syncthreads();
+  double mm = red[0];
+  for (int i = 1; i < NW; ++i) mm = fmax(mm, red[i]);
+  __syncthreads();
+  double s = 0;
+  for (int i = threadIdx.x; i < P.V; i += NT) s += exp((double)Vec<T>::load(x + i) - mm);
+  s = warp_sum(s);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = 0;
+  for (int i = 0; i < NW; ++i) s += red[i];
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *m_out = mm;
+    *lns_out = log(s);
+  }
+}
+
+// One CTA a request. Dynamic shared memory: W * n entries (the beams' lists), W * n 2-byte
+// places of surviving candidates, and parts * n entries for each warp's join.
+template <typename T>
+__global__ void __launch_bounds__(NT, 1) k_beam_pick(const PickP Q) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ PickS S;
+  const RowsP& P = Q.r;
+  const int W = Q.W, n = P.n, req = blockIdx.x, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  u64* lists = reinterpret_cast<u64*>(dyn);
+  u64* join = lists + W * n + w * P.parts * n;
+  unsigned short* live = reinterpret_cast<unsigned short*>(lists + W * n + NW * P.parts * n);
+  if (tid == 0) {
+    S.flags = 0;
+    S.alive = 0;
+    S.nsel = 0;
+  }
+  grid_dependency_wait();
+
+  for (int beam = w; beam < W; beam += NW) {
+    const int64_t row = (int64_t)req * W + beam;
+    const float b = P.scores[row];
+    int cnt = 0;
+    double lns = 0, top = 0;
+    if (b > neg_inf() && b < -neg_inf()) {
+      const PartHdr* H = P.hdr + row * P.parts;
+      const u64* E = P.list + row * P.parts * n;
+      float m = neg_inf();
+      for (int p = lane; p < P.parts; p += 32) m = fmaxf(m, H[p].m);
+      m = warp_max(m);
+      double s = 0;
+      for (int p = lane; p < P.parts; p += 32)
+        if (H[p].s != 0.f) s += (double)H[p].s * exp2(((double)H[p].m - (double)m) * (double)L2E);
+      s = warp_sum(s);
+      if (s > 0 && s < (double)FLT_MAX) {
+        top = m;
+        lns = log(s);
+        // n best of the parts' lists. Every lane's k-th best bounds the n-th best of all from
+        // below (32k >= n); what reaches the least of them survives, and is ranked by counting.
+        const int total = P.parts * n, k = (n + 31) / 32;
+        u64 bound = 0;
+        {
+          u64 t[4] = {~0ull, ~0ull, ~0ull, ~0ull};  // this lane's four best, ascending
+          for (int i = lane; i < total; i += 32) {
+            const int p = i / n;
+            u64 e = i - p * n < H[p].cnt ? E[i] : ~0ull;
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+              if (e < t[a]) {
+                const u64 o = t[a];
+                t[a] = e;
+                e = o;
+              }
+          }
+          bound = k == 1 ? t[0] : k == 2 ? t[1] : k == 3 ? t[2] : t[3];
+#pragma unroll
+          for (int o = 16; o; o >>= 1) {
+            const u64 other = __shfl_xor_sync(FULL, bound, o);
+            bound = other > bound ? other : bound;
+          }
+        }
+        int alive = 0;
+        for (int i0 = 0; i0 < total; i0 += 32) {
+          const int i = i0 + lane, p = i / n;
+          const u64 e = i < total && i - p * n < H[p].cnt ? E[i] : ~0ull;
+          const bool keep = e <= bound && e != ~0ull;
+          const unsigned m = __ballot_sync(FULL, keep);
+          if (keep) join[alive + __popc(m & ((1u << lane) - 1))] = e;
+          alive += __popc(m);
+        }
+        __syncwarp();
+        for (int i = lane; i < alive; i += 32) {
+          const u64 e = join[i];
+          int rank = 0;
+          for (int j = 0; j < alive; ++j) rank += join[j] < e;
+          if (rank < n) lists[beam * n + rank] = e;
+        }
+        cnt = min(alive, n);
+      } else if (lane == 0 && Q.status) {  // a NaN or +inf, or every logit -inf
+        atomicOr(Q.status, (int)VINFER_ST_NONFINITE);
+      }
+    } else if (lane == 0 && Q.status && !(b == neg_inf())) {
+      atomicOr(Q.status, (int)VINFER_ST_BAD_SCORE);
+    }
+    if (lane == 0) {
+      S.b[beam] = b;
+      S.m[beam] = top;
+      S.lns[beam] = lns;
+      S.cnt[beam] = cnt;
+    }
+  }
+  __syncthreads();
+
+  auto score = [&](int beam, int j) {
+    return (double)S.b[beam] + (((double)entry_x(lists[beam * n + j]) - S.m[beam]) - S.lns[beam]);
+  };
+  // candidates that can be among the n best, or within NEAR of the last of them
+  {
+    const int k = (n + NW - 1) / NW;
+    float mine = neg_inf();
+    for (int i = tid; i < W * n; i += NT) {
+      const int beam = i / n, j = i - beam * n;
+      if (j < S.cnt[beam]) mine = fmaxf(mine, __double2float_rd(score(beam, j)));
+    }
+    uint32_t key = okey(mine), top = 0;
+    for (int a = 0; a < k; ++a) {
+      top = __reduce_max_sync(FULL, key);
+      const unsigned who = __ballot_sync(FULL, key == top);
+      if (lane == __ffs(who) - 1) key = 0;
+    }
+    if (lane == 0) S.kth[w] = top ? from_okey(top) : neg_inf();
+    __syncthreads();
+    float t = S.kth[0];
+    for (int i = 1; i < NW; ++i) t = fminf(t, S.kth[i]);
+    for (int i = tid; i < W * n; i += NT) {
+      const int beam = i / n, j = i - beam * n;
+      if (j < S.cnt[beam] && score(beam, j) >= (double)t - 2 * NEAR)
+        live[atomicAdd(&S.alive, 1)] = (unsigned short)(beam << 8 | j);
+    }
+    __syncthreads();
+  }
+  for (int pass = 0; pass < 2; ++pass) {
+    for (int i = tid; i < S.alive; i += NT) {
+      const int bi = live[i] >> 8, ji = live[i] & 255;
+      const double si = score(bi, ji);
+      int rank = 0;
+      uint32_t close = 0;
+      for (int k = 0; k < S.alive; ++k) {
+        const int bk = live[k] >> 8, jk = live[k] & 255;
+        if (bk == bi) {
+          rank += jk < ji;
+        } else {
+          const double sk = score(bk, jk);
+          rank += sk > si || (sk == si && bk < bi);
+          if (fabs(sk - si) <= NEAR) close |= 1u << bk;
+        }
+      }
+      if (rank < n) {
+        S.head[rank] = bi << 16 | ji;
+        if (close && pass == 0) atomicOr(&S.flags, close | 1u << bi);
+      }
+    }
+    __syncthreads();
+    const uint32_t flags = S.flags;
+    if (pass == 1 || flags == 0) break;
+    for (int beam = 0; beam < W; ++beam)
+      if (flags >> beam & 1)
+        row_sum_double<T>(P, req * W + beam, S.red, &S.m[beam], &S.lns[beam]);
+    __syncthreads();
+  }
+
+  // the list of candidates
+  const int have = min(S.alive, n);
+  for (int i = tid; i < n; i += NT) {
+    const int64_t o = (int64_t)req * n + i;
+    if (i < have) {
+      const int beam = S.head[i] >> 16, j = S.head[i] & 0xffff;
+      Q.out_scores[o] = (float)score(beam, j);
+      Q.out_beams[o] = beam;
+      Q.out_tokens[o] = entry_id(lists[beam * n + j]);
+    } else {
+      Q.out_scores[o] = neg_inf();
+      Q.out_beams[o] = -1;
+      Q.out_tokens[o] = -1;
+    }
+  }
+  // the beams that go on: the first W candidates whose token is no stop id
+  if (tid < 32 && Q.parents) {
+    int nsel = 0;
+    for (int i0 = 0; i0 < have && nsel < W; i0 += 32) {
+      const int i = i0 + lane;
+      bool on = i < have;
+      if (on) {
+        const int id = entry_id(lists[(S.head[i] >> 16) * n + (S.head[i] & 0xffff)]);
+        for (int e = 0; e < Q.n_eos; ++e) on = on && id != Q.eos[e];
+      }
+      const unsigned m = __ballot_sync(FULL, on);
+      const int at = nsel + __popc(m & ((1u << lane) - 1));
+      if (on && at < W) S.sel[at] = i;
+      nsel = min(W, nsel + __popc(m));
+    }
+    __syncwarp();
+    // lane i: the i-th of them. The best child of a beam keeps the beam's slot (its state stays
+    // where it is), the others take the slots without a child in turn.
+    const bool on = lane < nsel;
+    const int cand = on ? S.head[S.sel[lane]] : 0;
+    const int beam = on ? cand >> 16 : MAXW + lane;
+    const unsigned same = __match_any_sync(FULL, beam);
+    const bool stays = on && (__ffs(same) - 1) == lane;
+    const unsigned taken = __reduce_or_sync(FULL, stays ? 1u << beam : 0u);
+    const unsigned late = __ballot_sync(FULL, on && !stays);
+    int slot = beam;
+    const unsigned open = ~taken & (W == 32 ? FULL : (1u << W) - 1);
+    if (on && !stays) {
+      unsigned f = open;
+      for (int k = __popc(late & ((1u << lane) - 1)); k > 0; --k) f &= f - 1;
+      slot = __ffs(f) - 1;
+    }
+    const unsigned filled = __reduce_or_sync(FULL, on ? 1u << slot : 0u);
+    if (on) {
+      const int64_t o = (int64_t)req * W + slot;
+      Q.next_scores[o] = (float)score(beam, cand & 0xffff);
+      Q.parents[o] = req * W + beam;
+      Q.next_tokens[o] = entry_id(lists[beam * n + (cand & 0xffff)]);
+    }
+    if (lane < W && !(filled >> lane & 1)) {
+      const int64_t o = (int64_t)req * W + lane;
+      Q.next_scores[o] = neg_inf();
+      Q.parents[o] = req * W + lane;
+      Q.next_tokens[o] = -1;
+    }
+  }
+}
+
+// Parts of a row: enough CTAs to fill the 148 SMs several times over, at least two vectors a
+// thread in each, and no more entries than a warp joins.
+int beam_parts(int64_t rows, int64_t vocab, int dtype, int n) {
+  const int64_t A = dtype == VINFER_DTYPE_BF16 ? 8 : 4;
+  const int64_t nv = (vocab + A - 1) / A;
+  int64_t p = (148 * 8 + rows - 1) / rows;
+  p = std::min<int64_t>(p, (nv + 2 * NT - 1) / (2 * NT));
+  p = std::min<int64_t>(p, std::min<int64_t>(MAX_PARTS, MAX_JOIN / n));
+  return (int)std::max<int64_t>(1, p);
+}
+
+size_t pick_smem(int W, int n, int parts) {
+  return (size_t)W * n * 8 + (size_t)NW * parts * n * 8 + (size_t)W * n * 2;
+}
+
+bool beam_shape_ok(int64_t requests, int32_t beams, int64_t vocab, int32_t dtype, int32_t n) {
+  return requests >= 1 && beams >= 1 && beams <= MAXW && vocab >= 1 && vocab <= VINFER_MAX_VOCAB &&
+         n >= 1 && n <= MAXN && requests <= VINFER_MAX_BATCH && requests * beams <= VINFER_MAX_BATCH &&
+         (dtype == VINFER_DTYPE_F32 || dtype == VINFER_DTYPE_BF16);
+}
+
+template <typename T>
+int launch_beam(const PickP& Q, int64_t requests, cudaStream_t st) {
+  const int64_t rows_ = requests * Q.W;
+  const size_t sm_rows = (size_t)list_cap(Q.r.n, Vec<T>::A) * 8;
+  const size_t sm_pick = pick_smem(Q.W, Q.r.n, Q.r.parts);
+  if (opt_in(k_beam_rows<T>, sm_rows) != VINFER_OK || opt_in(k_beam_pick<T>, sm_pick) != VINFER_OK)
+    return VINFER_E_CUDA;
+  const int rc = launch(k_beam_rows<T>, (unsigned)(rows_ * Q.r.parts), NT, sm_rows, st, false, Q.r);
+  if (rc != VINFER_OK) return rc;
+  return launch(k_beam_pick<T>, (unsigned)requests, NT, sm_pick, st, true, Q);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vinfer_beam_workspace_bytes(int64_t requests, int32_t beams, int64_t vocab, int32_t dtype,
+                                   int32_t n) {
+  if (!beam_shape_ok(requests, beams, vocab, dtype, n)) return 0;
+  const int64_t rows_ = requests * beams;
+  return (size_t)rows_ * beam_parts(rows_, vocab, dtype, n) * (sizeof(PartHdr) + 8 * (size_t)n);
+}
+
+int vinfer_beam_select(const VinferBeamArgs* a, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  NvtxRange nvtx_range("vinfer_beam_select");
+  if (!a || !a->logits || !a->scores || !a->out_scores || !a->out_beams || !a->out_tokens)
+    return VINFER_E_ARG;
+  if (a->dtype != VINFER_DTYPE_F32 && a->dtype != VINFER_DTYPE_BF16) return VINFER_E_ARG;
+  if (a->requests < 1 || a->beams < 1 || a->vocab < 1 || a->ld < a->vocab || a->n < 1)
+    return VINFER_E_ARG;
+  if (a->n_eos < 0 || (a->n_eos > 0 && !a->eos)) return VINFER_E_ARG;
+  if (!a->next_scores != !a->parents || !a->parents != !a->next_tokens) return VINFER_E_ARG;
+  if (((uintptr_t)a->logits) % (a->dtype == VINFER_DTYPE_BF16 ? 2 : 4)) return VINFER_E_ARG;
+  if (a->n_eos > VINFER_BEAM_MAX_EOS ||
+      !beam_shape_ok(a->requests, a->beams, a->vocab, a->dtype, a->n))
+    return VINFER_E_LIMIT;
+  if (!workspace || ((uintptr_t)workspace) % 16) return VINFER_E_ARG;
+  if (workspace_bytes <
+      vinfer_beam_workspace_bytes(a->requests, a->beams, a->vocab, a->dtype, a->n))
+    return VINFER_E_LIMIT;
+  const int64_t rows_ = a->requests * a->beams;
+  PickP Q = {};
+  Q.r.logits = a->logits;
+  Q.r.ld = a->ld;
+  Q.r.V = (int)a->vocab;
+  Q.r.n = a->n;
+  Q.r.parts = beam_parts(rows_, a->vocab, a->dtype, a->n);
+  Q.r.scores = a->scores;
+  Q.r.hdr = static_cast<PartHdr*>(workspace);
+  Q.r.list = reinterpret_cast<u64*>(static_cast<unsigned char*>(workspace) +
+                                    (size_t)rows_ * Q.r.parts * sizeof(PartHdr));
+  Q.W = a->beams;
+  Q.n_eos = a->n_eos;
+  Q.eos = a->eos;
+  Q.out_scores = a->out_scores;
+  Q.out_beams = a->out_beams;
+  Q.out_tokens = a->out_tokens;
+  Q.next_scores = a->next_scores;
+  Q.parents = a->parents;
+  Q.next_tokens = a->next_tokens;
+  Q.status = a->status;
+  cudaStream_t st = (cudaStream_t)stream;
+  return a->dtype == VINFER_DTYPE_BF16 ? launch_beam<__nv_bfloat16>(Q, a->requests, st)
+                                       : launch_beam<float>(Q, a->requests, st);
+}
+
+}  // extern "C"

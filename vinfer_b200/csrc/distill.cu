@@ -1,0 +1,442 @@
+// distill.cu — distillation from a teacher's top log-probabilities, loss and gradient (sm_100a).
+//
+// A row of student logits x[V], temperature T, z = x / T, q = softmax(z); the teacher's list
+// (id_j, l_j), j < k, with p_j = exp(l_j), renormalised to one without the tail, or as they are
+// with it (the rest of the mass, p_t = 1 - sum p, is then matched with the student's mass outside
+// the list, q_t):
+//   loss = sum_j p_j (ln p_j - ln q_{id_j})  [ + p_t (ln p_t - ln q_t) ]
+//   T dloss/dx_i = M q_i - (p_j summed over entries that list i)   inside the list
+//                = q_i (M - p_t / q_t)                              outside it
+// where M = sum p + p_t is the target's mass. Ids below 0 are empty entries.
+//
+//   * k_distill_rows streams each row once, cut into parts for small batches: the online softmax
+//     sum over the elements OUTSIDE the list (a listed element is set to -inf in the registers
+//     that hold it), so that q_t is summed, not left over from a difference.
+//   * k_distill_finish, one warp a row: joins the parts and the list's k terms in double.
+//   * k_distill_grad reads the row again and writes the gradient, one exponential an element; the
+//     listed elements are stored behind it.
+#include "rows.cuh"
+
+#include <algorithm>
+
+namespace {
+
+using namespace rows;
+
+constexpr int NT = 256, NW = NT / 32;
+constexpr int U = 8;            // 16-byte vectors a thread holds: 32 KiB a CTA and round
+constexpr int MAX_PARTS = 64;
+constexpr int MAXK = VINFER_DISTILL_MAX_K;
+static_assert(MAXK <= NT && MAXK <= 128, "one thread an entry; four entries a lane");
+
+struct Part {
+  float m, s;  // softmax sum outside the list, (m, s)
+};
+struct Stat {
+  float m, coef;  // an element outside the list has dloss/dz = coef * 2^((x - m) * scale)
+};
+
+struct DistP {
+  const void* logits;
+  int64_t ld, rows;
+  int V, k, parts;
+  int tail;
+  float scale;       // log2(e) / T rounded to float
+  double scale_d;
+  float inv_t;
+  const int* ids;
+  const float* lp;
+  const float* weights;
+  Part* part;        // [rows, parts]
+  float* loss;
+  Stat* stat;        // [rows], null: loss only
+  float* listg;      // [rows, k]: dloss/dz of the listed elements
+  int* status;
+  const float* grad_out;
+  void* grad;
+  int64_t ldg;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
+  using VT = Vec<T>;
+  constexpr int A = VT::A;
+  __shared__ float sm[2 * NW];
+  __shared__ int hit[MAXK];
+  __shared__ int hits;
+  const int64_t row = blockIdx.x / P.parts;
+  const int part = (int)(blockIdx.x - row * P.parts), tid = threadIdx.x;
+  if (P.weights && P.weights[row] == 0.f) return;
+  const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
+  const int v0 = (int)((int64_t)R.nv * part / P.parts);
+  const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
+  if (tid == 0) hits = 0;
+  __syncthreads();
+  if (tid < P.k) {  // the part's listed elements, counted from its first vector
+    const int id = P.ids[row * P.k + tid];
+    const int e = id + R.off - v0 * A;
+    if (id >= 0 && id < P.V && e >= 0 && e < (v1 - v0) * A) hit[atomicAdd(&hits, 1)] = e;
+  }
+  __syncthreads();
+  float m = neg_inf(), s = 0.f;
+  for (int vb = v0; vb < v1; vb += NT * U) {
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = vb + u * NT + tid;
+      const uint32_t ni = VT::NEG_INF_WORD;
+      q[u] = v < v1 ? R.load(v) : make_uint4(ni, ni, ni, ni);
+    }
+    for (int h = 0; h < hits; ++h) {
+      const int e = hit[h] - (vb - v0) * A;
+      if (e >= 0 && e < NT * U * A && ((e / A) & (NT - 1)) == tid) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (u == e / (A * NT)) VT::put(q[u], e & (A - 1), VT::NEG_INF_BITS);
+      }
+    }
+    float mx = VT::max(q[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) mx = fmaxf(mx, VT::max(q[u]));
+    add_exps<T>(q, mx, P.scale, m, s);
+  }
+  block_join<NW>(m, s, P.scale, sm);
+  if (tid == 0) P.part[blockIdx.x] = Part{m, s};
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT) k_distill_finish(const DistP P) {
+  __shared__ int sid[NW][MAXK];
+  __shared__ float sp[NW][MAXK];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * NW + w;
+  const bool there = row < P.rows;
+  const float weight = there && P.weights ? P.weights[row] : 1.f;
+  int id[4];
+  float l[4];
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = lane + 32 * i;
+    id[i] = -1;
+    l[i] = neg_inf();
+    if (there && j < P.k) {
+      id[i] = P.ids[row * P.k + j];
+      if (id[i] >= 0) l[i] = P.lp[row * P.k + j];
+      if (id[i] >= P.V || !(l[i] < -neg_inf())) bad = true;
+      sid[w][j] = id[i];
+      sp[w][j] = l[i];
+    }
+  }
+  __syncwarp();
+  grid_dependency_wait();
+  if (!there) return;
+  if (weight == 0.f) {
+    if (lane == 0) P.loss[row] = 0.f;
+    return;
+  }
+  bad = __any_sync(FULL, bad);
+  if (bad) {
+    const float nan = __int_as_float(0x7fffffff);
+    if (lane == 0) {
+      P.loss[row] = nan;
+      if (P.stat) P.stat[row] = Stat{nan, nan};
+      if (P.status) atomicOr(P.status, (int)VINFER_ST_BAD_LIST);
+    }
+    if (P.stat)
+      for (int j = lane; j < P.k; j += 32) P.listg[row * P.k + j] = nan;
+    return;
+  }
+  // the sum outside the list: r * 2^rest with rest = m * log2(e) / T
+  float m = neg_inf();
+  for (int p = lane; p < P.parts; p += 32)
+    if (P.part[row * P.parts + p].s != 0.f) m = fmaxf(m, P.part[row * P.parts + p].m);
+  m = warp_max(m);
+  double r = 0;
+  for (int p = lane; p < P.parts; p += 32) {
+    const Part h = P.part[row * P.parts + p];
+    if (h.s != 0.f) r += (double)h.s * exp2(((double)h.m - (double)m) * (double)P.scale);
+  }
+  r = warp_sum(r);
+  const double inf = (double)-neg_inf();
+  // all in distances from the row's largest logit `ref`, whatever its magnitude
+  double ref = r == 0 ? -inf : (double)m;
+  // the list
+  const T* x = static_cast<const T*>(P.logits) + row * P.ld;
+  double z[4], p[4], psum[4], mass = 0;
+  bool lead[4];  // the first entry that lists its id
+  int distinct = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = lane + 32 * i;
+    z[i] = -inf;
+    p[i] = psum[i] = 0;
+    lead[i] = false;
+    if (id[i] >= 0) {
+      z[i] = (double)Vec<T>::load(x + id[i]);
+      p[i] = exp((double)l[i]);
+      lead[i] = true;
+      for (int o = 0; o < P.k; ++o)
+        if (sid[w][o] == id[i]) {
+          if (o < j) lead[i] = false;
+          psum[i] += o == j ? p[i] : exp((double)sp[w][o]);
+        }
+      mass += p[i];
+      distinct += lead[i];
+      if (z[i] > ref || z[i] != z[i]) ref = z[i];
+    }
+  }
+  mass = warp_sum(mass);
+  distinct = (int)__reduce_add_sync(FULL, (unsigned)distinct);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const double t = __shfl_xor_sync(FULL, ref, o);
+    if (t > ref || t != t) ref = t;
+  }
+  double total = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    z[i] = (z[i] - ref) * P.scale_d;
+    if (lead[i]) total += exp2(z[i]);
+  }
+  const double rest = r == 0 ? -inf : ((double)m - ref) * P.scale_d + log2(r);
+  total = warp_sum(total) + (r == 0 ? 0.0 : exp2(rest));
+  const double lse = log2(total);  // of the distances
+  if (lane == 0 && P.status && !(fabs(lse) < inf)) atomicOr(P.status, (int)VINFER_ST_NONFINITE);
+  // target masses
+  double pt = 0, norm = 1, lnorm = 0;
+  if (P.tail) {
+    pt = distinct < P.V ? fmax(0.0, 1.0 - mass) : 0.0;
+  } else if (mass > 0) {
+    norm = 1.0 / mass;
+    lnorm = log(mass);
+    mass = 1.0;
+  }
+  const double qt = r == 0 ? 0.0 : exp2(rest - lse);
+  double loss = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (p[i] > 0) loss += p[i] * norm * (((double)l[i] - lnorm) - (z[i] - lse) * LN2_D);
+  loss = warp_sum(loss);
+  if (pt > 0) loss += pt * (log(pt) - (rest - lse) * LN2_D);
+  if (lse != lse) loss = lse;
+  if (lane == 0) P.loss[row] = (float)(loss * (double)weight);
+  if (!P.stat) return;
+  const double M = mass + pt;
+  if (lane == 0) {
+    Stat t = {0.f, 0.f};
+    if (r != 0) {
+      t.m = m;
+      t.coef = (float)((M * qt - pt) / r);
+    }
+    if (lse != lse) t.m = t.coef = __int_as_float(0x7fffffff);
+    P.stat[row] = t;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = lane + 32 * i;
+    if (j < P.k)
+      P.listg[row * P.k + j] =
+          id[i] >= 0 ? (float)(M * exp2(z[i] - lse) - psum[i] * norm) : 0.f;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
+  using VT = Vec<T>;
+  constexpr int A = VT::A;
+  const int64_t row = blockIdx.x / P.parts;
+  const int part = (int)(blockIdx.x - row * P.parts), tid = threadIdx.x;
+  const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
+  T* out = static_cast<T*>(P.grad) + row * P.ldg;
+  const bool aligned = (int)(((uintptr_t)out & 15) / sizeof(T)) == R.off;
+  const int v0 = (int)((int64_t)R.nv * part / P.parts);
+  const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
+  const float weight = P.weights ? P.weights[row] : 1.f;
+  grid_dependency_wait();
+  const float f =
+      weight == 0.f ? 0.f : weight * P.inv_t * (P.grad_out ? P.grad_out[row] : 1.f);
+  Stat st = {0.f, 0.f};
+  if (f != 0.f) st = P.stat[row];
+  const float coef = f * st.coef;
+  for (int vb = v0; vb < v1; vb += NT * U) {
+    uint4 q[U];
+    if (f != 0.f) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int v = vb + u * NT + tid;
+        if (v < v1) q[u] = R.load(v);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = vb + u * NT + tid;
+      if (v < v1) {
+        float g[A];
+        if (f != 0.f) {
+          VT::unpack(q[u], g);
+#pragma unroll
+          for (int j = 0; j < A; ++j) g[j] = coef * ex2((g[j] - st.m) * P.scale);
+        } else {
+#pragma unroll
+          for (int j = 0; j < A; ++j) g[j] = 0.f;
+        }
+        const int64_t e0 = (int64_t)v * A - R.off;
+        if (aligned && R.whole(v)) {
+          *reinterpret_cast<uint4*>(out + e0) = VT::pack(g);
+        } else {
+#pragma unroll
+          for (int j = 0; j < A; ++j)
+            if (e0 + j >= 0 && e0 + j < P.V) out[e0 + j] = VT::round(g[j]);
+        }
+      }
+    }
+  }
+  if (f == 0.f) return;
+  __syncthreads();  // the listed elements over what was just stored
+  if (tid < P.k) {
+    const int id = P.ids[row * P.k + tid];
+    const int e = id + R.off;
+    if (id >= 0 && id < P.V && e >= v0 * A && e < v1 * A)
+      out[id] = VT::round(f * P.listg[row * P.k + tid]);
+  }
+}
+
+// Parts of a row: enough CTAs to fill the 148 SMs several times over, at least two vectors a
+// thread in each.
+int distill_parts(int64_t rows_, int64_t vocab, int dtype) {
+  const int64_t A = dtype == VINFER_DTYPE_BF16 ? 8 : 4;
+  const int64_t nv = (vocab + A - 1) / A;
+  int64_t p = (148 * 8 + rows_ - 1) / rows_;
+  p = std::min<int64_t>(p, (nv + 2 * NT - 1) / (2 * NT));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(p, MAX_PARTS));
+}
+
+int check(const VinferDistillArgs* a) {
+  if (!a || !a->logits || !a->ids || !a->logprobs) return VINFER_E_ARG;
+  if (a->dtype != VINFER_DTYPE_F32 && a->dtype != VINFER_DTYPE_BF16) return VINFER_E_ARG;
+  if (a->rows < 1 || a->vocab < 1 || a->ld < a->vocab || a->k < 1) return VINFER_E_ARG;
+  if (!(a->temperature > 0.f) || !(a->temperature < INFINITY)) return VINFER_E_ARG;
+  if (((uintptr_t)a->logits) % (a->dtype == VINFER_DTYPE_BF16 ? 2 : 4)) return VINFER_E_ARG;
+  if (a->vocab > VINFER_MAX_VOCAB || a->rows > VINFER_DISTILL_MAX_ROWS || a->k > MAXK)
+    return VINFER_E_LIMIT;
+  return VINFER_OK;
+}
+
+DistP params(const VinferDistillArgs* a) {
+  DistP P = {};
+  P.logits = a->logits;
+  P.ld = a->ld;
+  P.rows = a->rows;
+  P.V = (int)a->vocab;
+  P.k = a->k;
+  P.parts = distill_parts(a->rows, a->vocab, a->dtype);
+  P.tail = a->tail != 0;
+  P.scale_d = L2E_D / (double)a->temperature;
+  P.scale = (float)P.scale_d;
+  P.inv_t = 1.f / a->temperature;
+  P.ids = a->ids;
+  P.lp = a->logprobs;
+  P.weights = a->weights;
+  P.status = a->status;
+  return P;
+}
+
+template <typename T>
+int launch_loss(const DistP& P, cudaStream_t st) {
+  const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, 0, st, false, P);
+  if (rc != VINFER_OK) return rc;
+  return launch(k_distill_finish<T>, (unsigned)((P.rows + NW - 1) / NW), NT, 0, st, true, P);
+}
+
+template <typename T>
+int launch_grad(const DistP& P, cudaStream_t st, bool dependent) {
+  return launch(k_distill_grad<T>, (unsigned)(P.rows * P.parts), NT, 0, st, dependent, P);
+}
+
+size_t align_up(size_t n) { return (n + 255) / 256 * 256; }
+
+bool grad_ok(const VinferDistillArgs* a, const void* grad, int64_t ld_grad) {
+  return grad && ld_grad >= a->vocab && ((uintptr_t)grad) % (a->dtype == VINFER_DTYPE_BF16 ? 2 : 4) == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t vinfer_distill_workspace_bytes(int64_t rows_, int64_t vocab, int32_t dtype, int32_t k) {
+  if (rows_ < 1 || rows_ > VINFER_DISTILL_MAX_ROWS || vocab < 1 || vocab > VINFER_MAX_VOCAB ||
+      k < 1 || k > MAXK || (dtype != VINFER_DTYPE_F32 && dtype != VINFER_DTYPE_BF16))
+    return 0;
+  return align_up((size_t)rows_ * distill_parts(rows_, vocab, dtype) * sizeof(Part)) +
+         align_up((size_t)rows_ * sizeof(Stat)) + (size_t)rows_ * k * sizeof(float);
+}
+
+int vinfer_distill_loss(const VinferDistillArgs* a, float* loss, float* row_stats,
+                        float* list_grads, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  NvtxRange nvtx_range("vinfer_distill_loss");
+  const int rc = check(a);
+  if (rc != VINFER_OK) return rc;
+  if (!loss || !row_stats != !list_grads || !workspace) return VINFER_E_ARG;
+  if (((uintptr_t)workspace) % 16 || ((uintptr_t)row_stats) % 8) return VINFER_E_ARG;
+  if (workspace_bytes < vinfer_distill_workspace_bytes(a->rows, a->vocab, a->dtype, a->k))
+    return VINFER_E_LIMIT;
+  DistP P = params(a);
+  P.part = static_cast<Part*>(workspace);
+  P.loss = loss;
+  P.stat = reinterpret_cast<Stat*>(row_stats);
+  P.listg = list_grads;
+  cudaStream_t st = (cudaStream_t)stream;
+  return a->dtype == VINFER_DTYPE_BF16 ? launch_loss<__nv_bfloat16>(P, st)
+                                       : launch_loss<float>(P, st);
+}
+
+int vinfer_distill_grad(const VinferDistillArgs* a, const float* row_stats,
+                        const float* list_grads, const float* grad_out, void* grad,
+                        int64_t ld_grad, void* stream) {
+  NvtxRange nvtx_range("vinfer_distill_grad");
+  const int rc = check(a);
+  if (rc != VINFER_OK) return rc;
+  if (!row_stats || !list_grads || !grad_ok(a, grad, ld_grad)) return VINFER_E_ARG;
+  if (((uintptr_t)row_stats) % 8) return VINFER_E_ARG;
+  DistP P = params(a);
+  P.stat = reinterpret_cast<Stat*>(const_cast<float*>(row_stats));
+  P.listg = const_cast<float*>(list_grads);
+  P.grad_out = grad_out;
+  P.grad = grad;
+  P.ldg = ld_grad;
+  cudaStream_t st = (cudaStream_t)stream;
+  return a->dtype == VINFER_DTYPE_BF16 ? launch_grad<__nv_bfloat16>(P, st, false)
+                                       : launch_grad<float>(P, st, false);
+}
+
+int vinfer_distill_step(const VinferDistillArgs* a, float* loss, void* grad, int64_t ld_grad,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  NvtxRange nvtx_range("vinfer_distill_step");
+  int rc = check(a);
+  if (rc != VINFER_OK) return rc;
+  if (!loss || !grad_ok(a, grad, ld_grad) || !workspace) return VINFER_E_ARG;
+  if (((uintptr_t)workspace) % 16) return VINFER_E_ARG;
+  if (workspace_bytes < vinfer_distill_workspace_bytes(a->rows, a->vocab, a->dtype, a->k))
+    return VINFER_E_LIMIT;
+  DistP P = params(a);
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  P.part = reinterpret_cast<Part*>(ws);
+  ws += align_up((size_t)P.rows * P.parts * sizeof(Part));
+  P.stat = reinterpret_cast<Stat*>(ws);
+  ws += align_up((size_t)P.rows * sizeof(Stat));
+  P.listg = reinterpret_cast<float*>(ws);
+  P.loss = loss;
+  P.grad = grad;
+  P.ldg = ld_grad;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (a->dtype == VINFER_DTYPE_BF16) {
+    rc = launch_loss<__nv_bfloat16>(P, st);
+    return rc != VINFER_OK ? rc : launch_grad<__nv_bfloat16>(P, st, true);
+  }
+  rc = launch_loss<float>(P, st);
+  return rc != VINFER_OK ? rc : launch_grad<float>(P, st, true);
+}
+
+}  // extern "C"

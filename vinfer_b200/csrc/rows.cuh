@@ -1,0 +1,292 @@
+// rows.cuh — reading rows of logits: 16-byte vectors at any element alignment, exponentials in
+// base 2, and warp and block helpers shared by the kernels beside the sampler.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <float.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <nvtx3/nvToolsExt.h>
+
+#include "vinfer_sampler.h"
+
+namespace rows {
+
+constexpr unsigned FULL = 0xffffffffu;
+constexpr float L2E = 1.4426950408889634f;      // log2(e) rounded to float
+constexpr double L2E_D = 1.4426950408889634074;  // log2(e)
+constexpr double LN2_D = 0.69314718055994530942;
+
+__device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
+
+// 2^x by the hardware's approximation (2 ulp; 0 below the normal range)
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// order-preserving key of a float; -0 folds into +0
+__device__ __forceinline__ uint32_t okey(float v) {
+  const uint32_t b = __float_as_uint(__fadd_rn(v, 0.0f));
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float from_okey(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
+}
+
+// 16 bytes of logits as floats
+template <typename T>
+struct Vec;
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int A = 8;
+  static constexpr uint32_t NEG_INF_WORD = 0xff80ff80u;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&f)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  // largest element, NaN ignored (two packed comparisons a word pair)
+  static __device__ __forceinline__ float max(const uint4& q) {
+    __nv_bfloat162 a, b, c, d;
+    memcpy(&a, &q.x, 4);
+    memcpy(&b, &q.y, 4);
+    memcpy(&c, &q.z, 4);
+    memcpy(&d, &q.w, 4);
+    const __nv_bfloat162 m = __hmax2(__hmax2(a, b), __hmax2(c, d));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ float get(const uint4& q, int j) {
+    const uint32_t w = j < 4 ? (j < 2 ? q.x : q.y) : (j < 6 ? q.z : q.w);
+    return __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));
+  }
+  static __device__ __forceinline__ void put(uint4& q, int j, uint32_t bits) {
+    const uint32_t keep = (j & 1) ? 0x0000ffffu : 0xffff0000u;
+    const uint32_t add = (j & 1) ? bits << 16 : bits & 0xffffu;
+    if (j < 2) q.x = (q.x & keep) | add;
+    else if (j < 4) q.y = (q.y & keep) | add;
+    else if (j < 6) q.z = (q.z & keep) | add;
+    else q.w = (q.w & keep) | add;
+  }
+  static __device__ __forceinline__ uint32_t bits(const __nv_bfloat16* p) {
+    return *reinterpret_cast<const unsigned short*>(p);
+  }
+  static constexpr uint32_t NEG_INF_BITS = 0xff80u;
+  static __device__ __forceinline__ float load(const __nv_bfloat16* p) {
+    return __bfloat162float(*p);
+  }
+  static __device__ __forceinline__ __nv_bfloat16 round(float f) { return __float2bfloat16_rn(f); }
+  // rounded to nearest even, the gradient's type
+  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      memcpy(&w[i], &h, 4);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+template <>
+struct Vec<float> {
+  static constexpr int A = 4;
+  static constexpr uint32_t NEG_INF_WORD = 0xff800000u;
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&f)[4]) {
+    f[0] = __uint_as_float(q.x);
+    f[1] = __uint_as_float(q.y);
+    f[2] = __uint_as_float(q.z);
+    f[3] = __uint_as_float(q.w);
+  }
+  static __device__ __forceinline__ float max(const uint4& q) {
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)),
+                 fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+  }
+  static __device__ __forceinline__ float get(const uint4& q, int j) {
+    return __uint_as_float(j < 2 ? (j == 0 ? q.x : q.y) : (j == 2 ? q.z : q.w));
+  }
+  static __device__ __forceinline__ void put(uint4& q, int j, uint32_t bits) {
+    if (j == 0) q.x = bits;
+    else if (j == 1) q.y = bits;
+    else if (j == 2) q.z = bits;
+    else q.w = bits;
+  }
+  static __device__ __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(*p); }
+  static constexpr uint32_t NEG_INF_BITS = 0xff800000u;
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ float round(float f) { return f; }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                      __float_as_uint(f[3]));
+  }
+};
+
+// A row cut into aligned 16-byte vectors: vector v holds elements [v * A - off, v * A - off + A).
+// The first and the last one may hold elements outside the row; those are never read.
+template <typename T>
+struct Row {
+  const T* p;  // the row's first element
+  int off;     // elements between the aligned address below p and p
+  int V;
+  int nv;      // vectors that hold an element of the row
+  __device__ __forceinline__ Row(const T* p_, int V_) : p(p_), V(V_) {
+    off = (int)(((uintptr_t)p & 15) / sizeof(T));
+    nv = (V + off + Vec<T>::A - 1) / Vec<T>::A;
+  }
+  __device__ __forceinline__ bool whole(int v) const {
+    const int e = v * Vec<T>::A - off;
+    return e >= 0 && e + Vec<T>::A <= V;
+  }
+  // vector v; elements outside the row read as -inf
+  __device__ __forceinline__ uint4 load(int v) const {
+    if (whole(v)) {
+      uint4 q;
+      asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w)
+                   : "l"(p + ((int64_t)v * Vec<T>::A - off)));
+      return q;
+    }
+    return edge(p, V, v * Vec<T>::A - off);
+  }
+  // the vector whose first element is e0, element by element
+  static __device__ __noinline__ uint4 edge(const T* p, int V, int e0) {
+    const uint32_t n = Vec<T>::NEG_INF_WORD;
+    uint4 q = make_uint4(n, n, n, n);
+    for (int j = 0; j < Vec<T>::A; ++j)
+      if (e0 + j >= 0 && e0 + j < V) Vec<T>::put(q, j, Vec<T>::bits(p + e0 + j));
+    return q;
+  }
+};
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
+  return v;
+}
+__device__ __forceinline__ double warp_sum(double v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+  return v;
+}
+
+// Softmax sums are held as (m, s): s in units of 2^(m * scale), m the largest logit summed, scale =
+// log2(e) / temperature rounded to float. m stays a logit, so sums of rows at the type's lowest
+// value (a mask) need no exponent beyond the float's range, and the rounding of `scale` only
+// stretches distances from the maximum.
+
+// Adds the U vectors q, whose largest element is mx, to the thread's sum. One multiply-add, one
+// ex2 and one addition an element: the argument x * scale - c is rounded once, and what c misses
+// of m * scale is put right in the round's sum.
+template <typename T, int U>
+__device__ __forceinline__ void add_exps(const uint4 (&q)[U], float mx, float scale, float& m,
+                                         float& s) {
+  if (mx > m) {
+    if (s != 0.f) s *= ex2((m - mx) * scale);
+    m = mx;
+  }
+  const float ref = m == neg_inf() ? 0.f : m;  // only -inf so far (or NaN, which the sum shows)
+  const float c = ref * scale;
+  float sum = 0.f;
+  if (fabsf(c) < 1e37f) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float f[Vec<T>::A];
+      Vec<T>::unpack(q[u], f);
+      float t = 0.f;
+#pragma unroll
+      for (int j = 0; j < Vec<T>::A; ++j) t += ex2(fmaf(f[j], scale, -c));
+      sum += t;
+    }
+    const float lo = fmaf(ref, scale, -c);
+    sum = fmaf(sum, -lo * (float)LN2_D, sum);
+  } else {  // c near the float's range, or infinite: distances first
+#pragma unroll 1
+    for (int u = 0; u < U; ++u) {
+      uint4 v = q[0];
+#pragma unroll
+      for (int i = 1; i < U; ++i)
+        if (i == u) v = q[i];
+      for (int j = 0; j < Vec<T>::A; ++j) sum += ex2((Vec<T>::get(v, j) - ref) * scale);
+    }
+  }
+  s += sum;
+}
+
+// Joins the sums of a block's threads: every thread gets the block's. Fixed order: the result does
+// not depend on timing. `sm`: 2 * NW floats.
+template <int NW>
+__device__ __forceinline__ void block_join(float& m, float& s, float scale, float* sm) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  if (s == 0.f) m = neg_inf();
+  const float mw = warp_max(m);
+  float sw = s == 0.f ? 0.f : s * ex2((m - mw) * scale);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sw += __shfl_xor_sync(FULL, sw, o);
+  if (lane == 0) {
+    sm[w] = mw;
+    sm[NW + w] = sw;
+  }
+  __syncthreads();
+  float mb = sm[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) mb = fmaxf(mb, sm[i]);
+  float sb = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) sb += sm[NW + i] == 0.f ? 0.f : sm[NW + i] * ex2((sm[i] - mb) * scale);
+  m = mb;
+  s = sb;
+  __syncthreads();
+}
+
+__device__ __forceinline__ void grid_dependency_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// An NVTX range over one entry point's host work.
+struct NvtxRange {
+  explicit NvtxRange(const char* name) { nvtxRangePushA(name); }
+  ~NvtxRange() { nvtxRangePop(); }
+  NvtxRange(const NvtxRange&) = delete;
+  NvtxRange& operator=(const NvtxRange&) = delete;
+};
+
+// An error code for the caller; the runtime's own error state is cleared, so that a refused launch
+// does not show up in somebody else's check.
+inline int result(cudaError_t e) {
+  if (e == cudaSuccess) return VINFER_OK;
+  (void)cudaGetLastError();
+  return VINFER_E_CUDA;
+}
+
+// Shared memory above 48 KB, static included (below 4 KB here), has to be asked for (a host-side
+// setting of the kernel on the current device, no work on a stream).
+template <typename K>
+int opt_in(K kern, size_t smem) {
+  if (smem <= 44 * 1024) return VINFER_OK;
+  return result(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+}
+
+// One launch; `dependent`: may begin while the stream's kernel before it drains (that kernel's
+// writes are read behind grid_dependency_wait()).
+template <typename... KA, typename... A>
+int launch(void (*kern)(KA...), unsigned grid, unsigned block, size_t smem, cudaStream_t st,
+           bool dependent, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return result(cudaLaunchKernelEx(&cfg, kern, args...));
+}
+
+}  // namespace rows

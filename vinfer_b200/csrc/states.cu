@@ -1,0 +1,205 @@
+// states.cu — decode states follow the beams: slot s takes the state of slot parents[s] (sm_100a).
+//
+// A state is a tensor with a slot dimension (token counts, recurrent and convolution states,
+// key/value caches); the host describes it as runs of contiguous bytes under up to three outer
+// dimensions. One launch copies the moved slots of up to MAX_STATES tensors.
+//
+// In place, a slot may only take the state of a slot that keeps its own (parents[parents[s]] ==
+// parents[s], as vinfer_beam_select lays beams out): sources are then never written, so the copies
+// need no order and no second buffer. Into another buffer any slot may take any slot's state.
+//
+// Copies are bound by HBM: each distinct source is read from HBM once (the copies of one chunk of
+// a state run side by side, so a source's other readers find it in L2) and each moved slot written
+// once. Slots that stay cost nothing but their entry of the list of moves.
+#include "rows.cuh"
+
+#include <algorithm>
+
+namespace {
+
+using namespace rows;
+
+constexpr int NT = 256;
+constexpr int UV = 4;           // vectors a thread copies per item, all loads before the stores
+constexpr int MAX_STATES = 64;  // tensors of one launch (they travel as kernel parameters)
+constexpr int OUTER = VINFER_STATE_MAX_OUTER;
+
+struct Desc {
+  const unsigned char* src;
+  unsigned char* dst;
+  int64_t src_slot, dst_slot;   // byte strides of the slot dimension
+  int64_t size[OUTER], src_st[OUTER], dst_st[OUTER];
+  int64_t run;                  // contiguous bytes
+  int64_t vecs;                 // vectors of one slot: outer sizes x run / vec
+  int64_t chunks;               // items of one moved slot
+  int64_t unit;                 // bytes of one position of the run, 0: lengths do not cut the run
+  int64_t len_max;              // positions along the length dimension
+  int32_t len_outer;            // the outer dimension that lengths cut, -1: none
+  int32_t vec;                  // bytes of a vector: 16, 8, 4, 2 or 1
+};
+
+struct StatesP {
+  Desc d[MAX_STATES];
+  int n;
+  int slots, in_place;
+  const int* parents;
+  const int* lengths;
+  int* status;
+};
+
+template <typename VT>
+__device__ __forceinline__ void copy_item(const Desc& D, int from, int to, int64_t chunk, int len) {
+  const unsigned char* src = D.src + (int64_t)from * D.src_slot;
+  unsigned char* dst = D.dst + (int64_t)to * D.dst_slot;
+  const int64_t run_vecs = D.run / (int64_t)sizeof(VT);
+  const int64_t end = D.unit ? (int64_t)len * D.unit : D.run;  // live bytes of a run
+  VT v[UV];
+  int64_t at[UV];
+#pragma unroll
+  for (int u = 0; u < UV; ++u) {
+    const int64_t i = (chunk * UV + u) * NT + threadIdx.x;
+    at[u] = -1;
+    if (i < D.vecs) {
+      int64_t o = i / run_vecs;
+      const int64_t r = (i - o * run_vecs) * (int64_t)sizeof(VT);
+      int64_t so = r, po = r;
+      bool live = r < end;
+#pragma unroll
+      for (int k = OUTER - 1; k >= 0; --k) {
+        const int64_t q = o / D.size[k], x = o - q * D.size[k];
+        o = q;
+        so += x * D.src_st[k];
+        po += x * D.dst_st[k];
+        if (k == D.len_outer) live = live && x < len;
+      }
+      if (live) {
+        v[u] = *reinterpret_cast<const VT*>(src + so);
+        at[u] = po;
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < UV; ++u)
+    if (at[u] >= 0) *reinterpret_cast<VT*>(dst + at[u]) = v[u];
+}
+
+// Dynamic shared memory: one packed move (source << 16 | slot) a slot.
+__global__ void __launch_bounds__(NT) k_reorder(const __grid_constant__ StatesP P) {
+  extern __shared__ uint32_t moves[];
+  __shared__ int wcnt[NT / 32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int M = 0;  // the slots that move, ascending: every CTA makes the same list
+  for (int s0 = 0; s0 < P.slots; s0 += NT) {
+    const int s = s0 + threadIdx.x;
+    bool move = false;
+    int p = 0;
+    if (s < P.slots) {
+      p = P.parents[s];
+      const bool ok = p >= 0 && p < P.slots && (!P.in_place || p == s || P.parents[p] == p);
+      if (!ok && P.status && blockIdx.x == 0) atomicOr(P.status, (int)VINFER_ST_BAD_PARENT);
+      move = ok && (!P.in_place || p != s);
+    }
+    const unsigned m = __ballot_sync(FULL, move);
+    if (lane == 0) wcnt[w] = __popc(m);
+    __syncthreads();
+    int at = M + __popc(m & ((1u << lane) - 1));
+    for (int i = 0; i < NT / 32; ++i) {
+      if (i < w) at += wcnt[i];
+      M += wcnt[i];
+    }
+    if (move) moves[at] = (uint32_t)p << 16 | (uint32_t)s;
+    __syncthreads();
+  }
+  // items: the moves of a chunk side by side, chunk after chunk, tensor after tensor
+  int64_t g = blockIdx.x;
+  for (int t = 0; t < P.n; ++t) {
+    const Desc& D = P.d[t];
+    const int64_t items = D.chunks * M;
+    for (; g < items; g += gridDim.x) {
+      const int64_t chunk = g / M;
+      const uint32_t mv = moves[g - chunk * M];
+      const int from = mv >> 16, to = mv & 0xffff;
+      int len = 0;
+      if (D.unit || D.len_outer >= 0)
+        len = (int)min((int64_t)max(P.lengths[to], 0), D.len_max);
+      switch (D.vec) {
+        case 16: copy_item<uint4>(D, from, to, chunk, len); break;
+        case 8: copy_item<uint2>(D, from, to, chunk, len); break;
+        case 4: copy_item<uint32_t>(D, from, to, chunk, len); break;
+        case 2: copy_item<uint16_t>(D, from, to, chunk, len); break;
+        default: copy_item<uint8_t>(D, from, to, chunk, len); break;
+      }
+    }
+    g -= items;
+  }
+}
+
+}  // namespace
+
+extern "C" int vinfer_reorder_states(const VinferState* states, int32_t n_states,
+                                     const int32_t* parents, int64_t slots,
+                                     const int32_t* lengths, int32_t* status, void* stream) {
+  NvtxRange nvtx_range("vinfer_reorder_states");
+  if (!states || n_states < 1 || !parents || slots < 1) return VINFER_E_ARG;
+  if (slots > VINFER_STATE_MAX_SLOTS) return VINFER_E_LIMIT;
+  const bool in_place = states[0].src == states[0].dst;
+  for (int i = 0; i < n_states; ++i) {
+    const VinferState& s = states[i];
+    if (!s.src || !s.dst || s.run_bytes < 1 || s.n_outer < 0 || s.n_outer > OUTER) return VINFER_E_ARG;
+    if ((s.src == s.dst) != in_place || s.len_outer < -1 || s.len_outer >= s.n_outer) return VINFER_E_ARG;
+    if (s.len_unit_bytes < 0 || (s.len_unit_bytes > 0 && (s.run_bytes % s.len_unit_bytes || s.len_outer >= 0)))
+      return VINFER_E_ARG;
+    if ((s.len_unit_bytes > 0 || s.len_outer >= 0) && !lengths) return VINFER_E_ARG;
+    for (int k = 0; k < s.n_outer; ++k)
+      if (s.outer_size[k] < 1) return VINFER_E_ARG;
+  }
+  for (int i0 = 0; i0 < n_states; i0 += MAX_STATES) {
+    StatesP P = {};
+    P.n = std::min(MAX_STATES, n_states - i0);
+    P.slots = (int)slots;
+    P.in_place = in_place;
+    P.parents = parents;
+    P.lengths = lengths;
+    P.status = status;
+    int64_t chunks = 0;
+    for (int i = 0; i < P.n; ++i) {
+      const VinferState& s = states[i0 + i];
+      Desc& D = P.d[i];
+      D.src = static_cast<const unsigned char*>(s.src);
+      D.dst = static_cast<unsigned char*>(s.dst);
+      D.src_slot = s.src_slot_stride;
+      D.dst_slot = s.dst_slot_stride;
+      D.run = s.run_bytes;
+      D.unit = s.len_unit_bytes;
+      D.len_outer = -1;
+      uint64_t bits = (uint64_t)(uintptr_t)s.src | (uint64_t)(uintptr_t)s.dst |
+                      (uint64_t)s.src_slot_stride | (uint64_t)s.dst_slot_stride |
+                      (uint64_t)s.run_bytes | (uint64_t)s.len_unit_bytes | 16;
+      D.len_max = D.unit ? s.run_bytes / D.unit : 0;
+      int64_t outer = 1;
+      for (int k = 0; k < OUTER; ++k) {  // the dimensions given, behind ones of size 1
+        const int from = k - (OUTER - s.n_outer);
+        D.size[k] = from >= 0 ? s.outer_size[from] : 1;
+        D.src_st[k] = from >= 0 ? s.src_outer_stride[from] : 0;
+        D.dst_st[k] = from >= 0 ? s.dst_outer_stride[from] : 0;
+        if (from >= 0 && from == s.len_outer) {
+          D.len_outer = k;
+          D.len_max = D.size[k];
+        }
+        bits |= (uint64_t)D.src_st[k] | (uint64_t)D.dst_st[k];
+        outer *= D.size[k];
+      }
+      D.vec = (int)(bits & (~bits + 1));  // the lowest set bit divides every address and size
+      D.vecs = outer * (s.run_bytes / D.vec);
+      D.chunks = (D.vecs + (int64_t)NT * UV - 1) / ((int64_t)NT * UV);
+      chunks += D.chunks;
+    }
+    // every slot may move: no more CTAs than items, eight of 256 threads an SM at most
+    const int64_t grid = std::min<int64_t>(148 * 8, chunks * slots);
+    const size_t smem = (size_t)slots * 4;
+    if (opt_in(k_reorder, smem) != VINFER_OK) return VINFER_E_CUDA;
+    const int rc = launch(k_reorder, (unsigned)grid, NT, smem, (cudaStream_t)stream, false, P);
+    if (rc != VINFER_OK) return rc;
+  }
+  return VINFER_OK;
+}

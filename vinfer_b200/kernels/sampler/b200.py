@@ -15,10 +15,13 @@ from vinfer_b200 import _lib
 from vinfer_b200.kernels.sampler.base import SAMPLER
 from vinfer_b200.registry import BackendContext
 from vinfer_b200.sampling import (
+    BeamStep,
+    DecodeStates,
     RowParams,
     SamplingParams,
     SlotHistogram,
     TokenHistogram,
+    _overlap,
     position_uniform,
 )
 
@@ -213,6 +216,201 @@ class B200Sampler:
                                                  ws.data_ptr(), ws.numel(), self._stream()),
                    "vinfer_sample_decode")
         return out
+
+    # ---- beam search ---------------------------------------------------------------------------
+    def _call(self, fn, what: str, *args) -> None:
+        """``fn(*args, current stream)`` with the backend's device current."""
+        if torch.cuda.current_device() == self.device.index:
+            _lib.check(fn(*args, self._stream()), what)
+        else:
+            with torch.cuda.device(self.device):
+                _lib.check(fn(*args, self._stream()), what)
+
+    def _rows(self, logits: torch.Tensor) -> tuple[int, int, int]:
+        """(rows, vocabulary, row stride) of checked logits."""
+        if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+            raise ValueError("logits must be [rows, vocab] with unit column stride")
+        if logits.dtype not in _DTYPES:
+            raise ValueError(f"logits dtype {logits.dtype} is not supported (float32, bfloat16)")
+        if logits.device != self.device:
+            raise ValueError(f"logits are on {logits.device}, backend on {self.device}")
+        n, v = logits.shape
+        if not 1 <= v <= _lib.MAX_VOCAB:
+            raise ValueError(f"the vocabulary must have 1 to {_lib.MAX_VOCAB} tokens, got {v}")
+        ld = logits.stride(0) if n > 1 else v
+        if ld < v:
+            raise ValueError("rows of logits must not overlap")
+        return n, v, ld
+
+    def _vector(self, name: str, t: torch.Tensor, dtype: torch.dtype, *shape: int) -> int:
+        if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.device != self.device:
+            raise ValueError(f"{name} must be a contiguous {dtype} {list(shape)} on {self.device}")
+        return t.data_ptr()
+
+    def beam_select(self, logits: torch.Tensor, scores: torch.Tensor, n: int | None = None,
+                    eos: torch.Tensor | None = None, out: BeamStep | None = None) -> BeamStep:
+        """One step of beam search for R requests of W beams: ``logits`` ``[R * W, vocab]``,
+        ``scores`` ``[R, W]`` (float32, accumulated log-probabilities; -inf: a dead beam, whose
+        row is not read). Lists each request's ``n`` best continuations over beams and
+        vocabulary (descending score; ties by beam, then token) and lays the W best that do not
+        end in one of ``eos`` (int32 stop ids on the device) into its slots: the best child of a
+        beam stays in the beam's slot, so ``reorder_states`` only copies the others. ``n``
+        defaults to ``W * (1 + len(eos))``, which always finds W. ``out.next_scores`` may be
+        ``scores``. Nothing leaves the device."""
+        rows, v, ld = self._rows(logits)
+        if scores.dim() != 2 or scores.shape[0] * scores.shape[1] != rows:
+            raise ValueError(f"scores must be [requests, beams] for {rows} rows of logits")
+        r, w = scores.shape
+        if not 1 <= w <= _lib.BEAM_MAX_WIDTH:
+            raise ValueError(f"1 to {_lib.BEAM_MAX_WIDTH} beams are supported, got {w}")
+        if rows > _lib.MAX_BATCH:
+            raise ValueError(f"at most {_lib.MAX_BATCH} rows are supported, got {rows}")
+        stops = 0 if eos is None else eos.numel()
+        if stops > _lib.BEAM_MAX_EOS:
+            raise ValueError(f"at most {_lib.BEAM_MAX_EOS} stop ids are supported, got {stops}")
+        if n is None:
+            n = min(w * (1 + stops), _lib.BEAM_MAX_N)
+        if not 1 <= n <= _lib.BEAM_MAX_N:
+            raise ValueError(f"n must be in [1, {_lib.BEAM_MAX_N}], got {n}")
+        a = _lib.BeamArgs()
+        a.scores = self._vector("scores", scores, torch.float32, r, w)
+        if out is None:
+            out = BeamStep.empty(r, w, n, self.device)
+        else:
+            for name, dt, m in (("scores", torch.float32, n), ("beams", torch.int32, n),
+                                ("tokens", torch.int32, n), ("next_scores", torch.float32, w),
+                                ("parents", torch.int32, w), ("next_tokens", torch.int32, w)):
+                self._vector(f"out.{name}", getattr(out, name), dt, r, m)
+        if stops:
+            a.eos = self._vector("eos", eos, torch.int32, stops)
+        if r == 0:
+            return out
+        a.logits, a.dtype, a.beams = logits.data_ptr(), _DTYPES[logits.dtype], w
+        a.requests, a.vocab, a.ld, a.n_eos, a.n = r, v, ld, stops, n
+        a.out_scores, a.out_beams = out.scores.data_ptr(), out.beams.data_ptr()
+        a.out_tokens, a.next_scores = out.tokens.data_ptr(), out.next_scores.data_ptr()
+        a.parents, a.next_tokens = out.parents.data_ptr(), out.next_tokens.data_ptr()
+        a.status = self.status.data_ptr()
+        nbytes = self.lib.vinfer_beam_workspace_bytes(r, w, v, a.dtype, n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        self._call(self.lib.vinfer_beam_select, "vinfer_beam_select", C.byref(a), ws.data_ptr(),
+                   nbytes)
+        return out
+
+    def reorder_states(self, states: DecodeStates, parents: torch.Tensor,
+                       lengths: torch.Tensor | None = None) -> None:
+        """Slot ``s`` of every state takes the contents of slot ``parents[s]`` (int32, one for each
+        slot, any shape: ``BeamStep.parents``). In place a moved slot's parent must keep its own
+        state, as ``beam_select`` lays beams out; into ``out`` tensors any parent will do. With
+        a ``length_dim``, only the first ``lengths[s]`` (int32) positions are copied. A parent
+        out of range, or one that moves itself, leaves the slot alone and sets a status bit."""
+        if states.device != self.device:
+            raise ValueError(f"states are on {states.device}, backend on {self.device}")
+        for name, t in (("parents", parents), ("lengths", lengths)):
+            if t is not None and (t.dtype != torch.int32 or t.numel() != states.slots
+                                  or not t.is_contiguous() or t.device != self.device):
+                raise ValueError(f"{name} must be a contiguous int32 of {states.slots} slots on "
+                                 f"{self.device}")
+        if (lengths is not None) != states.has_lengths:
+            raise ValueError("lengths and a length_dim of the states go together")
+        if states.count == 0:
+            return
+        self._call(self.lib.vinfer_reorder_states, "vinfer_reorder_states", states.array,
+                   states.count, parents.data_ptr(), states.slots, _ptr(lengths),
+                   self.status.data_ptr())
+
+    # ---- distillation ---------------------------------------------------------------------------
+    def _distill_args(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                      weights: torch.Tensor | None, temperature: float,
+                      tail: bool) -> _lib.DistillArgs:
+        n, v, ld = self._rows(logits)
+        if n > _lib.DISTILL_MAX_ROWS:
+            raise ValueError(f"at most {_lib.DISTILL_MAX_ROWS} rows are supported, got {n}")
+        k = ids.shape[1] if ids.dim() == 2 else 0
+        if not 1 <= k <= _lib.DISTILL_MAX_K:
+            raise ValueError(f"ids must be [rows, k] with k in [1, {_lib.DISTILL_MAX_K}]")
+        if not 0 < temperature < float("inf"):
+            raise ValueError(f"temperature must be finite and > 0, got {temperature}")
+        a = _lib.DistillArgs()
+        a.ids = self._vector("ids", ids, torch.int32, n, k)
+        a.logprobs = self._vector("logprobs", logprobs, torch.float32, n, k)
+        if weights is not None:
+            a.weights = self._vector("weights", weights, torch.float32, n)
+        a.logits, a.dtype, a.k = logits.data_ptr(), _DTYPES[logits.dtype], k
+        a.rows, a.vocab, a.ld = n, v, ld
+        a.temperature, a.tail = temperature, bool(tail)
+        a.status = self.status.data_ptr()
+        return a
+
+    def _grad_like(self, logits: torch.Tensor, ld: int) -> torch.Tensor:
+        """The gradient's tensor, with the logits' row stride where that is a padded one, so that
+        rows of both are aligned alike."""
+        n, v = logits.shape
+        if v < ld <= 2 * v:
+            return torch.empty(n, ld, dtype=logits.dtype, device=self.device)[:, :v]
+        return torch.empty(n, v, dtype=logits.dtype, device=self.device)
+
+    def distill_loss(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                     weights: torch.Tensor | None = None, *, temperature: float = 1.0,
+                     tail: bool = False, for_grad: bool = False
+                     ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+        """The rows' distillation losses (float32 ``[rows]``), and with ``for_grad`` what
+        ``distill_grad`` needs (row statistics ``[rows, 2]``, the list's gradients
+        ``[rows, k]``). ``vinfer_b200.distill.distillation_loss`` is the differentiable form."""
+        a = self._distill_args(logits, ids, logprobs, weights, temperature, tail)
+        loss = torch.empty(a.rows, dtype=torch.float32, device=self.device)
+        stats = lists = None
+        if for_grad:
+            stats = torch.empty(a.rows, 2, dtype=torch.float32, device=self.device)
+            lists = torch.empty(a.rows, a.k, dtype=torch.float32, device=self.device)
+        if a.rows:
+            nbytes = self.lib.vinfer_distill_workspace_bytes(a.rows, a.vocab, a.dtype, a.k)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            self._call(self.lib.vinfer_distill_loss, "vinfer_distill_loss", C.byref(a),
+                       loss.data_ptr(), _ptr(stats), _ptr(lists), ws.data_ptr(), nbytes)
+        return loss, stats, lists
+
+    def distill_grad(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                     weights: torch.Tensor | None, stats: torch.Tensor, lists: torch.Tensor,
+                     grad_out: torch.Tensor | None = None, *, temperature: float = 1.0,
+                     tail: bool = False) -> torch.Tensor:
+        """The gradient of ``sum(grad_out * loss)`` with respect to the logits, of their type
+        (``grad_out``: float32 ``[rows]``, None for ones)."""
+        a = self._distill_args(logits, ids, logprobs, weights, temperature, tail)
+        sp = self._vector("stats", stats, torch.float32, a.rows, 2)
+        lp = self._vector("lists", lists, torch.float32, a.rows, a.k)
+        gp = None if grad_out is None else self._vector("grad_out", grad_out, torch.float32, a.rows)
+        grad = self._grad_like(logits, a.ld)
+        if a.rows:
+            self._call(self.lib.vinfer_distill_grad, "vinfer_distill_grad", C.byref(a), sp, lp, gp,
+                       grad.data_ptr(), grad.stride(0) if a.rows > 1 else a.vocab)
+        return grad
+
+    def distill_step(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                     weights: torch.Tensor | None = None, *, temperature: float = 1.0,
+                     tail: bool = False, out: torch.Tensor | None = None
+                     ) -> tuple[torch.Tensor, torch.Tensor]:
+        """The rows' losses and the gradient of their sum with respect to the logits in one call,
+        for a training step whose row weights are known ahead (``logits.backward(grad)``
+        carries on). ``out`` receives the gradient; it may be ``logits`` itself, whose memory
+        the step then reuses."""
+        a = self._distill_args(logits, ids, logprobs, weights, temperature, tail)
+        if out is None:
+            out = self._grad_like(logits, a.ld)
+        elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != self.device or \
+                (out.stride(1) != 1 and a.vocab > 1) or (a.rows > 1 and out.stride(0) < a.vocab):
+            raise ValueError("out must have the logits' shape and type, with unit column stride")
+        loss = torch.empty(a.rows, dtype=torch.float32, device=self.device)
+        if a.rows:
+            if out.data_ptr() != logits.data_ptr() or (a.rows > 1 and out.stride(0) != a.ld):
+                if _overlap(logits, out):
+                    raise ValueError("out must be the logits themselves or not overlap them")
+            nbytes = self.lib.vinfer_distill_workspace_bytes(a.rows, a.vocab, a.dtype, a.k)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+            self._call(self.lib.vinfer_distill_step, "vinfer_distill_step", C.byref(a),
+                       loss.data_ptr(), out.data_ptr(),
+                       out.stride(0) if a.rows > 1 else a.vocab, ws.data_ptr(), nbytes)
+        return loss, out
 
     def sample(self, logits: torch.Tensor, params: SamplingParams, seed: int,
                position: int) -> int:

@@ -17,6 +17,8 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
+from vinfer_b200 import _lib
+
 
 @dataclass(frozen=True)
 class SamplingParams:
@@ -239,6 +241,11 @@ class SlotHistogram:
         t = (lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(device))
         return cls(cap, t(sid), t(sc), t(lens), t(np.arange(n + 1, dtype=np.int64) * cap))
 
+    def states(self) -> DecodeStates:
+        """The slots' counts as decode states, for ``reorder_states``."""
+        s, c = self.slots, self.cap
+        return DecodeStates([self.ids.view(s, c), self.counts.view(s, c), self.lens.view(s, 1)])
+
     def to_counts(self) -> list[dict[int, int]]:
         """Each slot's {token: count}, read back to the host (synchronises)."""
         ids, counts, lens = (x.cpu().numpy() for x in (self.ids, self.counts, self.lens))
@@ -247,3 +254,129 @@ class SlotHistogram:
             a = s * self.cap
             out.append({int(i): int(c) for i, c in zip(ids[a:a + lens[s]], counts[a:a + lens[s]])})
         return out
+
+
+@dataclass
+class BeamStep:
+    """What one ``beam_select`` leaves on the device, for R requests of W beams."""
+
+    scores: torch.Tensor  # float32 [R, n]: the best continuations' scores, descending; -inf: none
+    beams: torch.Tensor  # int32 [R, n]: the beam each continues; -1: none
+    tokens: torch.Tensor  # int32 [R, n]; -1: none
+    next_scores: torch.Tensor  # float32 [R, W]: the score each slot goes on with; -inf: dead
+    parents: torch.Tensor  # int32 [R, W]: the slot (r * W + beam) whose state each slot takes
+    next_tokens: torch.Tensor  # int32 [R, W]: the token each slot appends; -1: none
+
+    @classmethod
+    def empty(cls, requests: int, width: int, n: int, device: torch.device | str) -> BeamStep:
+        f = (lambda m: torch.empty(requests, m, dtype=torch.float32, device=device))
+        i = (lambda m: torch.empty(requests, m, dtype=torch.int32, device=device))
+        return cls(f(n), i(n), i(n), f(width), i(width), i(width))
+
+
+class DecodeStates:
+    """Tensors that hold one decode state for each slot, described once for ``reorder_states``.
+
+    ``tensors`` share ``slot_dim``, the dimension that counts the slots (key/value caches
+    ``[slots, heads, length, dim]``, recurrent states, token counts, in any strided layout
+    without overlap). ``length_dim``, if given, is the dimension along which a call's ``lengths``
+    say how many positions of a slot hold data. ``out`` are the tensors that receive the copies
+    (same shapes and types, any strides); without it slots are copied in place. The tensors are
+    held and their addresses used by every call: they are not to be resized meanwhile. They
+    play the role of vinfer's per-request state slots (``src/vinfer/state/pool.py:70-131``).
+    """
+
+    def __init__(self, tensors: Sequence[torch.Tensor], slot_dim: int = 0,
+                 length_dim: int | None = None,
+                 out: Sequence[torch.Tensor] | None = None) -> None:
+        self.tensors = list(tensors)
+        self.out = self.tensors if out is None else list(out)
+        if not self.tensors:
+            raise ValueError("no states")
+        if len(self.out) != len(self.tensors):
+            raise ValueError(f"{len(self.out)} outputs for {len(self.tensors)} states")
+        self.device = self.tensors[0].device
+        self.has_lengths = length_dim is not None
+        self.slots = self._dim(self.tensors[0], slot_dim, "slot_dim")[1]
+        if not 1 <= self.slots <= _lib.STATE_MAX_SLOTS:
+            raise ValueError(f"states must have 1 to {_lib.STATE_MAX_SLOTS} slots, got {self.slots}")
+        found = []
+        for i, (t, u) in enumerate(zip(self.tensors, self.out)):
+            if t.device != self.device or u.device != self.device:
+                raise ValueError(f"state {i} is not on {self.device}")
+            if t.shape != u.shape or t.dtype != u.dtype:
+                raise ValueError(f"output {i} must have the shape and type of its state")
+            sd, n = self._dim(t, slot_dim, "slot_dim")
+            if n != self.slots:
+                raise ValueError(f"state {i} has {n} slots, the first {self.slots}")
+            ld = None if length_dim is None else self._dim(t, length_dim, "length_dim")[0]
+            if ld == sd:
+                raise ValueError("length_dim must not be slot_dim")
+            if out is not None and _overlap(t, u):
+                raise ValueError(f"output {i} overlaps its state")
+            if t.numel():
+                found.append(_describe(i, t, u, sd, ld))
+        self.count = len(found)
+        self.array = (_lib.State * max(1, self.count))(*found)
+
+    @staticmethod
+    def _dim(t: torch.Tensor, dim: int, name: str) -> tuple[int, int]:
+        if not -t.dim() <= dim < t.dim():
+            raise ValueError(f"{name} {dim} is out of range for a state of {t.dim()} dimensions")
+        return dim % t.dim(), t.shape[dim]
+
+
+def _extent(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _overlap(t: torch.Tensor, u: torch.Tensor) -> bool:
+    if not t.numel():
+        return False
+    a, b = t.data_ptr(), u.data_ptr()
+    return a < b + _extent(u) and b < a + _extent(t)
+
+
+def _describe(i: int, t: torch.Tensor, u: torch.Tensor, slot_dim: int,
+              length_dim: int | None) -> _lib.State:
+    """A state as contiguous runs under outer dimensions (``VinferState``)."""
+    es = t.element_size()
+    for x in (t, u):  # dimensions nest: each stride steps over all that is inside it
+        inside = es
+        for n, s in sorted(((n, s * es) for n, s in zip(x.shape, x.stride()) if n > 1),
+                           key=lambda d: d[1]):
+            if s < inside:
+                raise ValueError(f"state {i} overlaps itself (shape {tuple(x.shape)}, strides "
+                                 f"{tuple(x.stride())})")
+            inside += (n - 1) * s
+    dims = [(t.stride(d) * es, u.stride(d) * es, t.shape[d], d == length_dim)
+            for d in range(t.dim()) if d != slot_dim and (t.shape[d] > 1 or d == length_dim)]
+    dims.sort(key=lambda d: d[0] if d[2] > 1 else 0)  # innermost first
+    run, unit = es, 0
+    while dims and not unit and (dims[0][2] == 1 or dims[0][0] == dims[0][1] == run):
+        _, _, n, is_len = dims.pop(0)
+        if is_len:
+            unit = run
+        run *= n
+    outer: list[list] = []  # innermost first
+    for a, b, n, is_len in dims:
+        if outer and not is_len and not outer[-1][3] and a == outer[-1][0] * outer[-1][2] \
+                and b == outer[-1][1] * outer[-1][2]:
+            outer[-1][2] *= n
+        else:
+            outer.append([a, b, n, is_len])
+    if len(outer) > _lib.STATE_MAX_OUTER:
+        raise ValueError(f"state {i} is too scattered (shape {tuple(t.shape)}, strides "
+                         f"{tuple(t.stride())})")
+    outer.reverse()
+    d = _lib.State()
+    d.src, d.dst = t.data_ptr(), u.data_ptr()
+    d.src_slot_stride, d.dst_slot_stride = t.stride(slot_dim) * es, u.stride(slot_dim) * es
+    d.run_bytes, d.len_unit_bytes = run, unit
+    d.len_outer, d.n_outer = -1, len(outer)
+    for k, (a, b, n, is_len) in enumerate(outer):
+        d.outer_size[k], d.src_outer_stride[k], d.dst_outer_stride[k] = n, a, b
+        if is_len:
+            d.len_outer = k
+    return d
