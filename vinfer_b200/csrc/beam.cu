@@ -56,12 +56,18 @@ struct RowsP {
   u64* list;     // [rows, parts, n]
 };
 
-// shared memory of k_beam_rows: the list under construction, then
+constexpr int DCAP = 512;  // delegates: vectors that may hold one of the part's n best
+constexpr int LCAP = 1024; // their elements that still may
+struct Delegates {         // dynamic shared memory of k_beam_rows
+  uint4 q[DCAP];
+  int e0[DCAP];            // id of the vector's first element
+  u64 list[LCAP];
+};
 struct RowsS {
   u64 best[MAXN];
   float f[2 * NW];
   float kth[NW];
-  int cnt, got;
+  int cnt, got, nd;
   uint32_t hist[256];
   uint32_t bin, before;
 };
@@ -131,12 +137,91 @@ __device__ float nth_lane_max(float mx, int n, float* all, float* out) {
   return *out;
 }
 
+// A part's n best whatever the data (flat, sorted or clustered rows, few elements): every round
+// lists at most (n - 1) * U * A elements above a bar, and the lowest ids of those equal to it.
+// Returns the entries of `list`, which holds at most list_cap(n, A).
+template <typename T>
+__device__ __noinline__ int list_carefully(const T* p, int V, int v0, int v1, int n, u64* list,
+                                           RowsS& S) {
+  using V8 = Vec<T>;
+  constexpr int A = V8::A;
+  const Row<T> R(p, V);
+  const int cap = list_cap(n, A), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  float bar = neg_inf();  // n listed elements are >= bar, at lower ids than what follows
+  int have = 0;
+  for (int vb = v0; vb < v1; vb += NT * U) {
+    float mx = neg_inf();
+    for (int u = 0; u < U; ++u) {
+      const int v = vb + u * NT + tid;
+      if (v < v1) mx = fmaxf(mx, V8::max(R.load(v)));
+    }
+    if (have > n) {
+      select_best(list, have, n, S);
+      for (int i = tid; i < n; i += NT) list[i] = S.best[i];
+      have = n;
+    }
+    __syncthreads();
+    // above the higher of the bar so far and this round's n-th lane maximum lie the elements of
+    // fewer than n lanes
+    const float nth = nth_lane_max(mx, n, reinterpret_cast<float*>(S.hist), S.f);
+    const float lo = fmaxf(bar, nth);
+    int eq_room = nth > bar ? n : 0;  // elements equal to the bar count only where this round set it
+    if (tid == 0) S.cnt = have;
+    __syncthreads();
+    for (int u = 0; u < U; ++u) {
+      const int v = vb + u * NT + tid;
+      const uint32_t ni = V8::NEG_INF_WORD;
+      const uint4 r = v < v1 ? R.load(v) : make_uint4(ni, ni, ni, ni);
+      const int e0 = v * A - R.off;
+      int eq = 0;
+      for (int j = 0; j < A; ++j) {
+        const float x = V8::get(r, j);
+        if (x > lo) {
+          const int at = atomicAdd(&S.cnt, 1);
+          if (at < cap) list[at] = entry(x, e0 + j);
+        }
+        eq += x == lo && x > neg_inf();
+      }
+      if (eq_room > 0) {  // uniform: the lowest ids among the elements equal to the bar
+        int incl = eq;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int t = __shfl_up_sync(FULL, incl, o);
+          if (lane >= o) incl += t;
+        }
+        __syncthreads();
+        int* wsum = reinterpret_cast<int*>(S.kth);
+        if (lane == 31) wsum[w] = incl;
+        __syncthreads();
+        int base = incl - eq, total = 0;
+        for (int i = 0; i < NW; ++i) {
+          if (i < w) base += wsum[i];
+          total += wsum[i];
+        }
+        for (int j = 0; j < A && base < eq_room; ++j) {
+          const float x = V8::get(r, j);
+          if (x == lo && x > neg_inf()) {
+            const int at = atomicAdd(&S.cnt, 1);
+            if (at < cap) list[at] = entry(x, e0 + j);
+            ++base;
+          }
+        }
+        eq_room -= total;
+      }
+    }
+    __syncthreads();
+    have = min(S.cnt, cap);
+    bar = lo;
+    __syncthreads();
+  }
+  return have;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
   using V8 = Vec<T>;
   constexpr int A = V8::A;
   extern __shared__ __align__(16) unsigned char dyn[];
-  u64* list = reinterpret_cast<u64*>(dyn);
+  Delegates& D = *reinterpret_cast<Delegates*>(dyn);
   __shared__ RowsS S;
   const int row = blockIdx.x / P.parts, part = blockIdx.x - row * P.parts;
   const float b = P.scores[row];
@@ -144,142 +229,92 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
   const Row<T> R(static_cast<const T*>(P.logits) + (int64_t)row * P.ld, P.V);
   const int v0 = (int)((int64_t)R.nv * part / P.parts);
   const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
-  const int n = P.n, cap = list_cap(n, A), tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  if (tid == 0) S.cnt = 0;
+  const int n = P.n, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  if (tid == 0) {
+    S.nd = 0;
+    S.cnt = 0;
+  }
 
-  float m = neg_inf(), s = 0.f;  // this thread's softmax sum
-  float bar = neg_inf();   // n listed or listable elements are >= bar, at lower ids than what follows
-  bool first = true;
-  int listed = 0;          // entries of the list when the round begins
-  for (int vb = v0; vb < v1; vb += NT * U) {
+  // The bar: a logit that at least n lanes' maxima, so at least n elements, reach: the smallest of
+  // the warps' k-th largest lane maxima (8k >= n). A vector below it holds none of the n best; the
+  // others (about 3n a round) are kept as delegates. The warps raise it as their maxima rise;
+  // a warp that still sees the older, lower one keeps a few vectors more.
+  float m = neg_inf(), s = 0.f;
+  float seen = neg_inf();  // this lane's largest element so far
+  const int k = (n + NW - 1) / NW;
+  volatile float* kth = S.kth;
+  int round = 0;
+  for (int vb = v0; vb < v1; vb += NT * U, ++round) {
     uint4 q[U];
+    R.template load_round<U, NT>(vb, v1, q);
+    float vm[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = vb + u * NT + tid;
-      const uint32_t ni = V8::NEG_INF_WORD;
-      q[u] = v < v1 ? R.load(v) : make_uint4(ni, ni, ni, ni);
-    }
-    float mx = V8::max(q[0]);
+    for (int u = 0; u < U; ++u) vm[u] = V8::max(q[u]);
+    float mx = vm[0];
 #pragma unroll
-    for (int u = 1; u < U; ++u) mx = fmaxf(mx, V8::max(q[u]));
-    add_exps<T>(q, mx, L2E, m, s);
-
-    // The bar: a value that at least n lanes' maxima reach, so at least n elements do. The first
-    // round takes the smallest of the warps' k-th largest maxima (8k >= n); about 3n elements
-    // pass. Where that is -inf (short parts) or too many elements pass, the exact n-th maximum.
-    bool tight = false;
-    if (first) {
-      uint32_t key = okey(mx), top = 0;
-      for (int k = (n + NW - 1) / NW; k > 0; --k) {
+    for (int u = 1; u < U; ++u) mx = fmaxf(mx, vm[u]);
+    seen = fmaxf(seen, mx);
+    if ((round & (round + 1)) == 0) {  // rounds 0, 1, 3, 7, ...
+      uint32_t key = okey(seen), top = 0;
+      for (int i = k; i > 0; --i) {
         top = __reduce_max_sync(FULL, key);
         const unsigned who = __ballot_sync(FULL, key == top);
         if (lane == __ffs(who) - 1) key = 0;
       }
-      if (lane == 0) S.kth[w] = from_okey(top);
-      __syncthreads();
-      float t = S.kth[0];
+      if (lane == 0) kth[w] = from_okey(top);
+      if (round == 0) __syncthreads();
+    }
+    float bar = kth[0];
 #pragma unroll
-      for (int i = 1; i < NW; ++i) t = fminf(t, S.kth[i]);
-      bar = t;
-      if (!(t > neg_inf())) tight = true;
-    }
-    if (!tight) {
-      if (first ? mx >= bar : mx > bar) {
+    for (int i = 1; i < NW; ++i) bar = fminf(bar, kth[i]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float vm = V8::max(q[u]);
-          if (first ? vm >= bar : vm > bar) {
-            const int e0 = (vb + u * NT + tid) * A - R.off;
-            for (int j = 0; j < A; ++j) {
-              const float x = V8::get(q[u], j);
-              if ((first ? x >= bar : x > bar) && x > neg_inf()) {
-                const int at = atomicAdd(&S.cnt, 1);
-                if (at < cap) list[at] = entry(x, e0 + j);
-              }
-            }
-          }
+    for (int u = 0; u < U; ++u) {
+      const bool keep = vm[u] >= bar;
+      const unsigned who = __ballot_sync(FULL, keep);
+      if (who) {
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&S.nd, __popc(who));
+        at = __shfl_sync(FULL, at, 0) + __popc(who & ((1u << lane) - 1));
+        if (keep && at < DCAP) {
+          D.q[at] = q[u];
+          D.e0[at] = (vb + u * NT + tid) * A - R.off;
         }
       }
-      __syncthreads();
-      tight = S.cnt > cap;
     }
-    if (tight) {  // uniform: bounded and exact, whatever the data
-      __syncthreads();
-      int have = listed;
-      if (have > n) {
-        select_best(list, have, n, S);
-        for (int i = tid; i < n; i += NT) list[i] = S.best[i];
-        have = n;
-        __syncthreads();
-      }
-      // above the higher of the bar so far and this round's n-th lane maximum lie the elements
-      // of fewer than n lanes: at most (n - 1) * U * A
-      const float old = first ? neg_inf() : bar;
-      float* all = reinterpret_cast<float*>(S.hist);
-      const float nth = nth_lane_max(mx, n, all, S.f);
-      const float lo = fmaxf(old, nth);
-      if (tid == 0) S.cnt = have;
-      __syncthreads();
-      int eq_room = nth > old ? n : 0;  // equal elements count only where this round sets the bar
-      for (int u = 0; u < U; ++u) {
-        // q[u] by a dynamic index would live in local memory; the vector is read again
-        const int v = vb + u * NT + tid;
-        const uint32_t ni = V8::NEG_INF_WORD;
-        const uint4 r = v < v1 ? R.load(v) : make_uint4(ni, ni, ni, ni);
-        const int e0 = v * A - R.off;
-        int eq = 0;
-        for (int j = 0; j < A; ++j) {
-          const float x = V8::get(r, j);
-          if (x > lo) {
-            const int at = atomicAdd(&S.cnt, 1);
-            if (at < cap) list[at] = entry(x, e0 + j);
-          }
-          eq += x == lo && x > neg_inf();
-        }
-        if (eq_room > 0) {  // uniform: the lowest ids among the elements equal to the bar
-          int incl = eq;
-          for (int o = 1; o < 32; o <<= 1) {
-            const int t = __shfl_up_sync(FULL, incl, o);
-            if (lane >= o) incl += t;
-          }
-          __syncthreads();
-          int* wsum = reinterpret_cast<int*>(S.kth);
-          if (lane == 31) wsum[w] = incl;
-          __syncthreads();
-          int base = incl - eq, total = 0;
-          for (int i = 0; i < NW; ++i) {
-            if (i < w) base += wsum[i];
-            total += wsum[i];
-          }
-          for (int j = 0; j < A && base < eq_room; ++j) {
-            const float x = V8::get(r, j);
-            if (x == lo && x > neg_inf()) {
-              const int at = atomicAdd(&S.cnt, 1);
-              if (at < cap) list[at] = entry(x, e0 + j);
-              ++base;
-            }
-          }
-          eq_room -= total;
-        }
-      }
-      __syncthreads();
-      bar = lo;
-    }
-    first = false;
-    listed = S.cnt;
-    __syncthreads();
+    add_exps<T>(q, mx, L2E, m, s);
   }
+  __syncthreads();
 
-  // the part's n best, in order, and its sum
-  const int L = min(S.cnt, cap);
-  const u64* src = list;
-  int have = L;
-  if (L > 384) {
-    if (L > n) {
-      select_best(list, L, n, S);
-      src = S.best;
-      have = n;
+  // the delegates' elements that reach the final bar, one a thread
+  float bar = S.kth[0];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) bar = fminf(bar, S.kth[i]);
+  bool careful = !(bar > neg_inf()) || S.nd > DCAP;
+  if (!careful) {
+    for (int i = tid; i < S.nd * A; i += NT) {
+      const T* x = reinterpret_cast<const T*>(&D.q[i / A]) + i % A;
+      const float f = V8::load(x);
+      if (f >= bar) {
+        const int at = atomicAdd(&S.cnt, 1);
+        if (at < LCAP) D.list[at] = entry(f, D.e0[i / A] + i % A);
+      }
     }
+    __syncthreads();
+    careful = S.cnt > LCAP;
+  }
+  const u64* src = D.list;
+  u64* all = reinterpret_cast<u64*>(dyn);
+  int have = S.cnt;
+  __syncthreads();
+  if (careful) {
+    have = list_carefully<T>(R.p, P.V, v0, v1, n, all, S);
+    src = all;
+  }
+  // the part's n best, in order, and its sum
+  if (have > 384 && have > n) {
+    select_best(src, have, n, S);
+    src = S.best;
+    have = n;
   }
   const int64_t at = (int64_t)blockIdx.x;
   u64* out = P.list + at * n;
@@ -591,7 +626,7 @@ bool beam_shape_ok(int64_t requests, int32_t beams, int64_t vocab, int32_t dtype
 template <typename T>
 int launch_beam(const PickP& Q, int64_t requests, cudaStream_t st) {
   const int64_t rows_ = requests * Q.W;
-  const size_t sm_rows = (size_t)list_cap(Q.r.n, Vec<T>::A) * 8;
+  const size_t sm_rows = std::max(sizeof(Delegates), (size_t)list_cap(Q.r.n, Vec<T>::A) * 8);
   const size_t sm_pick = pick_smem(Q.W, Q.r.n, Q.r.parts);
   if (opt_in(k_beam_rows<T>, sm_rows) != VINFER_OK || opt_in(k_beam_pick<T>, sm_pick) != VINFER_OK)
     return VINFER_E_CUDA;

@@ -57,10 +57,20 @@ struct DistP {
   int64_t ldg;
 };
 
+// Vector v of the part with its listed elements taken out.
+template <typename T>
+__device__ __noinline__ uint4 without(uint4 q, int v, const int* hit, int hits) {
+  for (int h = 0; h < hits; ++h)
+    if (hit[h] / Vec<T>::A == v) Vec<T>::put(q, hit[h] & (Vec<T>::A - 1), Vec<T>::NEG_INF_BITS);
+  return q;
+}
+
+// Dynamic shared memory: one bit for each vector of the part, set where it holds a listed element.
 template <typename T>
 __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   using VT = Vec<T>;
   constexpr int A = VT::A;
+  extern __shared__ uint32_t marked[];
   __shared__ float sm[2 * NW];
   __shared__ int hit[MAXK];
   __shared__ int hits;
@@ -70,29 +80,27 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
   const int v0 = (int)((int64_t)R.nv * part / P.parts);
   const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
+  const int id = tid < P.k ? P.ids[row * P.k + tid] : -1;
+  for (int i = tid; i < (v1 - v0 + 31) / 32; i += NT) marked[i] = 0;
   if (tid == 0) hits = 0;
   __syncthreads();
-  if (tid < P.k) {  // the part's listed elements, counted from its first vector
-    const int id = P.ids[row * P.k + tid];
-    const int e = id + R.off - v0 * A;
-    if (id >= 0 && id < P.V && e >= 0 && e < (v1 - v0) * A) hit[atomicAdd(&hits, 1)] = e;
+  {
+    const int e = id + R.off - v0 * A;  // the part's elements, counted from its first vector
+    if (id >= 0 && id < P.V && e >= 0 && e < (v1 - v0) * A) {
+      hit[atomicAdd(&hits, 1)] = e;
+      atomicOr(&marked[e / A / 32], 1u << (e / A & 31));
+    }
   }
   __syncthreads();
   float m = neg_inf(), s = 0.f;
   for (int vb = v0; vb < v1; vb += NT * U) {
     uint4 q[U];
+    R.template load_round<U, NT>(vb, v1, q);
+    if (hits) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = vb + u * NT + tid;
-      const uint32_t ni = VT::NEG_INF_WORD;
-      q[u] = v < v1 ? R.load(v) : make_uint4(ni, ni, ni, ni);
-    }
-    for (int h = 0; h < hits; ++h) {
-      const int e = hit[h] - (vb - v0) * A;
-      if (e >= 0 && e < NT * U * A && ((e / A) & (NT - 1)) == tid) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (u == e / (A * NT)) VT::put(q[u], e & (A - 1), VT::NEG_INF_BITS);
+      for (int u = 0; u < U; ++u) {
+        const int v = vb - v0 + u * NT + tid;
+        if (v < v1 - v0 && marked[v / 32] >> (v & 31) & 1) q[u] = without<T>(q[u], v, hit, hits);
       }
     }
     float mx = VT::max(q[0]);
@@ -261,13 +269,7 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
   const float coef = f * st.coef;
   for (int vb = v0; vb < v1; vb += NT * U) {
     uint4 q[U];
-    if (f != 0.f) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int v = vb + u * NT + tid;
-        if (v < v1) q[u] = R.load(v);
-      }
-    }
+    if (f != 0.f) R.template load_round<U, NT>(vb, v1, q);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int v = vb + u * NT + tid;
@@ -344,7 +346,9 @@ DistP params(const VinferDistillArgs* a) {
 
 template <typename T>
 int launch_loss(const DistP& P, cudaStream_t st) {
-  const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, 0, st, false, P);
+  const int part_vecs = (P.V / Vec<T>::A + 2 + P.parts - 1) / P.parts + 1;
+  const size_t smem = (size_t)(part_vecs + 31) / 32 * 4;
+  const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, smem, st, false, P);
   if (rc != VINFER_OK) return rc;
   return launch(k_distill_finish<T>, (unsigned)((P.rows + NW - 1) / NW), NT, 0, st, true, P);
 }

@@ -153,6 +153,32 @@ struct Row {
     }
     return edge(p, V, v * Vec<T>::A - off);
   }
+  // The thread's vectors vb + u * NT + threadIdx.x of a round, below v1; -inf behind it. Predicated
+  // loads without branches between them, so that all are in flight together; the row's ragged ends
+  // are read behind them.
+  template <int U, int NT>
+  __device__ __forceinline__ void load_round(int vb, int v1, uint4 (&q)[U]) const {
+    const T* at = p + ((int64_t)(vb + (int)threadIdx.x) * Vec<T>::A - off);
+    const int lo = off ? 1 : 0, hi = min(v1, (V + off) / Vec<T>::A);  // whole vectors
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int v = vb + u * NT + (int)threadIdx.x;
+      const uint32_t n = Vec<T>::NEG_INF_WORD;
+      q[u] = make_uint4(n, n, n, n);
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
+          "@p ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
+          : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w)
+          : "l"(at + (int64_t)u * NT * Vec<T>::A), "r"((uint32_t)(v >= lo && v < hi)));
+    }
+    if (vb == 0 && off && threadIdx.x == 0) q[0] = edge(p, V, -off);
+    if (hi < v1 && hi >= vb && hi < vb + U * NT && (hi > 0 || !off)) {  // the last, a ragged one
+      const int mine = hi - vb - (int)threadIdx.x;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (mine == u * NT) q[u] = edge(p, V, hi * Vec<T>::A - off);
+    }
+  }
   // the vector whose first element is e0, element by element
   static __device__ __noinline__ uint4 edge(const T* p, int V, int e0) {
     const uint32_t n = Vec<T>::NEG_INF_WORD;
