@@ -262,7 +262,9 @@ int vinfer_beam_select(const VinferBeamArgs* args, void* workspace, size_t works
  *    positions (of len_unit_bytes each) of every run, with len_outer >= 0 only the first lengths[s]
  *    indices of that outer dimension; positions behind them are neither read nor written.
  * A parent outside [0, slots) leaves the slot alone and sets VINFER_ST_BAD_PARENT. `states` is a
- * host array, read during the call. slots <= VINFER_STATE_MAX_SLOTS. */
+ * host array, read during the call. slots <= VINFER_STATE_MAX_SLOTS. Copies go in vectors of up to
+ * 16 bytes, the largest that divides every address, stride and size of the state; VINFER_E_LIMIT
+ * when a slot has 2^31 of them or more. */
 #define VINFER_STATE_MAX_OUTER 4
 #define VINFER_STATE_MAX_SLOTS 8192
 typedef struct VinferState {

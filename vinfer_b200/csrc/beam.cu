@@ -24,6 +24,8 @@ constexpr int NT = 256, NW = NT / 32;
 constexpr int U = 8;              // 16-byte vectors a thread holds: 32 KiB a CTA and round
 constexpr int MAX_PARTS = 64;     // parts of a row
 constexpr int MAX_JOIN = 1024;    // entries of a beam's parts together (a warp joins them)
+constexpr int MAX_STAGED = 8192;  // entries of a request's parts together (64 KiB staged)
+constexpr int PT = 512, PW = PT / 32;  // threads of k_beam_pick
 constexpr int MAXN = VINFER_BEAM_MAX_N, MAXW = VINFER_BEAM_MAX_WIDTH;
 // Scores of different beams within this distance are compared with sums taken in double: about
 // ten times the error of a streamed log-sum (2^-20 from rounding the largest exponents, 2^-22
@@ -43,8 +45,7 @@ __device__ __forceinline__ int entry_id(u64 e) { return (int)(uint32_t)e; }
 
 struct PartHdr {
   float m, s;  // softmax sum of the part, (m, s) at scale L2E
-  int cnt;     // listed entries, ascending
-  int pad;
+  int pad[2];
 };
 
 struct RowsP {
@@ -53,8 +54,9 @@ struct RowsP {
   int V, n, parts;
   const float* scores;
   PartHdr* hdr;  // [rows, parts]
-  u64* list;     // [rows, parts, n]
+  u64* list;     // [rows, parts, n], ascending, NONE behind the last
 };
+constexpr u64 NONE = ~0ull;
 
 constexpr int DCAP = 512;  // delegates: vectors that may hold one of the part's n best
 constexpr int LCAP = 1024; // their elements that still may
@@ -324,15 +326,9 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
     for (int j = 0; j < have; ++j) rank += src[j] < e;
     if (rank < n) out[rank] = e;
   }
+  for (int i = have + tid; i < n; i += NT) out[i] = NONE;
   block_join<NW>(m, s, L2E, S.f);
-  if (tid == 0) {
-    PartHdr h;
-    h.m = m;
-    h.s = s;
-    h.cnt = min(have, n);
-    h.pad = 0;
-    P.hdr[at] = h;
-  }
+  if (tid == 0) P.hdr[at] = PartHdr{m, s, {0, 0}};
 }
 
 struct PickP {
@@ -350,15 +346,15 @@ struct PickP {
 
 struct PickS {
   double m[MAXW], lns[MAXW];  // log-sum of each beam's row: m + lns
-  float b[MAXW];        // beam scores
-  int cnt[MAXW];        // entries of each beam's list
-  int head[MAXN];       // ranked candidates: beam << 16 | place in its list
-  uint32_t flags;       // beams whose sums are taken again
-  int alive;            // surviving candidates
-  float kth[NW];
-  double red[NW];
-  int sel[MAXW];        // continuing candidates: their ranks
-  int nsel;
+  float b[MAXW];              // beam scores
+  int cnt[MAXW];              // entries of each beam's list
+  int head[MAXN];             // ranked candidates: beam << 16 | place in its list
+  int eos[VINFER_BEAM_MAX_EOS];
+  uint32_t flags;             // beams whose sums are taken again
+  int alive;                  // surviving candidates
+  float kth[PW];
+  double red[PW];
+  int sel[MAXW];              // continuing candidates: their ranks
 };
 
 template <typename T>
@@ -367,21 +363,21 @@ __device__ void row_sum_double(const RowsP& P, int row, double* red, double* m_o
   // strided by element, so equal rows get equal sums whatever their alignment
   const T* x = static_cast<const T*>(P.logits) + (int64_t)row * P.ld;
   float m = neg_inf();
-  for (int i = threadIdx.x; i < P.V; i += NT) m = fmaxf(m, Vec<T>::load(x + i));
+  for (int i = threadIdx.x; i < P.V; i += PT) m = fmaxf(m, Vec<T>::load(x + i));
   m = warp_max(m);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
   __syncthreads();
   double mm = red[0];
-  for (int i = 1; i < NW; ++i) mm = fmax(mm, red[i]);
+  for (int i = 1; i < PW; ++i) mm = fmax(mm, red[i]);
   __syncthreads();
   double s = 0;
-  for (int i = threadIdx.x; i < P.V; i += NT) s += exp((double)Vec<T>::load(x + i) - mm);
+  for (int i = threadIdx.x; i < P.V; i += PT) s += exp((double)Vec<T>::load(x + i) - mm);
   s = warp_sum(s);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
   __syncthreads();
   s = 0;
-  for (int i = 0; i < NW; ++i) s += red[i];
+  for (int i = 0; i < PW; ++i) s += red[i];
   __syncthreads();
   if (threadIdx.x == 0) {
     *m_out = mm;
@@ -389,111 +385,129 @@ __device__ void row_sum_double(const RowsP& P, int row, double* red, double* m_o
   }
 }
 
-// One CTA a request. Dynamic shared memory: W * n entries (the beams' lists), W * n 2-byte
-// places of surviving candidates, and parts * n entries for each warp's join.
+// One CTA a request. Dynamic shared memory: the staged entries of its parts [W, parts, n], the
+// beams' lists [W, n], the survivors' scores and places [W * n] each.
 template <typename T>
-__global__ void __launch_bounds__(NT, 1) k_beam_pick(const PickP Q) {
+__global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ PickS S;
   const RowsP& P = Q.r;
-  const int W = Q.W, n = P.n, req = blockIdx.x, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  u64* lists = reinterpret_cast<u64*>(dyn);
-  u64* join = lists + W * n + w * P.parts * n;
-  unsigned short* live = reinterpret_cast<unsigned short*>(lists + W * n + NW * P.parts * n);
+  const int W = Q.W, n = P.n, per = P.parts * n;
+  const int req = blockIdx.x, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  u64* staged = reinterpret_cast<u64*>(dyn);
+  u64* lists = staged + W * per;
+  double* sc = reinterpret_cast<double*>(lists + W * n);
+  unsigned short* live = reinterpret_cast<unsigned short*>(sc + W * n);
   if (tid == 0) {
     S.flags = 0;
     S.alive = 0;
-    S.nsel = 0;
   }
+  if (tid < W) S.b[tid] = P.scores[(int64_t)req * W + tid];
+  if (tid < Q.n_eos) S.eos[tid] = Q.eos[tid];
   grid_dependency_wait();
 
-  for (int beam = w; beam < W; beam += NW) {
-    const int64_t row = (int64_t)req * W + beam;
-    const float b = P.scores[row];
+  const u64* E = P.list + (int64_t)req * W * per;
+  for (int i = tid; i < W * per; i += PT) staged[i] = E[i];  // dead beams': whatever is there
+  for (int beam = w; beam < W; beam += PW) {
+    const PartHdr* H = P.hdr + ((int64_t)req * W + beam) * P.parts;
+    float m = neg_inf(), m2 = neg_inf(), s0 = 0, s1 = 0;  // MAX_PARTS is two a lane
+    if (lane < P.parts) {
+      m = H[lane].m;
+      s0 = H[lane].s;
+    }
+    if (lane + 32 < P.parts) {
+      m2 = H[lane + 32].m;
+      s1 = H[lane + 32].s;
+    }
+    const float top = warp_max(fmaxf(m, m2));
+    // in double: the sum of at most 64 floats, each scaled by a power of two
+    double s = 0;
+    if (s0 != 0.f) s += (double)s0 * exp2(((double)m - (double)top) * (double)L2E);
+    if (s1 != 0.f) s += (double)s1 * exp2(((double)m2 - (double)top) * (double)L2E);
+    s = warp_sum(s);
+    if (lane == 0) {
+      S.m[beam] = top;
+      S.lns[beam] = s;  // its logarithm below
+    }
+  }
+  __syncthreads();
+
+  for (int beam = w; beam < W; beam += PW) {
+    const float b = S.b[beam];
+    const double s = S.lns[beam];
     int cnt = 0;
-    double lns = 0, top = 0;
-    if (b > neg_inf() && b < -neg_inf()) {
-      const PartHdr* H = P.hdr + row * P.parts;
-      const u64* E = P.list + row * P.parts * n;
-      float m = neg_inf();
-      for (int p = lane; p < P.parts; p += 32) m = fmaxf(m, H[p].m);
-      m = warp_max(m);
-      double s = 0;
-      for (int p = lane; p < P.parts; p += 32)
-        if (H[p].s != 0.f) s += (double)H[p].s * exp2(((double)H[p].m - (double)m) * (double)L2E);
-      s = warp_sum(s);
-      if (s > 0 && s < (double)FLT_MAX) {
-        top = m;
-        lns = log(s);
-        // n best of the parts' lists. Every lane's k-th best bounds the n-th best of all from
-        // below (32k >= n); what reaches the least of them survives, and is ranked by counting.
-        const int total = P.parts * n, k = (n + 31) / 32;
-        u64 bound = 0;
-        {
-          u64 t[4] = {~0ull, ~0ull, ~0ull, ~0ull};  // this lane's four best, ascending
-          for (int i = lane; i < total; i += 32) {
-            const int p = i / n;
-            u64 e = i - p * n < H[p].cnt ? E[i] : ~0ull;
+    unsigned bad = 0;
+    if (!(b > neg_inf() && b < -neg_inf())) {
+      if (b != neg_inf()) bad = VINFER_ST_BAD_SCORE;
+    } else if (!(s > 0 && s < (double)FLT_MAX)) {
+      bad = VINFER_ST_NONFINITE;  // a NaN or +inf, or every logit -inf
+    } else {
+      // n best of the parts' lists. Every lane's k-th best bounds the n-th best of all from below
+      // (32k >= n); what reaches the least of them survives, and is ranked by counting.
+      u64* mine = staged + beam * per;
+      const int k = (n + 31) / 32;
+      u64 t[4] = {NONE, NONE, NONE, NONE};  // this lane's best, ascending
+      if (k == 1) {
+        for (int i = lane; i < per; i += 32) t[0] = mine[i] < t[0] ? mine[i] : t[0];
+      } else {
+        for (int i = lane; i < per; i += 32) {
+          u64 e = mine[i];
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
-              if (e < t[a]) {
-                const u64 o = t[a];
-                t[a] = e;
-                e = o;
-              }
-          }
-          bound = k == 1 ? t[0] : k == 2 ? t[1] : k == 3 ? t[2] : t[3];
-#pragma unroll
-          for (int o = 16; o; o >>= 1) {
-            const u64 other = __shfl_xor_sync(FULL, bound, o);
-            bound = other > bound ? other : bound;
-          }
+          for (int a = 0; a < 4; ++a)
+            if (e < t[a]) {
+              const u64 o = t[a];
+              t[a] = e;
+              e = o;
+            }
         }
-        int alive = 0;
-        for (int i0 = 0; i0 < total; i0 += 32) {
-          const int i = i0 + lane, p = i / n;
-          const u64 e = i < total && i - p * n < H[p].cnt ? E[i] : ~0ull;
-          const bool keep = e <= bound && e != ~0ull;
-          const unsigned m = __ballot_sync(FULL, keep);
-          if (keep) join[alive + __popc(m & ((1u << lane) - 1))] = e;
-          alive += __popc(m);
-        }
-        __syncwarp();
-        for (int i = lane; i < alive; i += 32) {
-          const u64 e = join[i];
-          int rank = 0;
-          for (int j = 0; j < alive; ++j) rank += join[j] < e;
-          if (rank < n) lists[beam * n + rank] = e;
-        }
-        cnt = min(alive, n);
-      } else if (lane == 0 && Q.status) {  // a NaN or +inf, or every logit -inf
-        atomicOr(Q.status, (int)VINFER_ST_NONFINITE);
       }
-    } else if (lane == 0 && Q.status && !(b == neg_inf())) {
-      atomicOr(Q.status, (int)VINFER_ST_BAD_SCORE);
+      u64 bound = k == 1 ? t[0] : k == 2 ? t[1] : k == 3 ? t[2] : t[3];
+#pragma unroll
+      for (int o = 16; o; o >>= 1) {
+        const u64 other = __shfl_xor_sync(FULL, bound, o);
+        bound = other > bound ? other : bound;
+      }
+      int alive = 0;
+      for (int i0 = 0; i0 < per; i0 += 32) {
+        const u64 e = i0 + lane < per ? mine[i0 + lane] : NONE;
+        const bool keep = e <= bound && e != NONE;
+        const unsigned who = __ballot_sync(FULL, keep);  // all have read; places are behind i0
+        if (keep) mine[alive + __popc(who & ((1u << lane) - 1))] = e;
+        alive += __popc(who);
+      }
+      __syncwarp();
+      for (int i = lane; i < alive; i += 32) {
+        const u64 e = mine[i];
+        int rank = 0;
+        for (int j = 0; j < alive; ++j) rank += mine[j] < e;
+        if (rank < n) lists[beam * n + rank] = e;
+      }
+      cnt = min(alive, n);
     }
     if (lane == 0) {
-      S.b[beam] = b;
-      S.m[beam] = top;
-      S.lns[beam] = lns;
+      if (bad && Q.status) atomicOr(Q.status, (int)bad);
       S.cnt[beam] = cnt;
+      if (cnt) S.lns[beam] = log(s);
     }
   }
   __syncthreads();
 
   auto score = [&](int beam, int j) {
-    return (double)S.b[beam] + (((double)entry_x(lists[beam * n + j]) - S.m[beam]) - S.lns[beam]);
+    return (double)S.b[beam] +
+           (((double)entry_x(lists[beam * n + j]) - S.m[beam]) - S.lns[beam]);
   };
   // candidates that can be among the n best, or within NEAR of the last of them
   {
-    const int k = (n + NW - 1) / NW;
     float mine = neg_inf();
-    for (int i = tid; i < W * n; i += NT) {
+    for (int i = tid; i < W * n; i += PT) {
       const int beam = i / n, j = i - beam * n;
-      if (j < S.cnt[beam]) mine = fmaxf(mine, __double2float_rd(score(beam, j)));
+      if (j < S.cnt[beam]) {
+        sc[i] = score(beam, j);
+        mine = fmaxf(mine, __double2float_rd(sc[i]));
+      }
     }
     uint32_t key = okey(mine), top = 0;
-    for (int a = 0; a < k; ++a) {
+    for (int a = (n + PW - 1) / PW; a > 0; --a) {
       top = __reduce_max_sync(FULL, key);
       const unsigned who = __ballot_sync(FULL, key == top);
       if (lane == __ffs(who) - 1) key = 0;
@@ -501,26 +515,26 @@ __global__ void __launch_bounds__(NT, 1) k_beam_pick(const PickP Q) {
     if (lane == 0) S.kth[w] = top ? from_okey(top) : neg_inf();
     __syncthreads();
     float t = S.kth[0];
-    for (int i = 1; i < NW; ++i) t = fminf(t, S.kth[i]);
-    for (int i = tid; i < W * n; i += NT) {
+    for (int i = 1; i < PW; ++i) t = fminf(t, S.kth[i]);
+    for (int i = tid; i < W * n; i += PT) {
       const int beam = i / n, j = i - beam * n;
-      if (j < S.cnt[beam] && score(beam, j) >= (double)t - 2 * NEAR)
+      if (j < S.cnt[beam] && sc[i] >= (double)t - 2 * NEAR)
         live[atomicAdd(&S.alive, 1)] = (unsigned short)(beam << 8 | j);
     }
     __syncthreads();
   }
   for (int pass = 0; pass < 2; ++pass) {
-    for (int i = tid; i < S.alive; i += NT) {
+    for (int i = tid; i < S.alive; i += PT) {
       const int bi = live[i] >> 8, ji = live[i] & 255;
-      const double si = score(bi, ji);
+      const double si = sc[bi * n + ji];
       int rank = 0;
       uint32_t close = 0;
       for (int k = 0; k < S.alive; ++k) {
         const int bk = live[k] >> 8, jk = live[k] & 255;
+        const double sk = sc[bk * n + jk];
         if (bk == bi) {
           rank += jk < ji;
         } else {
-          const double sk = score(bk, jk);
           rank += sk > si || (sk == si && bk < bi);
           if (fabs(sk - si) <= NEAR) close |= 1u << bk;
         }
@@ -537,15 +551,20 @@ __global__ void __launch_bounds__(NT, 1) k_beam_pick(const PickP Q) {
       if (flags >> beam & 1)
         row_sum_double<T>(P, req * W + beam, S.red, &S.m[beam], &S.lns[beam]);
     __syncthreads();
+    for (int i = tid; i < S.alive; i += PT) {
+      const int beam = live[i] >> 8, j = live[i] & 255;
+      sc[beam * n + j] = score(beam, j);
+    }
+    __syncthreads();
   }
 
   // the list of candidates
   const int have = min(S.alive, n);
-  for (int i = tid; i < n; i += NT) {
+  for (int i = tid; i < n; i += PT) {
     const int64_t o = (int64_t)req * n + i;
     if (i < have) {
       const int beam = S.head[i] >> 16, j = S.head[i] & 0xffff;
-      Q.out_scores[o] = (float)score(beam, j);
+      Q.out_scores[o] = (float)sc[beam * n + j];
       Q.out_beams[o] = beam;
       Q.out_tokens[o] = entry_id(lists[beam * n + j]);
     } else {
@@ -562,7 +581,7 @@ __global__ void __launch_bounds__(NT, 1) k_beam_pick(const PickP Q) {
       bool on = i < have;
       if (on) {
         const int id = entry_id(lists[(S.head[i] >> 16) * n + (S.head[i] & 0xffff)]);
-        for (int e = 0; e < Q.n_eos; ++e) on = on && id != Q.eos[e];
+        for (int e = 0; e < Q.n_eos; ++e) on = on && id != S.eos[e];
       }
       const unsigned m = __ballot_sync(FULL, on);
       const int at = nsel + __popc(m & ((1u << lane) - 1));
@@ -589,7 +608,7 @@ __global__ void __launch_bounds__(NT, 1) k_beam_pick(const PickP Q) {
     const unsigned filled = __reduce_or_sync(FULL, on ? 1u << slot : 0u);
     if (on) {
       const int64_t o = (int64_t)req * W + slot;
-      Q.next_scores[o] = (float)score(beam, cand & 0xffff);
+      Q.next_scores[o] = (float)sc[beam * n + (cand & 0xffff)];
       Q.parents[o] = req * W + beam;
       Q.next_tokens[o] = entry_id(lists[beam * n + (cand & 0xffff)]);
     }
@@ -604,17 +623,17 @@ __global__ void __launch_bounds__(NT, 1) k_beam_pick(const PickP Q) {
 
 // Parts of a row: enough CTAs to fill the 148 SMs several times over, at least two vectors a
 // thread in each, and no more entries than a warp joins.
-int beam_parts(int64_t rows, int64_t vocab, int dtype, int n) {
+int beam_parts(int64_t rows, int W, int64_t vocab, int dtype, int n) {
   const int64_t A = dtype == VINFER_DTYPE_BF16 ? 8 : 4;
   const int64_t nv = (vocab + A - 1) / A;
   int64_t p = (148 * 8 + rows - 1) / rows;
   p = std::min<int64_t>(p, (nv + 2 * NT - 1) / (2 * NT));
-  p = std::min<int64_t>(p, std::min<int64_t>(MAX_PARTS, MAX_JOIN / n));
+  p = std::min<int64_t>(p, std::min(MAX_PARTS, std::min(MAX_JOIN / n, MAX_STAGED / (W * n))));
   return (int)std::max<int64_t>(1, p);
 }
 
 size_t pick_smem(int W, int n, int parts) {
-  return (size_t)W * n * 8 + (size_t)NW * parts * n * 8 + (size_t)W * n * 2;
+  return (size_t)W * n * (8 * (size_t)parts + 8 + 8 + 2);
 }
 
 bool beam_shape_ok(int64_t requests, int32_t beams, int64_t vocab, int32_t dtype, int32_t n) {
@@ -632,7 +651,7 @@ int launch_beam(const PickP& Q, int64_t requests, cudaStream_t st) {
     return VINFER_E_CUDA;
   const int rc = launch(k_beam_rows<T>, (unsigned)(rows_ * Q.r.parts), NT, sm_rows, st, false, Q.r);
   if (rc != VINFER_OK) return rc;
-  return launch(k_beam_pick<T>, (unsigned)requests, NT, sm_pick, st, true, Q);
+  return launch(k_beam_pick<T>, (unsigned)requests, PT, sm_pick, st, true, Q);
 }
 
 }  // namespace
@@ -643,7 +662,7 @@ size_t vinfer_beam_workspace_bytes(int64_t requests, int32_t beams, int64_t voca
                                    int32_t n) {
   if (!beam_shape_ok(requests, beams, vocab, dtype, n)) return 0;
   const int64_t rows_ = requests * beams;
-  return (size_t)rows_ * beam_parts(rows_, vocab, dtype, n) * (sizeof(PartHdr) + 8 * (size_t)n);
+  return (size_t)rows_ * beam_parts(rows_, beams, vocab, dtype, n) * (sizeof(PartHdr) + 8 * (size_t)n);
 }
 
 int vinfer_beam_select(const VinferBeamArgs* a, void* workspace, size_t workspace_bytes,
@@ -670,7 +689,7 @@ int vinfer_beam_select(const VinferBeamArgs* a, void* workspace, size_t workspac
   Q.r.ld = a->ld;
   Q.r.V = (int)a->vocab;
   Q.r.n = a->n;
-  Q.r.parts = beam_parts(rows_, a->vocab, a->dtype, a->n);
+  Q.r.parts = beam_parts(rows_, a->beams, a->vocab, a->dtype, a->n);
   Q.r.scores = a->scores;
   Q.r.hdr = static_cast<PartHdr*>(workspace);
   Q.r.list = reinterpret_cast<u64*>(static_cast<unsigned char*>(workspace) +

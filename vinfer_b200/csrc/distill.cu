@@ -112,53 +112,168 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   if (tid == 0) P.part[blockIdx.x] = Part{m, s};
 }
 
+// A row's list as one warp works on it, four entries a lane.
+struct ListS {
+  double z[MAXK];     // listed logits; behind the join distances from the row's largest, in log2
+  double p[MAXK];     // masses as listed
+  double psum[MAXK];  // ... summed over the entries of the same id
+  float l[MAXK];      // log-probabilities
+  int id[MAXK];       // -1: empty
+  bool lead[MAXK];    // the first entry of its id
+  double mass;        // sum of p
+  double top;         // largest z
+  int distinct;       // ids
+  bool bad;           // an id or a log-probability out of range
+};
+
+// What depends on the list alone, and its logits.
 template <typename T>
-__global__ void __launch_bounds__(NT) k_distill_finish(const DistP P) {
-  __shared__ int sid[NW][MAXK];
-  __shared__ float sp[NW][MAXK];
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * NW + w;
-  const bool there = row < P.rows;
-  const float weight = there && P.weights ? P.weights[row] : 1.f;
+__device__ __forceinline__ void list_begin(const DistP& P, int64_t row, ListS& L) {
+  const int lane = threadIdx.x & 31;
+  const T* x = static_cast<const T*>(P.logits) + row * P.ld;
   int id[4];
-  float l[4];
   bool bad = false;
+  double mass = 0, top = (double)neg_inf();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int j = lane + 32 * i;
     id[i] = -1;
-    l[i] = neg_inf();
-    if (there && j < P.k) {
+    if (j < P.k) {
       id[i] = P.ids[row * P.k + j];
-      if (id[i] >= 0) l[i] = P.lp[row * P.k + j];
-      if (id[i] >= P.V || !(l[i] < -neg_inf())) bad = true;
-      sid[w][j] = id[i];
-      sp[w][j] = l[i];
+      float l = P.lp[row * P.k + j];
+      if (id[i] < 0) {
+        id[i] = -1;
+        l = neg_inf();
+      }
+      const bool off = id[i] >= P.V || !(l < -neg_inf());
+      bad = bad || off;
+      const double z = id[i] >= 0 && !off ? (double)Vec<T>::load(x + id[i]) : (double)neg_inf();
+      const double p = id[i] >= 0 ? exp((double)l) : 0.0;
+      L.id[j] = id[i];
+      L.l[j] = l;
+      L.z[j] = z;
+      L.p[j] = p;
+      mass += p;
+      if (z > top || z != z) top = z;
     }
   }
   __syncwarp();
+  double psum[4] = {0, 0, 0, 0};
+  bool lead[4] = {id[0] >= 0, id[1] >= 0, id[2] >= 0, id[3] >= 0};
+  for (int o = 0; o < P.k; ++o) {
+    const int other = L.id[o];
+    const double po = L.p[o];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (other == id[i] && other >= 0) {
+        psum[i] += po;
+        if (o < lane + 32 * i) lead[i] = false;
+      }
+  }
+  int distinct = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int j = lane + 32 * i;
+    if (j < P.k) {
+      L.psum[j] = psum[i];
+      L.lead[j] = lead[i];
+      distinct += lead[i];
+    }
+  }
+  mass = warp_sum(mass);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const double t = __shfl_xor_sync(FULL, top, o);
+    if (t > top || t != t) top = t;
+  }
+  distinct = (int)__reduce_add_sync(FULL, (unsigned)distinct);
+  bad = __any_sync(FULL, bad);
+  if (lane == 0) {
+    L.mass = mass;
+    L.top = top;
+    L.distinct = distinct;
+    L.bad = bad;
+  }
+  __syncwarp();
+}
+
+// The row's loss and gradient terms from the list and the sum outside it, (m, r) with r in units of
+// 2^(m * scale). listg[j]: dloss/dz of the j-th listed element.
+__device__ __forceinline__ float list_finish(const DistP& P, ListS& L, float m, double r,
+                                             Stat* stat, float* listg) {
+  const int lane = threadIdx.x & 31;
+  const float nan = __int_as_float(0x7fffffff);
+  if (L.bad) {
+    if (lane == 0 && P.status) atomicOr(P.status, (int)VINFER_ST_BAD_LIST);
+    if (listg)
+      for (int j = lane; j < P.k; j += 32) listg[j] = nan;
+    if (stat) *stat = Stat{nan, nan};
+    return nan;
+  }
+  // all in distances from the row's largest logit, whatever its magnitude, and in log2
+  const double inf = (double)-neg_inf();
+  double ref = L.top;
+  if (r != 0 && !(ref != ref) && (double)m > ref) ref = m;
+  double total = 0;
+  for (int j = lane; j < P.k; j += 32) {
+    L.z[j] = (L.z[j] - ref) * P.scale_d;
+    if (L.lead[j]) total += exp2(L.z[j]);
+  }
+  const double rest = r == 0 ? -inf : ((double)m - ref) * P.scale_d + log2(r);
+  total = warp_sum(total) + (r == 0 ? 0.0 : exp2(rest));
+  const double lse = log2(total);
+  if (lane == 0 && P.status && !(fabs(lse) < inf)) atomicOr(P.status, (int)VINFER_ST_NONFINITE);
+  // the target's masses
+  double mass = L.mass, pt = 0, norm = 1, lnorm = 0;
+  if (P.tail) {
+    pt = L.distinct < P.V ? fmax(0.0, 1.0 - mass) : 0.0;
+  } else if (mass > 0) {
+    norm = 1.0 / mass;
+    lnorm = log(mass);
+    mass = 1.0;
+  }
+  const double M = mass + pt;
+  double loss = 0;
+  for (int j = lane; j < P.k; j += 32) {
+    const double z = L.z[j] - lse, p = L.p[j];
+    if (p > 0) loss += p * norm * (((double)L.l[j] - lnorm) - z * LN2_D);
+    if (listg) listg[j] = L.id[j] >= 0 ? (float)(M * exp2(z) - L.psum[j] * norm) : 0.f;
+  }
+  loss = warp_sum(loss);
+  if (pt > 0) loss += pt * (log(pt) - (rest - lse) * LN2_D);
+  if (lse != lse) loss = lse;
+  if (stat) {
+    Stat t = {0.f, 0.f};
+    if (r != 0) t = Stat{m, (float)((M * exp2(rest - lse) - pt) / r)};
+    if (lse != lse) t = Stat{nan, nan};
+    *stat = t;
+  }
+  return (float)loss;
+}
+
+constexpr int FW = 4;  // rows of a finishing CTA, one a warp
+
+template <typename T>
+__global__ void __launch_bounds__(FW * 32) k_distill_finish(const DistP P) {
+  __shared__ ListS lists[FW];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * FW + w;
+  const bool there = row < P.rows;
+  const float weight = there && P.weights ? P.weights[row] : 1.f;
+  const bool live = there && weight != 0.f;
+  ListS& L = lists[w];
+  if (live) list_begin<T>(P, row, L);
   grid_dependency_wait();
   if (!there) return;
-  if (weight == 0.f) {
+  if (!live) {
     if (lane == 0) P.loss[row] = 0.f;
     return;
   }
-  bad = __any_sync(FULL, bad);
-  if (bad) {
-    const float nan = __int_as_float(0x7fffffff);
-    if (lane == 0) {
-      P.loss[row] = nan;
-      if (P.stat) P.stat[row] = Stat{nan, nan};
-      if (P.status) atomicOr(P.status, (int)VINFER_ST_BAD_LIST);
-    }
-    if (P.stat)
-      for (int j = lane; j < P.k; j += 32) P.listg[row * P.k + j] = nan;
-    return;
-  }
-  // the sum outside the list: r * 2^rest with rest = m * log2(e) / T
   float m = neg_inf();
-  for (int p = lane; p < P.parts; p += 32)
-    if (P.part[row * P.parts + p].s != 0.f) m = fmaxf(m, P.part[row * P.parts + p].m);
+  for (int p = lane; p < P.parts; p += 32) {
+    const Part h = P.part[row * P.parts + p];
+    if (h.s != 0.f) m = fmaxf(m, h.m);
+  }
   m = warp_max(m);
   double r = 0;
   for (int p = lane; p < P.parts; p += 32) {
@@ -166,86 +281,12 @@ __global__ void __launch_bounds__(NT) k_distill_finish(const DistP P) {
     if (h.s != 0.f) r += (double)h.s * exp2(((double)h.m - (double)m) * (double)P.scale);
   }
   r = warp_sum(r);
-  const double inf = (double)-neg_inf();
-  // all in distances from the row's largest logit `ref`, whatever its magnitude
-  double ref = r == 0 ? -inf : (double)m;
-  // the list
-  const T* x = static_cast<const T*>(P.logits) + row * P.ld;
-  double z[4], p[4], psum[4], mass = 0;
-  bool lead[4];  // the first entry that lists its id
-  int distinct = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = lane + 32 * i;
-    z[i] = -inf;
-    p[i] = psum[i] = 0;
-    lead[i] = false;
-    if (id[i] >= 0) {
-      z[i] = (double)Vec<T>::load(x + id[i]);
-      p[i] = exp((double)l[i]);
-      lead[i] = true;
-      for (int o = 0; o < P.k; ++o)
-        if (sid[w][o] == id[i]) {
-          if (o < j) lead[i] = false;
-          psum[i] += o == j ? p[i] : exp((double)sp[w][o]);
-        }
-      mass += p[i];
-      distinct += lead[i];
-      if (z[i] > ref || z[i] != z[i]) ref = z[i];
-    }
-  }
-  mass = warp_sum(mass);
-  distinct = (int)__reduce_add_sync(FULL, (unsigned)distinct);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const double t = __shfl_xor_sync(FULL, ref, o);
-    if (t > ref || t != t) ref = t;
-  }
-  double total = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    z[i] = (z[i] - ref) * P.scale_d;
-    if (lead[i]) total += exp2(z[i]);
-  }
-  const double rest = r == 0 ? -inf : ((double)m - ref) * P.scale_d + log2(r);
-  total = warp_sum(total) + (r == 0 ? 0.0 : exp2(rest));
-  const double lse = log2(total);  // of the distances
-  if (lane == 0 && P.status && !(fabs(lse) < inf)) atomicOr(P.status, (int)VINFER_ST_NONFINITE);
-  // target masses
-  double pt = 0, norm = 1, lnorm = 0;
-  if (P.tail) {
-    pt = distinct < P.V ? fmax(0.0, 1.0 - mass) : 0.0;
-  } else if (mass > 0) {
-    norm = 1.0 / mass;
-    lnorm = log(mass);
-    mass = 1.0;
-  }
-  const double qt = r == 0 ? 0.0 : exp2(rest - lse);
-  double loss = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (p[i] > 0) loss += p[i] * norm * (((double)l[i] - lnorm) - (z[i] - lse) * LN2_D);
-  loss = warp_sum(loss);
-  if (pt > 0) loss += pt * (log(pt) - (rest - lse) * LN2_D);
-  if (lse != lse) loss = lse;
-  if (lane == 0) P.loss[row] = (float)(loss * (double)weight);
-  if (!P.stat) return;
-  const double M = mass + pt;
+  Stat st;
+  const float loss = list_finish(P, L, m, r, P.stat ? &st : nullptr,
+                                 P.stat ? P.listg + row * P.k : nullptr);
   if (lane == 0) {
-    Stat t = {0.f, 0.f};
-    if (r != 0) {
-      t.m = m;
-      t.coef = (float)((M * qt - pt) / r);
-    }
-    if (lse != lse) t.m = t.coef = __int_as_float(0x7fffffff);
-    P.stat[row] = t;
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int j = lane + 32 * i;
-    if (j < P.k)
-      P.listg[row * P.k + j] =
-          id[i] >= 0 ? (float)(M * exp2(z[i] - lse) - psum[i] * norm) : 0.f;
+    P.loss[row] = loss * weight;
+    if (P.stat) P.stat[row] = st;
   }
 }
 
@@ -350,7 +391,7 @@ int launch_loss(const DistP& P, cudaStream_t st) {
   const size_t smem = (size_t)(part_vecs + 31) / 32 * 4;
   const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, smem, st, false, P);
   if (rc != VINFER_OK) return rc;
-  return launch(k_distill_finish<T>, (unsigned)((P.rows + NW - 1) / NW), NT, 0, st, true, P);
+  return launch(k_distill_finish<T>, (unsigned)((P.rows + FW - 1) / FW), FW * 32, 0, st, true, P);
 }
 
 template <typename T>

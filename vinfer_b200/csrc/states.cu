@@ -20,6 +20,7 @@ namespace {
 using namespace rows;
 
 constexpr int NT = 256;
+constexpr int CTAS = 4;         // CTAs of an SM: 64 KiB of copies in flight
 constexpr int UV = 4;           // vectors a thread copies per item, all loads before the stores
 constexpr int MAX_STATES = 64;  // tensors of one launch (they travel as kernel parameters)
 constexpr int OUTER = VINFER_STATE_MAX_OUTER;
@@ -28,13 +29,15 @@ struct Desc {
   const unsigned char* src;
   unsigned char* dst;
   int64_t src_slot, dst_slot;   // byte strides of the slot dimension
-  int64_t size[OUTER], src_st[OUTER], dst_st[OUTER];
-  int64_t run;                  // contiguous bytes
-  int64_t vecs;                 // vectors of one slot: outer sizes x run / vec
-  int64_t chunks;               // items of one moved slot
-  int64_t unit;                 // bytes of one position of the run, 0: lengths do not cut the run
-  int64_t len_max;              // positions along the length dimension
+  int64_t src_st[OUTER], dst_st[OUTER];
+  uint32_t size[OUTER];         // outer dimensions, the last n_outer places
+  uint32_t run_vecs;            // vectors of a run
+  uint32_t vecs;                // vectors of one slot: outer sizes x run_vecs
+  uint32_t chunks;              // items of one moved slot
+  uint32_t unit_vecs;           // vectors of one position of the run, 0: lengths do not cut it
+  int32_t len_max;              // positions along the length dimension
   int32_t len_outer;            // the outer dimension that lengths cut, -1: none
+  int32_t n_outer;
   int32_t vec;                  // bytes of a vector: 16, 8, 4, 2 or 1
 };
 
@@ -47,36 +50,42 @@ struct StatesP {
   int* status;
 };
 
+// One item: NT * UV vectors of slot `from` to slot `to`. 32-bit index arithmetic, and divisions only
+// where runs are shorter than an item or lie under several outer dimensions.
 template <typename VT>
-__device__ __forceinline__ void copy_item(const Desc& D, int from, int to, int64_t chunk, int len) {
+__device__ __forceinline__ void copy_item(const Desc& D, int from, int to, uint32_t chunk, int len) {
+  constexpr uint32_t SPAN = NT * UV;
   const unsigned char* src = D.src + (int64_t)from * D.src_slot;
   unsigned char* dst = D.dst + (int64_t)to * D.dst_slot;
-  const int64_t run_vecs = D.run / (int64_t)sizeof(VT);
-  const int64_t end = D.unit ? (int64_t)len * D.unit : D.run;  // live bytes of a run
+  const uint32_t rv = D.run_vecs, i0 = chunk * SPAN;
+  const uint32_t o0 = D.n_outer ? i0 / rv : 0, r0 = i0 - o0 * rv;
+  const uint32_t end = D.unit_vecs ? (uint32_t)len * D.unit_vecs : rv;  // live vectors of a run
+  if (r0 >= end && r0 + SPAN <= rv) return;
   VT v[UV];
   int64_t at[UV];
 #pragma unroll
   for (int u = 0; u < UV; ++u) {
-    const int64_t i = (chunk * UV + u) * NT + threadIdx.x;
-    at[u] = -1;
-    if (i < D.vecs) {
-      int64_t o = i / run_vecs;
-      const int64_t r = (i - o * run_vecs) * (int64_t)sizeof(VT);
-      int64_t so = r, po = r;
-      bool live = r < end;
-#pragma unroll
-      for (int k = OUTER - 1; k >= 0; --k) {
-        const int64_t q = o / D.size[k], x = o - q * D.size[k];
-        o = q;
-        so += x * D.src_st[k];
-        po += x * D.dst_st[k];
-        if (k == D.len_outer) live = live && x < len;
-      }
-      if (live) {
-        v[u] = *reinterpret_cast<const VT*>(src + so);
-        at[u] = po;
-      }
+    const uint32_t step = u * NT + threadIdx.x;
+    uint32_t r = r0 + step, o = o0;
+    if (r >= rv && D.n_outer) {
+      const uint32_t q = rv >= SPAN ? 1 : r / rv;
+      o += q;
+      r -= q * rv;
     }
+    bool live = i0 + step < D.vecs && r < end;
+    int64_t so = (int64_t)r * sizeof(VT), po = so;
+    for (int k = OUTER - 1; k >= OUTER - D.n_outer; --k) {
+      uint32_t x = o;
+      if (k > OUTER - D.n_outer) {
+        o /= D.size[k];
+        x -= o * D.size[k];
+      }
+      so += x * D.src_st[k];
+      po += x * D.dst_st[k];
+      if (k == D.len_outer) live = live && (int)x < len;
+    }
+    at[u] = live ? po : -1;
+    if (live) v[u] = *reinterpret_cast<const VT*>(src + so);
   }
 #pragma unroll
   for (int u = 0; u < UV; ++u)
@@ -84,11 +93,11 @@ __device__ __forceinline__ void copy_item(const Desc& D, int from, int to, int64
 }
 
 // Dynamic shared memory: one packed move (source << 16 | slot) a slot.
-__global__ void __launch_bounds__(NT) k_reorder(const __grid_constant__ StatesP P) {
+__global__ void __launch_bounds__(NT, CTAS) k_reorder(const __grid_constant__ StatesP P) {
   extern __shared__ uint32_t moves[];
   __shared__ int wcnt[NT / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int M = 0;  // the slots that move, ascending: every CTA makes the same list
+  uint32_t M = 0;  // the slots that move, ascending: every CTA makes the same list
   for (int s0 = 0; s0 < P.slots; s0 += NT) {
     const int s = s0 + threadIdx.x;
     bool move = false;
@@ -102,7 +111,7 @@ __global__ void __launch_bounds__(NT) k_reorder(const __grid_constant__ StatesP 
     const unsigned m = __ballot_sync(FULL, move);
     if (lane == 0) wcnt[w] = __popc(m);
     __syncthreads();
-    int at = M + __popc(m & ((1u << lane) - 1));
+    uint32_t at = M + __popc(m & ((1u << lane) - 1));
     for (int i = 0; i < NT / 32; ++i) {
       if (i < w) at += wcnt[i];
       M += wcnt[i];
@@ -111,17 +120,15 @@ __global__ void __launch_bounds__(NT) k_reorder(const __grid_constant__ StatesP 
     __syncthreads();
   }
   // items: the moves of a chunk side by side, chunk after chunk, tensor after tensor
-  int64_t g = blockIdx.x;
+  uint32_t g = blockIdx.x;
   for (int t = 0; t < P.n; ++t) {
     const Desc& D = P.d[t];
-    const int64_t items = D.chunks * M;
+    const uint32_t items = D.chunks * M;
     for (; g < items; g += gridDim.x) {
-      const int64_t chunk = g / M;
-      const uint32_t mv = moves[g - chunk * M];
+      const uint32_t chunk = g / M, mv = moves[g - chunk * M];
       const int from = mv >> 16, to = mv & 0xffff;
       int len = 0;
-      if (D.unit || D.len_outer >= 0)
-        len = (int)min((int64_t)max(P.lengths[to], 0), D.len_max);
+      if (D.unit_vecs || D.len_outer >= 0) len = min(max(P.lengths[to], 0), D.len_max);
       switch (D.vec) {
         case 16: copy_item<uint4>(D, from, to, chunk, len); break;
         case 8: copy_item<uint2>(D, from, to, chunk, len); break;
@@ -132,6 +139,46 @@ __global__ void __launch_bounds__(NT) k_reorder(const __grid_constant__ StatesP 
     }
     g -= items;
   }
+}
+
+// A state as the kernel takes it.
+int describe(const VinferState& s, int64_t slots, Desc* out) {
+  Desc& D = *out;
+  D = Desc{};
+  D.src = static_cast<const unsigned char*>(s.src);
+  D.dst = static_cast<unsigned char*>(s.dst);
+  D.src_slot = s.src_slot_stride;
+  D.dst_slot = s.dst_slot_stride;
+  D.n_outer = s.n_outer;
+  D.len_outer = -1;
+  uint64_t bits = (uint64_t)(uintptr_t)s.src | (uint64_t)(uintptr_t)s.dst |
+                  (uint64_t)s.src_slot_stride | (uint64_t)s.dst_slot_stride |
+                  (uint64_t)s.run_bytes | (uint64_t)s.len_unit_bytes | 16;
+  int64_t len_max = s.len_unit_bytes ? s.run_bytes / s.len_unit_bytes : 0;
+  int64_t outer = 1;
+  for (int j = 0; j < s.n_outer; ++j) {
+    const int k = OUTER - s.n_outer + j;
+    if (s.outer_size[j] > (int64_t)INT32_MAX / outer) return VINFER_E_LIMIT;
+    D.size[k] = (uint32_t)s.outer_size[j];
+    D.src_st[k] = s.src_outer_stride[j];
+    D.dst_st[k] = s.dst_outer_stride[j];
+    if (j == s.len_outer) {
+      D.len_outer = k;
+      len_max = s.outer_size[j];
+    }
+    bits |= (uint64_t)D.src_st[k] | (uint64_t)D.dst_st[k];
+    outer *= s.outer_size[j];
+  }
+  D.vec = (int)(bits & (~bits + 1));  // the lowest set bit divides every address and size
+  const int64_t run_vecs = s.run_bytes / D.vec;
+  if (run_vecs > (int64_t)INT32_MAX / outer) return VINFER_E_LIMIT;
+  D.run_vecs = (uint32_t)run_vecs;
+  D.vecs = (uint32_t)(outer * run_vecs);
+  D.unit_vecs = (uint32_t)(s.len_unit_bytes / D.vec);
+  D.len_max = (int32_t)len_max;
+  D.chunks = (D.vecs + (uint32_t)(NT * UV) - 1) / (uint32_t)(NT * UV);
+  if ((int64_t)D.chunks * slots > (int64_t)INT32_MAX) return VINFER_E_LIMIT;
+  return VINFER_OK;
 }
 
 }  // namespace
@@ -153,6 +200,11 @@ extern "C" int vinfer_reorder_states(const VinferState* states, int32_t n_states
     for (int k = 0; k < s.n_outer; ++k)
       if (s.outer_size[k] < 1) return VINFER_E_ARG;
   }
+  Desc d;
+  for (int i = 0; i < n_states; ++i) {  // nothing is copied unless everything can be
+    const int rc = describe(states[i], slots, &d);
+    if (rc != VINFER_OK) return rc;
+  }
   for (int i0 = 0; i0 < n_states; i0 += MAX_STATES) {
     StatesP P = {};
     P.n = std::min(MAX_STATES, n_states - i0);
@@ -163,39 +215,11 @@ extern "C" int vinfer_reorder_states(const VinferState* states, int32_t n_states
     P.status = status;
     int64_t chunks = 0;
     for (int i = 0; i < P.n; ++i) {
-      const VinferState& s = states[i0 + i];
-      Desc& D = P.d[i];
-      D.src = static_cast<const unsigned char*>(s.src);
-      D.dst = static_cast<unsigned char*>(s.dst);
-      D.src_slot = s.src_slot_stride;
-      D.dst_slot = s.dst_slot_stride;
-      D.run = s.run_bytes;
-      D.unit = s.len_unit_bytes;
-      D.len_outer = -1;
-      uint64_t bits = (uint64_t)(uintptr_t)s.src | (uint64_t)(uintptr_t)s.dst |
-                      (uint64_t)s.src_slot_stride | (uint64_t)s.dst_slot_stride |
-                      (uint64_t)s.run_bytes | (uint64_t)s.len_unit_bytes | 16;
-      D.len_max = D.unit ? s.run_bytes / D.unit : 0;
-      int64_t outer = 1;
-      for (int k = 0; k < OUTER; ++k) {  // the dimensions given, behind ones of size 1
-        const int from = k - (OUTER - s.n_outer);
-        D.size[k] = from >= 0 ? s.outer_size[from] : 1;
-        D.src_st[k] = from >= 0 ? s.src_outer_stride[from] : 0;
-        D.dst_st[k] = from >= 0 ? s.dst_outer_stride[from] : 0;
-        if (from >= 0 && from == s.len_outer) {
-          D.len_outer = k;
-          D.len_max = D.size[k];
-        }
-        bits |= (uint64_t)D.src_st[k] | (uint64_t)D.dst_st[k];
-        outer *= D.size[k];
-      }
-      D.vec = (int)(bits & (~bits + 1));  // the lowest set bit divides every address and size
-      D.vecs = outer * (s.run_bytes / D.vec);
-      D.chunks = (D.vecs + (int64_t)NT * UV - 1) / ((int64_t)NT * UV);
-      chunks += D.chunks;
+      describe(states[i0 + i], slots, &P.d[i]);
+      chunks += P.d[i].chunks;
     }
-    // every slot may move: no more CTAs than items, eight of 256 threads an SM at most
-    const int64_t grid = std::min<int64_t>(148 * 8, chunks * slots);
+    // every slot may move: no more CTAs than items, at most what is resident
+    const int64_t grid = std::min<int64_t>(148 * CTAS, chunks * slots);
     const size_t smem = (size_t)slots * 4;
     if (opt_in(k_reorder, smem) != VINFER_OK) return VINFER_E_CUDA;
     const int rc = launch(k_reorder, (unsigned)grid, NT, smem, (cudaStream_t)stream, false, P);
