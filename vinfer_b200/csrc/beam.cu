@@ -351,8 +351,6 @@ struct PickS {
   int head[MAXN];             // ranked candidates: beam << 16 | place in its list
   int eos[VINFER_BEAM_MAX_EOS];
   uint32_t flags;             // beams whose sums are taken again
-  int alive;                  // surviving candidates
-  float kth[PW];
   double red[PW];
   int sel[MAXW];              // continuing candidates: their ranks
 };
@@ -386,7 +384,7 @@ __device__ void row_sum_double(const RowsP& P, int row, double* red, double* m_o
 }
 
 // One CTA a request. Dynamic shared memory: the staged entries of its parts [W, parts, n], the
-// beams' lists [W, n], the survivors' scores and places [W * n] each.
+// beams' lists [W, n] and their scores [W, n].
 template <typename T>
 __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
   extern __shared__ __align__(16) unsigned char dyn[];
@@ -397,11 +395,7 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
   u64* staged = reinterpret_cast<u64*>(dyn);
   u64* lists = staged + W * per;
   double* sc = reinterpret_cast<double*>(lists + W * n);
-  unsigned short* live = reinterpret_cast<unsigned short*>(sc + W * n);
-  if (tid == 0) {
-    S.flags = 0;
-    S.alive = 0;
-  }
+  if (tid == 0) S.flags = 0;
   if (tid < W) S.b[tid] = P.scores[(int64_t)req * W + tid];
   if (tid < Q.n_eos) S.eos[tid] = Q.eos[tid];
   grid_dependency_wait();
@@ -442,26 +436,25 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
     } else if (!(s > 0 && s < (double)FLT_MAX)) {
       bad = VINFER_ST_NONFINITE;  // a NaN or +inf, or every logit -inf
     } else {
-      // n best of the parts' lists. Every lane's k-th best bounds the n-th best of all from below
-      // (32k >= n); what reaches the least of them survives, and is ranked by counting.
+      // n best of the parts' lists, which are sorted: with parts * (d + 1) >= n the largest of the
+      // parts' entries at depth d bounds the n-th best from below, and with as many parts as
+      // entries the n-th best of their first ones. What reaches it is ranked by counting.
       u64* mine = staged + beam * per;
-      const int k = (n + 31) / 32;
-      u64 t[4] = {NONE, NONE, NONE, NONE};  // this lane's best, ascending
-      if (k == 1) {
-        for (int i = lane; i < per; i += 32) t[0] = mine[i] < t[0] ? mine[i] : t[0];
-      } else {
-        for (int i = lane; i < per; i += 32) {
-          u64 e = mine[i];
-#pragma unroll
-          for (int a = 0; a < 4; ++a)
-            if (e < t[a]) {
-              const u64 o = t[a];
-              t[a] = e;
-              e = o;
-            }
+      const int d = (n + P.parts - 1) / P.parts - 1;
+      const u64 h0 = lane < P.parts ? mine[lane * n + d] : 0;
+      const u64 h1 = lane + 32 < P.parts ? mine[(lane + 32) * n + d] : 0;
+      u64 bound = h0 > h1 ? h0 : h1;
+      if (d == 0 && P.parts > n) {
+        int r0 = 0, r1 = 0;
+        for (int o = 0; o < P.parts; ++o) {
+          const u64 h = mine[o * n];
+          r0 += h < h0 || (h == h0 && o < lane);
+          r1 += h < h1 || (h == h1 && o < lane + 32);
         }
+        bound = 0;
+        if (lane < P.parts && r0 == n - 1) bound = h0;
+        if (lane + 32 < P.parts && r1 == n - 1) bound = h1;
       }
-      u64 bound = k == 1 ? t[0] : k == 2 ? t[1] : k == 3 ? t[2] : t[3];
 #pragma unroll
       for (int o = 16; o; o >>= 1) {
         const u64 other = __shfl_xor_sync(FULL, bound, o);
@@ -496,48 +489,33 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
     return (double)S.b[beam] +
            (((double)entry_x(lists[beam * n + j]) - S.m[beam]) - S.lns[beam]);
   };
-  // candidates that can be among the n best, or within NEAR of the last of them
-  {
-    float mine = neg_inf();
-    for (int i = tid; i < W * n; i += PT) {
-      const int beam = i / n, j = i - beam * n;
-      if (j < S.cnt[beam]) {
-        sc[i] = score(beam, j);
-        mine = fmaxf(mine, __double2float_rd(sc[i]));
-      }
-    }
-    uint32_t key = okey(mine), top = 0;
-    for (int a = (n + PW - 1) / PW; a > 0; --a) {
-      top = __reduce_max_sync(FULL, key);
-      const unsigned who = __ballot_sync(FULL, key == top);
-      if (lane == __ffs(who) - 1) key = 0;
-    }
-    if (lane == 0) S.kth[w] = top ? from_okey(top) : neg_inf();
-    __syncthreads();
-    float t = S.kth[0];
-    for (int i = 1; i < PW; ++i) t = fminf(t, S.kth[i]);
-    for (int i = tid; i < W * n; i += PT) {
-      const int beam = i / n, j = i - beam * n;
-      if (j < S.cnt[beam] && sc[i] >= (double)t - 2 * NEAR)
-        live[atomicAdd(&S.alive, 1)] = (unsigned short)(beam << 8 | j);
-    }
-    __syncthreads();
-  }
   for (int pass = 0; pass < 2; ++pass) {
-    for (int i = tid; i < S.alive; i += PT) {
-      const int bi = live[i] >> 8, ji = live[i] & 255;
-      const double si = sc[bi * n + ji];
-      int rank = 0;
+    for (int i = tid; i < W * n; i += PT) {
+      const int beam = i / n, j = i - beam * n;
+      sc[i] = j < S.cnt[beam] ? score(beam, j) : -HUGE_VAL;
+    }
+    __syncthreads();
+    // A candidate's place: its place in its own list and, by bisection, how many of every other
+    // list are better (higher, or equal from an earlier beam). Its neighbours there show scores
+    // that are too close to order.
+    for (int i = tid; i < W * n; i += PT) {
+      const int bi = i / n, ji = i - bi * n;
+      if (ji >= S.cnt[bi]) continue;
+      const double si = sc[i];
+      int rank = ji;
       uint32_t close = 0;
-      for (int k = 0; k < S.alive; ++k) {
-        const int bk = live[k] >> 8, jk = live[k] & 255;
-        const double sk = sc[bk * n + jk];
-        if (bk == bi) {
-          rank += jk < ji;
-        } else {
-          rank += sk > si || (sk == si && bk < bi);
-          if (fabs(sk - si) <= NEAR) close |= 1u << bk;
+      for (int k = 0; k < W && rank < n; ++k) {
+        if (k == bi) continue;
+        const double* o = sc + k * n;
+        int lo = 0, hi = S.cnt[k];
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (o[mid] > si || (o[mid] == si && k < bi)) lo = mid + 1;
+          else hi = mid;
         }
+        rank += lo;
+        if ((lo > 0 && o[lo - 1] - si <= NEAR) || (lo < S.cnt[k] && si - o[lo] <= NEAR))
+          close |= 1u << k;
       }
       if (rank < n) {
         S.head[rank] = bi << 16 | ji;
@@ -551,15 +529,12 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
       if (flags >> beam & 1)
         row_sum_double<T>(P, req * W + beam, S.red, &S.m[beam], &S.lns[beam]);
     __syncthreads();
-    for (int i = tid; i < S.alive; i += PT) {
-      const int beam = live[i] >> 8, j = live[i] & 255;
-      sc[beam * n + j] = score(beam, j);
-    }
-    __syncthreads();
   }
 
   // the list of candidates
-  const int have = min(S.alive, n);
+  int have = 0;  // candidates there are
+  for (int k = 0; k < W; ++k) have += S.cnt[k];
+  have = min(have, n);
   for (int i = tid; i < n; i += PT) {
     const int64_t o = (int64_t)req * n + i;
     if (i < have) {
@@ -633,7 +608,7 @@ int beam_parts(int64_t rows, int W, int64_t vocab, int dtype, int n) {
 }
 
 size_t pick_smem(int W, int n, int parts) {
-  return (size_t)W * n * (8 * (size_t)parts + 8 + 8 + 2);
+  return (size_t)W * n * (8 * (size_t)parts + 8 + 8);
 }
 
 bool beam_shape_ok(int64_t requests, int32_t beams, int64_t vocab, int32_t dtype, int32_t n) {
