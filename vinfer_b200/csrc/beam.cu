@@ -249,12 +249,7 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
   for (int vb = v0; vb < v1; vb += NT * U, ++round) {
     uint4 q[U];
     R.template load_round<U, NT>(vb, v1, q);
-    float vm[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) vm[u] = V8::max(q[u]);
-    float mx = vm[0];
-#pragma unroll
-    for (int u = 1; u < U; ++u) mx = fmaxf(mx, vm[u]);
+    const float mx = V8::max(q);
     seen = fmaxf(seen, mx);
     if ((round & (round + 1)) == 0) {  // rounds 0, 1, 3, 7, ...
       uint32_t key = okey(seen), top = 0;
@@ -269,17 +264,19 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
     float bar = kth[0];
 #pragma unroll
     for (int i = 1; i < NW; ++i) bar = fminf(bar, kth[i]);
+    if (__any_sync(FULL, mx >= bar)) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool keep = vm[u] >= bar;
-      const unsigned who = __ballot_sync(FULL, keep);
-      if (who) {
-        int at = 0;
-        if (lane == 0) at = atomicAdd(&S.nd, __popc(who));
-        at = __shfl_sync(FULL, at, 0) + __popc(who & ((1u << lane) - 1));
-        if (keep && at < DCAP) {
-          D.q[at] = q[u];
-          D.e0[at] = (vb + u * NT + tid) * A - R.off;
+      for (int u = 0; u < U; ++u) {
+        const bool keep = V8::max(q[u]) >= bar;
+        const unsigned who = __ballot_sync(FULL, keep);
+        if (who) {
+          int at = 0;
+          if (lane == 0) at = atomicAdd(&S.nd, __popc(who));
+          at = __shfl_sync(FULL, at, 0) + __popc(who & ((1u << lane) - 1));
+          if (keep && at < DCAP) {
+            D.q[at] = q[u];
+            D.e0[at] = (vb + u * NT + tid) * A - R.off;
+          }
         }
       }
     }

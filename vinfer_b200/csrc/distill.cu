@@ -65,7 +65,8 @@ __device__ __noinline__ uint4 without(uint4 q, int v, const int* hit, int hits) 
   return q;
 }
 
-// Dynamic shared memory: one bit for each vector of the part, set where it holds a listed element.
+// Dynamic shared memory: one bit for each vector of the part's rounds, set where it holds a listed
+// element.
 template <typename T>
 __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   using VT = Vec<T>;
@@ -81,7 +82,7 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   const int v0 = (int)((int64_t)R.nv * part / P.parts);
   const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
   const int id = tid < P.k ? P.ids[row * P.k + tid] : -1;
-  for (int i = tid; i < (v1 - v0 + 31) / 32; i += NT) marked[i] = 0;
+  for (int i = tid; i < (v1 - v0 + NT * U - 1) / (NT * U) * (NT * U / 32); i += NT) marked[i] = 0;
   if (tid == 0) hits = 0;
   __syncthreads();
   {
@@ -96,17 +97,12 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   for (int vb = v0; vb < v1; vb += NT * U) {
     uint4 q[U];
     R.template load_round<U, NT>(vb, v1, q);
-    if (hits) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int v = vb - v0 + u * NT + tid;
-        if (v < v1 - v0 && marked[v / 32] >> (v & 31) & 1) q[u] = without<T>(q[u], v, hit, hits);
-      }
+    for (int u = 0; u < U; ++u) {  // a warp's 32 vectors are one word (and zeros behind the part)
+      const uint32_t word = marked[(vb - v0 + u * NT) / 32 + tid / 32];
+      if (word && word >> (tid & 31) & 1) q[u] = without<T>(q[u], vb - v0 + u * NT + tid, hit, hits);
     }
-    float mx = VT::max(q[0]);
-#pragma unroll
-    for (int u = 1; u < U; ++u) mx = fmaxf(mx, VT::max(q[u]));
-    add_exps<T>(q, mx, P.scale, m, s);
+    add_exps<T>(q, VT::max(q), P.scale, m, s);
   }
   block_join<NW>(m, s, P.scale, sm);
   if (tid == 0) P.part[blockIdx.x] = Part{m, s};
@@ -308,6 +304,8 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
   Stat st = {0.f, 0.f};
   if (f != 0.f) st = P.stat[row];
   const float coef = f * st.coef;
+  const uint64_t neg_m = pair(-st.m, -st.m), scale = pair(P.scale, P.scale);
+  const uint64_t coef2 = pair(coef, coef);
   for (int vb = v0; vb < v1; vb += NT * U) {
     uint4 q[U];
     if (f != 0.f) R.template load_round<U, NT>(vb, v1, q);
@@ -317,9 +315,11 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
       if (v < v1) {
         float g[A];
         if (f != 0.f) {
-          VT::unpack(q[u], g);
+          uint64_t h[A / 2];
+          VT::pairs(q[u], h);
 #pragma unroll
-          for (int j = 0; j < A; ++j) g[j] = coef * ex2((g[j] - st.m) * P.scale);
+          for (int j = 0; j < A / 2; ++j)
+            split(mul2(ex2_2(mul2(add2(h[j], neg_m), scale)), coef2), g[2 * j], g[2 * j + 1]);
         } else {
 #pragma unroll
           for (int j = 0; j < A; ++j) g[j] = 0.f;
@@ -388,7 +388,7 @@ DistP params(const VinferDistillArgs* a) {
 template <typename T>
 int launch_loss(const DistP& P, cudaStream_t st) {
   const int part_vecs = (P.V / Vec<T>::A + 2 + P.parts - 1) / P.parts + 1;
-  const size_t smem = (size_t)(part_vecs + 31) / 32 * 4;
+  const size_t smem = (size_t)(part_vecs + NT * U - 1) / (NT * U) * (NT * U / 8);
   const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, smem, st, false, P);
   if (rc != VINFER_OK) return rc;
   return launch(k_distill_finish<T>, (unsigned)((P.rows + FW - 1) / FW), FW * 32, 0, st, true, P);

@@ -28,6 +28,36 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// two floats in one 64-bit register: sm_100 multiplies and adds them in one instruction
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t ex2_2(uint64_t a) {
+  float x, y;
+  split(a, x, y);
+  return pair(ex2(x), ex2(y));
+}
+
 // order-preserving key of a float; -0 folds into +0
 __device__ __forceinline__ uint32_t okey(float v) {
   const uint32_t b = __float_as_uint(__fadd_rn(v, 0.0f));
@@ -51,6 +81,28 @@ struct Vec<__nv_bfloat16> {
       f[2 * i] = __uint_as_float(w[i] << 16);
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
+  }
+  // pairs of floats, in element order
+  static __device__ __forceinline__ void pairs(const uint4& q, uint64_t (&f)[4]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  // largest element of U vectors, NaN ignored: packed comparisons, unpacked once
+  template <int U>
+  static __device__ __forceinline__ float max(const uint4 (&q)[U]) {
+    __nv_bfloat162 m[4];
+    memcpy(m, &q[0], 16);
+#pragma unroll
+    for (int u = 1; u < U; ++u) {
+      __nv_bfloat162 x[4];
+      memcpy(x, &q[u], 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) m[i] = __hmax2(m[i], x[i]);
+    }
+    const __nv_bfloat162 r = __hmax2(__hmax2(m[0], m[1]), __hmax2(m[2], m[3]));
+    return fmaxf(__low2float(r), __high2float(r));
   }
   // largest element, NaN ignored (two packed comparisons a word pair)
   static __device__ __forceinline__ float max(const uint4& q) {
@@ -103,6 +155,17 @@ struct Vec<float> {
     f[2] = __uint_as_float(q.z);
     f[3] = __uint_as_float(q.w);
   }
+  static __device__ __forceinline__ void pairs(const uint4& q, uint64_t (&f)[2]) {
+    f[0] = pair(__uint_as_float(q.x), __uint_as_float(q.y));
+    f[1] = pair(__uint_as_float(q.z), __uint_as_float(q.w));
+  }
+  template <int U>
+  static __device__ __forceinline__ float max(const uint4 (&q)[U]) {
+    float m = max(q[0]);
+#pragma unroll
+    for (int u = 1; u < U; ++u) m = fmaxf(m, max(q[u]));
+    return m;
+  }
   static __device__ __forceinline__ float max(const uint4& q) {
     return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)),
                  fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
@@ -153,13 +216,21 @@ struct Row {
     }
     return edge(p, V, v * Vec<T>::A - off);
   }
-  // The thread's vectors vb + u * NT + threadIdx.x of a round, below v1; -inf behind it. Predicated
-  // loads without branches between them, so that all are in flight together; the row's ragged ends
-  // are read behind them.
+  // The thread's vectors vb + u * NT + threadIdx.x of a round, below v1; -inf behind it. No
+  // branches between the loads, so that all are in flight together: rounds inside the row load
+  // at constant offsets, the others by predicate, and their ragged ends are read behind them.
   template <int U, int NT>
   __device__ __forceinline__ void load_round(int vb, int v1, uint4 (&q)[U]) const {
     const T* at = p + ((int64_t)(vb + (int)threadIdx.x) * Vec<T>::A - off);
     const int lo = off ? 1 : 0, hi = min(v1, (V + off) / Vec<T>::A);  // whole vectors
+    if (vb >= lo && vb + U * NT <= hi) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(q[u].x), "=r"(q[u].y), "=r"(q[u].z), "=r"(q[u].w)
+                     : "l"(at + u * NT * Vec<T>::A));
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int v = vb + u * NT + (int)threadIdx.x;
@@ -169,7 +240,7 @@ struct Row {
           "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\t"
           "@p ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n\t}"
           : "+r"(q[u].x), "+r"(q[u].y), "+r"(q[u].z), "+r"(q[u].w)
-          : "l"(at + (int64_t)u * NT * Vec<T>::A), "r"((uint32_t)(v >= lo && v < hi)));
+          : "l"(at + u * NT * Vec<T>::A), "r"((uint32_t)(v >= lo && v < hi)));
     }
     if (vb == 0 && off && threadIdx.x == 0) q[0] = edge(p, V, -off);
     if (hi < v1 && hi >= vb && hi < vb + U * NT && (hi > 0 || !off)) {  // the last, a ragged one
@@ -205,12 +276,13 @@ __device__ __forceinline__ double warp_sum(double v) {
 // value (a mask) need no exponent beyond the float's range, and the rounding of `scale` only
 // stretches distances from the maximum.
 
-// Adds the U vectors q, whose largest element is mx, to the thread's sum. One multiply-add, one
-// ex2 and one addition an element: the argument x * scale - c is rounded once, and what c misses
-// of m * scale is put right in the round's sum.
+// Adds the U vectors q, whose largest element is mx, to the thread's sum: an ex2 an element, and a
+// multiply-add and an addition for each two. The argument x * scale - c is rounded once, and
+// what c misses of m * scale is put right in the round's sum.
 template <typename T, int U>
 __device__ __forceinline__ void add_exps(const uint4 (&q)[U], float mx, float scale, float& m,
                                          float& s) {
+  constexpr int H = Vec<T>::A / 2;
   if (mx > m) {
     if (s != 0.f) s *= ex2((m - mx) * scale);
     m = mx;
@@ -219,15 +291,20 @@ __device__ __forceinline__ void add_exps(const uint4 (&q)[U], float mx, float sc
   const float c = ref * scale;
   float sum = 0.f;
   if (fabsf(c) < 1e37f) {
+    const uint64_t k = pair(scale, scale), d = pair(-c, -c);
+    uint64_t all = pair(0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float f[Vec<T>::A];
-      Vec<T>::unpack(q[u], f);
-      float t = 0.f;
+      uint64_t f[H];
+      Vec<T>::pairs(q[u], f);
+      uint64_t t = ex2_2(fma2(f[0], k, d));
 #pragma unroll
-      for (int j = 0; j < Vec<T>::A; ++j) t += ex2(fmaf(f[j], scale, -c));
-      sum += t;
+      for (int j = 1; j < H; ++j) t = add2(t, ex2_2(fma2(f[j], k, d)));
+      all = add2(all, t);
     }
+    float a, b;
+    split(all, a, b);
+    sum = a + b;
     const float lo = fmaf(ref, scale, -c);
     sum = fmaf(sum, -lo * (float)LN2_D, sum);
   } else {  // c near the float's range, or infinite: distances first
