@@ -57,7 +57,10 @@ def compare(x, ids, lp, w, temperature, tail, loss, grad=None):
     want_l, want_g = distill(xd, ids.cpu().numpy(), lp.double().cpu().numpy(),
                              w.double().cpu().numpy(), temperature, tail)
     tl, tg = tolerances(xd, temperature, want_l, want_g, x.dtype, w.double().cpu().numpy())
-    d = np.abs(loss.double().cpu().numpy() - want_l)
+    got = loss.double().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        d = np.where(got == want_l, 0.0, np.abs(got - want_l))  # an infinite loss is met exactly
+        tl = np.where(np.isfinite(want_l), tl, 0.0)
     assert np.all(d <= tl), (d.max(), np.argmax(d - tl))
     if grad is not None:
         assert grad.dtype == x.dtype
@@ -110,6 +113,36 @@ def test_matches_the_formulas(backend, N, V, k, T, pad, tail, dtype):
     compare(x, ids, lp, w, T, tail, loss, grad)
     for l, g in steps:
         compare(x, ids, lp, w, T, tail, l, g)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
+@pytest.mark.parametrize("N,V,k,pad", [(301, 32776, 9, 0), (310, 33001, 128, 0), (297, 50003, 33, 5),
+                                       (299, 120007, 20, 1), (610, 65536, 4, 0)])
+def test_many_long_rows(backend, N, V, k, pad, dtype):
+    """Rows taken whole by one CTA: more than the CTAs, ragged, masked, with bad lists among them."""
+    x, ids, lp, w = make(N, V, k, dtype, 1.5)
+    if pad:
+        wide = torch.zeros(N, V + pad, dtype=dtype)
+        wide[:, :V] = x
+        x = wide[:, :V]
+    w[3::7] = 0.0
+    w[-1] = 0.0
+    ids[5, 1:] = -1
+    ids[6, 1] = ids[6, 0]
+    ids[7] = torch.arange(k)            # neighbours in few vectors
+    ids[8, 0], ids[8, 1], ids[8, 2] = 0, V - 1, V - 2
+    x[9, 100:V - 5] = NEG
+    bad = [11, 13]
+    ids[11, 0] = V
+    x[13, 77] = float("nan")
+    good = [r for r in range(N) if r not in bad]
+    for tail in (False, True):
+        _, _, loss, grad, steps = run_all(backend, x, ids, lp, w, 1.5, tail,
+                                          _lib.ST_BAD_LIST | _lib.ST_NONFINITE)
+        rows = good if tail else good[:40]
+        for l, g in [(loss, grad), *steps]:
+            assert torch.isnan(l[bad]).all() and torch.isnan(g[bad]).all()
+            compare(x[rows], ids[rows], lp[rows], w[rows], 1.5, tail, l[rows], g[rows])
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])

@@ -57,12 +57,29 @@ struct DistP {
   int64_t ldg;
 };
 
-// Vector v of the part with its listed elements taken out.
+// Which elements of vector v are among the n places `at` (a place: element counted from the first
+// vector, -1: none): one bit each. The whole warp calls it with the same v.
+template <int A>
+__device__ __forceinline__ uint32_t listed_in(const int* at, int n, int v) {
+  uint32_t bits = 0;
+  for (int j = threadIdx.x & 31; j < n; j += 32)
+    if (at[j] >= 0 && at[j] / A == v) bits |= 1u << (at[j] & (A - 1));
+  return __reduce_or_sync(FULL, bits);
+}
+
+// Takes the listed elements out of the warp's vectors: lane l holds vector v0 + l, `word` has the
+// bit of each that holds one.
 template <typename T>
-__device__ __noinline__ uint4 without(uint4 q, int v, const int* hit, int hits) {
-  for (int h = 0; h < hits; ++h)
-    if (hit[h] / Vec<T>::A == v) Vec<T>::put(q, hit[h] & (Vec<T>::A - 1), Vec<T>::NEG_INF_BITS);
-  return q;
+__device__ __forceinline__ void take_out(uint4& q, uint32_t word, const int* at, int n, int v0) {
+  for (; word; word &= word - 1) {
+    const int l = __ffs(word) - 1;
+    const uint32_t bits = listed_in<Vec<T>::A>(at, n, v0 + l);
+    if ((threadIdx.x & 31) == l) {
+#pragma unroll
+      for (int j = 0; j < Vec<T>::A; ++j)
+        if (bits >> j & 1) Vec<T>::put(q, j, Vec<T>::NEG_INF_BITS);
+    }
+  }
 }
 
 // Dynamic shared memory: one bit for each vector of the part's rounds, set where it holds a listed
@@ -99,8 +116,8 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
     R.template load_round<U, NT>(vb, v1, q);
 #pragma unroll
     for (int u = 0; u < U; ++u) {  // a warp's 32 vectors are one word (and zeros behind the part)
-      const uint32_t word = marked[(vb - v0 + u * NT) / 32 + tid / 32];
-      if (word && word >> (tid & 31) & 1) q[u] = without<T>(q[u], vb - v0 + u * NT + tid, hit, hits);
+      const int first = vb - v0 + u * NT + (tid & ~31);
+      if (const uint32_t word = marked[first / 32]) take_out<T>(q[u], word, hit, hits, first);
     }
     add_exps<T>(q, VT::max(q), P.scale, m, s);
   }
@@ -193,21 +210,26 @@ __device__ __forceinline__ void list_begin(const DistP& P, int64_t row, ListS& L
   __syncwarp();
 }
 
-// The row's loss and gradient terms from the list and the sum outside it, (m, r) with r in units of
-// 2^(m * scale). listg[j]: dloss/dz of the j-th listed element.
-__device__ __forceinline__ float list_finish(const DistP& P, ListS& L, float m, double r,
-                                             Stat* stat, float* listg) {
+// The row solved: all in distances from its largest logit, whatever its magnitude, and in log2.
+struct Solved {
+  double lse;    // log-sum
+  double rest;   // ... of what is outside the list
+  double mass;   // the target's mass M
+  double pt;     // its tail
+  double norm, lnorm;  // a listed mass is p * norm, its logarithm l - lnorm
+  bool bad;
+};
+
+// From the list and the sum outside it, (m, r) with r in units of 2^(m * scale). Leaves ln q in L.z
+// (as log2 q).
+__device__ __forceinline__ Solved list_solve(const DistP& P, ListS& L, float m, double r) {
   const int lane = threadIdx.x & 31;
-  const float nan = __int_as_float(0x7fffffff);
+  const double inf = (double)-neg_inf();
+  Solved S = {0, 0, 0, 0, 1, 0, L.bad};
   if (L.bad) {
     if (lane == 0 && P.status) atomicOr(P.status, (int)VINFER_ST_BAD_LIST);
-    if (listg)
-      for (int j = lane; j < P.k; j += 32) listg[j] = nan;
-    if (stat) *stat = Stat{nan, nan};
-    return nan;
+    return S;
   }
-  // all in distances from the row's largest logit, whatever its magnitude, and in log2
-  const double inf = (double)-neg_inf();
   double ref = L.top;
   if (r != 0 && !(ref != ref) && (double)m > ref) ref = m;
   double total = 0;
@@ -215,35 +237,45 @@ __device__ __forceinline__ float list_finish(const DistP& P, ListS& L, float m, 
     L.z[j] = (L.z[j] - ref) * P.scale_d;
     if (L.lead[j]) total += exp2(L.z[j]);
   }
-  const double rest = r == 0 ? -inf : ((double)m - ref) * P.scale_d + log2(r);
-  total = warp_sum(total) + (r == 0 ? 0.0 : exp2(rest));
-  const double lse = log2(total);
-  if (lane == 0 && P.status && !(fabs(lse) < inf)) atomicOr(P.status, (int)VINFER_ST_NONFINITE);
-  // the target's masses
-  double mass = L.mass, pt = 0, norm = 1, lnorm = 0;
+  S.rest = r == 0 ? -inf : ((double)m - ref) * P.scale_d + log2(r);
+  total = warp_sum(total) + (r == 0 ? 0.0 : exp2(S.rest));
+  S.lse = log2(total);
+  for (int j = lane; j < P.k; j += 32) L.z[j] -= S.lse;
+  if (lane == 0 && P.status && !(fabs(S.lse) < inf))
+    atomicOr(P.status, (int)VINFER_ST_NONFINITE);
+  S.mass = L.mass;
   if (P.tail) {
-    pt = L.distinct < P.V ? fmax(0.0, 1.0 - mass) : 0.0;
-  } else if (mass > 0) {
-    norm = 1.0 / mass;
-    lnorm = log(mass);
-    mass = 1.0;
+    S.pt = L.distinct < P.V ? fmax(0.0, 1.0 - S.mass) : 0.0;
+  } else if (S.mass > 0) {
+    S.norm = 1.0 / S.mass;
+    S.lnorm = log(S.mass);
+    S.mass = 1.0;
   }
-  const double M = mass + pt;
+  S.mass += S.pt;
+  return S;
+}
+
+// The gradient's terms, times f: of the listed elements, and of those outside.
+__device__ __forceinline__ Stat list_grads(const DistP& P, const ListS& L, const Solved& S, float m,
+                                           double r, float f, float* listg) {
+  const float nan = __int_as_float(0x7fffffff);
+  const bool lost = S.bad || S.lse != S.lse;
+  for (int j = threadIdx.x & 31; j < P.k; j += 32)
+    listg[j] = lost          ? nan
+               : L.id[j] < 0 ? 0.f
+                             : f * (float)(S.mass * exp2(L.z[j]) - L.psum[j] * S.norm);
+  if (lost) return Stat{nan, nan};
+  if (r == 0) return Stat{0.f, 0.f};
+  return Stat{m, f * (float)((S.mass * exp2(S.rest - S.lse) - S.pt) / r)};
+}
+
+__device__ __forceinline__ float list_loss(const DistP& P, const ListS& L, const Solved& S) {
+  if (S.bad || S.lse != S.lse) return __int_as_float(0x7fffffff);
   double loss = 0;
-  for (int j = lane; j < P.k; j += 32) {
-    const double z = L.z[j] - lse, p = L.p[j];
-    if (p > 0) loss += p * norm * (((double)L.l[j] - lnorm) - z * LN2_D);
-    if (listg) listg[j] = L.id[j] >= 0 ? (float)(M * exp2(z) - L.psum[j] * norm) : 0.f;
-  }
+  for (int j = threadIdx.x & 31; j < P.k; j += 32)
+    if (L.p[j] > 0) loss += L.p[j] * S.norm * (((double)L.l[j] - S.lnorm) - L.z[j] * LN2_D);
   loss = warp_sum(loss);
-  if (pt > 0) loss += pt * (log(pt) - (rest - lse) * LN2_D);
-  if (lse != lse) loss = lse;
-  if (stat) {
-    Stat t = {0.f, 0.f};
-    if (r != 0) t = Stat{m, (float)((M * exp2(rest - lse) - pt) / r)};
-    if (lse != lse) t = Stat{nan, nan};
-    *stat = t;
-  }
+  if (S.pt > 0) loss += S.pt * (log(S.pt) - (S.rest - S.lse) * LN2_D);
   return (float)loss;
 }
 
@@ -277,13 +309,13 @@ __global__ void __launch_bounds__(FW * 32) k_distill_finish(const DistP P) {
     if (h.s != 0.f) r += (double)h.s * exp2(((double)h.m - (double)m) * (double)P.scale);
   }
   r = warp_sum(r);
-  Stat st;
-  const float loss = list_finish(P, L, m, r, P.stat ? &st : nullptr,
-                                 P.stat ? P.listg + row * P.k : nullptr);
-  if (lane == 0) {
-    P.loss[row] = loss * weight;
-    if (P.stat) P.stat[row] = st;
+  const Solved S = list_solve(P, L, m, r);
+  if (P.stat) {
+    const Stat st = list_grads(P, L, S, m, r, 1.f, P.listg + row * P.k);
+    if (lane == 0) P.stat[row] = st;
   }
+  const float loss = list_loss(P, L, S);
+  if (lane == 0) P.loss[row] = loss * weight;
 }
 
 template <typename T>
@@ -345,6 +377,294 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
   }
 }
 
+// ---- loss and gradient in one pass ------------------------------------------------------------
+// One persistent CTA an SM takes whole rows. A producer thread streams a row's chunks into a ring of
+// shared memory by bulk copies; CW warps sum them, releasing each chunk until the ring can hold the
+// rest of the row; the list's warp solves the row; the CW warps then write the gradient of the
+// chunks the ring still holds, and of the others, which the producer brings once more (from L2:
+// every SM re-reads what it read some microseconds before). HBM sees each row read once and written
+// once. While a row is solved and written, the producer fills the ring with the next row, and
+// the list's warp prepares the next list.
+constexpr int CW = 16, CT = CW * 32;      // warps and threads that sum and write
+constexpr int CU = 4;                     // vectors a thread takes of a chunk
+constexpr int CV = CT * CU;               // vectors of a chunk: 32 KiB
+constexpr int SLOTS = 6;                  // chunks of the ring
+constexpr int ROWQ = 4;                   // rows handed out ahead of the warps
+constexpr int STEP_T = CT + 64;           // and a warp each for the producer and the lists
+
+struct StepRow {  // what the warps need to write a row
+  float m, coef;
+};
+struct StepS {
+  uint64_t full[SLOTS], empty[SLOTS];
+  uint64_t row_full[ROWQ], row_empty[ROWQ];
+  uint64_t list_full[2], list_empty[2];  // lists and marks of this row and the next
+  uint64_t summed, solved;
+  int row[ROWQ];
+  float part_m[CW], part_s[CW];
+  StepRow out;
+  float listg[2][MAXK];
+  int at[2][MAXK];                       // places of the listed elements, -1: empty
+  ListS list;
+  int dead;
+};
+__host__ __device__ inline int step_chunks(int V, int A) { return (V + A - 1 + A - 1 + CV * A - 1) / (CV * A); }
+
+template <typename T>
+__global__ void __launch_bounds__(STEP_T, 1) k_distill_step(const DistP P, int* next_row) {
+  using VT = Vec<T>;
+  constexpr int A = VT::A;
+  extern __shared__ __align__(128) unsigned char dyn[];
+  uint4* ring = reinterpret_cast<uint4*>(dyn);
+  StepS& S = *reinterpret_cast<StepS*>(dyn + (size_t)SLOTS * CV * 16);
+  uint32_t* marks = reinterpret_cast<uint32_t*>(&S + 1);  // [2][chunks * CV / 32]
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int words = step_chunks(P.V, A) * (CV / 32);
+  if (tid == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      bar_init(&S.full[i], 1);
+      bar_init(&S.empty[i], CW);
+    }
+    for (int i = 0; i < ROWQ; ++i) {
+      bar_init(&S.row_full[i], 1);
+      bar_init(&S.row_empty[i], CW + 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      bar_init(&S.list_full[i], 1);
+      bar_init(&S.list_empty[i], CW);
+    }
+    bar_init(&S.summed, CW);
+    bar_init(&S.solved, 1);
+    S.dead = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int i = tid; i < 2 * words; i += STEP_T) marks[i] = 0;
+  for (int i = tid; i < 2 * MAXK; i += STEP_T) (&S.at[0][0])[i] = -1;
+  __syncthreads();
+  volatile int* dead = &S.dead;
+
+  if (w == CW) {  // ---- the producer
+    if (lane == 0) {
+      uint32_t it = 0;  // chunks so far
+      int row = blockIdx.x;
+      for (uint32_t i = 0;; ++i) {
+        const int qi = i % ROWQ;
+        if (i >= ROWQ && !bar_wait(&S.row_empty[qi], (i / ROWQ - 1) & 1, dead)) break;
+        S.row[qi] = row < P.rows ? row : -1;
+        bar_arrive(&S.row_full[qi]);
+        if (row >= P.rows) break;
+        if (!P.weights || P.weights[row] != 0.f) {
+          const Row<T> R(static_cast<const T*>(P.logits) + (int64_t)row * P.ld, P.V);
+          const int C = (R.nv + CV - 1) / CV, again = C > SLOTS ? C - SLOTS : 0;
+          const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;  // whole vectors
+          bool ok = true;
+          for (int c = 0; c < C + again && ok; ++c, ++it) {
+            const int slot = it % SLOTS, chunk = c < C ? c : c - C;
+            if (it >= SLOTS) ok = bar_wait(&S.empty[slot], (it / SLOTS - 1) & 1, dead);
+            if (!ok) break;
+            const int a = max(chunk * CV, lo), b = min((chunk + 1) * CV, hi);
+            if (b > a) {
+              bar_expect(&S.full[slot], (uint32_t)(b - a) * 16);
+              bulk_load(ring + (size_t)slot * CV + (a - chunk * CV),
+                        R.p + ((int64_t)a * A - R.off), (uint32_t)(b - a) * 16, &S.full[slot]);
+            } else {
+              bar_arrive(&S.full[slot]);
+            }
+          }
+          if (!ok) break;
+        }
+        row = gridDim.x + atomicAdd(next_row, 1);
+      }
+      // no copy of this CTA may land behind its end
+      if (*dead)
+        for (uint32_t k = it > SLOTS ? it - SLOTS : 0; k < it; ++k) {
+          int none = 0;
+          bar_wait(&S.full[k % SLOTS], (k / SLOTS) & 1, &none);
+        }
+    }
+    return;
+  }
+
+  if (w == CW + 1) {  // ---- the list's warp
+    uint32_t live = 0;
+    for (uint32_t i = 0;; ++i) {
+      if (!bar_wait(&S.row_full[i % ROWQ], (i / ROWQ) & 1, dead)) break;
+      const int row = S.row[i % ROWQ];
+      __syncwarp();
+      if (lane == 0) bar_arrive(&S.row_empty[i % ROWQ]);
+      if (row < 0) break;
+      const float weight = P.weights ? P.weights[row] : 1.f;
+      if (weight == 0.f) {
+        if (lane == 0) P.loss[row] = 0.f;
+        continue;
+      }
+      const int b = live & 1;
+      list_begin<T>(P, row, S.list);
+      if (live >= 2 && !bar_wait(&S.list_empty[b], (live / 2 - 1) & 1, dead)) break;
+      const int off = (int)(((uintptr_t)(static_cast<const T*>(P.logits) + (int64_t)row * P.ld) & 15) /
+                            sizeof(T));
+      uint32_t* mk = marks + b * words;
+      for (int j = lane; j < P.k; j += 32)
+        if (S.at[b][j] >= 0) mk[S.at[b][j] / A / 32] = 0;
+      __syncwarp();
+      for (int j = lane; j < P.k; j += 32) {
+        const int id = S.list.id[j];
+        const int at = id >= 0 && id < P.V ? id + off : -1;
+        S.at[b][j] = at;
+        if (at >= 0) atomicOr(&mk[at / A / 32], 1u << (at / A & 31));
+      }
+      __syncwarp();
+      if (lane == 0) bar_arrive(&S.list_full[b]);
+      if (!bar_wait(&S.summed, live & 1, dead)) break;
+      // the warps' sums, joined in a fixed order
+      const float pm = lane < CW ? S.part_m[lane] : neg_inf(), ps = lane < CW ? S.part_s[lane] : 0.f;
+      const float m = warp_max(pm);
+      const double r =
+          warp_sum(ps == 0.f ? 0.0 : (double)ps * exp2(((double)pm - (double)m) * (double)P.scale));
+      const Solved sol = list_solve(P, S.list, m, r);
+      const Stat st = list_grads(P, S.list, sol, m, r, weight * P.inv_t, S.listg[b]);
+      if (lane == 0) S.out = StepRow{st.m, st.coef};
+      __syncwarp();
+      if (lane == 0) bar_arrive(&S.solved);
+      const float loss = list_loss(P, S.list, sol);
+      if (lane == 0) P.loss[row] = loss * weight;
+      __syncwarp();
+      ++live;
+    }
+    if (lane == 0 && *dead && P.status) atomicOr(P.status, (int)VINFER_ST_INTERNAL);
+    return;
+  }
+
+  // ---- the warps that sum and write
+  uint32_t it = 0, live = 0;  // chunks and rows so far
+  const uint64_t scale2 = pair(P.scale, P.scale);
+  for (uint32_t i = 0;; ++i) {
+    if (!bar_wait(&S.row_full[i % ROWQ], (i / ROWQ) & 1, dead)) break;
+    const int row = S.row[i % ROWQ];
+    __syncwarp();
+    if (lane == 0) bar_arrive(&S.row_empty[i % ROWQ]);
+    if (row < 0) break;
+    const Row<T> R(static_cast<const T*>(P.logits) + (int64_t)row * P.ld, P.V);
+    T* out = static_cast<T*>(P.grad) + (int64_t)row * P.ldg;
+    const bool aligned = (int)(((uintptr_t)out & 15) / sizeof(T)) == R.off;
+    const int C = (R.nv + CV - 1) / CV, again = C > SLOTS ? C - SLOTS : 0;
+    const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;
+
+    // the thread's vectors of a chunk: in the ring, at the row's ragged ends from memory
+    auto take = [&](int chunk, uint32_t n, uint4 (&q)[CU]) {
+      const uint4* src = ring + (size_t)(n % SLOTS) * CV + tid;
+#pragma unroll
+      for (int u = 0; u < CU; ++u) q[u] = src[u * CT];
+      const int v0 = chunk * CV;
+      if (v0 < lo || v0 + CV > hi) {
+#pragma unroll
+        for (int u = 0; u < CU; ++u) {
+          const int v = v0 + u * CT + tid;
+          const uint32_t ni = VT::NEG_INF_WORD;
+          if (v >= R.nv) q[u] = make_uint4(ni, ni, ni, ni);
+          else if (v < lo || v >= hi) q[u] = R.edge(R.p, R.V, v * A - R.off);
+        }
+      }
+    };
+    auto put = [&](int v, const float (&g)[A]) {
+      const int64_t e0 = (int64_t)v * A - R.off;
+      if (aligned && v >= lo && v < hi) {
+        *reinterpret_cast<uint4*>(out + e0) = VT::pack(g);
+      } else {
+#pragma unroll
+        for (int j = 0; j < A; ++j)
+          if (e0 + j >= 0 && e0 + j < P.V) out[e0 + j] = VT::round(g[j]);
+      }
+    };
+
+    if (P.weights && P.weights[row] == 0.f) {
+      float g[A];
+#pragma unroll
+      for (int j = 0; j < A; ++j) g[j] = 0.f;
+      for (int v = tid; v < R.nv; v += CT) put(v, g);
+      continue;
+    }
+    const int b = live & 1;
+    const uint32_t* mk = marks + b * words;
+    if (!bar_wait(&S.list_full[b], (live / 2) & 1, dead)) break;
+    float m = neg_inf(), s = 0.f;
+    bool ok = true;
+    for (int c = 0; c < C; ++c, ++it) {
+      if (!(ok = bar_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead))) break;
+      uint4 q[CU];
+      take(c, it, q);
+      if (c < C - SLOTS) {  // not held for the gradient
+        __syncwarp();
+        if (lane == 0) bar_arrive(&S.empty[it % SLOTS]);
+      }
+#pragma unroll
+      for (int u = 0; u < CU; ++u) {
+        const int first = c * CV + u * CT + w * 32;
+        if (const uint32_t word = mk[first / 32]) take_out<T>(q[u], word, S.at[b], P.k, first);
+      }
+      add_exps<T>(q, VT::max(q), P.scale, m, s);
+    }
+    if (!ok) break;
+    if (s == 0.f) m = neg_inf();
+    const float mw = warp_max(m);
+    float sw = s == 0.f ? 0.f : s * ex2((m - mw) * P.scale);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sw += __shfl_xor_sync(FULL, sw, o);
+    if (lane == 0) {
+      S.part_m[w] = mw;
+      S.part_s[w] = sw;
+      bar_arrive(&S.summed);
+    }
+    __syncwarp();
+    if (!bar_wait(&S.solved, live & 1, dead)) break;
+    const StepRow o = S.out;
+    const uint64_t neg_m = pair(-o.m, -o.m), coef = pair(o.coef, o.coef);
+    // chunks the ring still holds, in order, then the others once more
+    const int held = C - again;
+    for (int k = 0; k < C; ++k) {
+      const int c = k < held ? again + k : k - held;
+      const uint32_t n = k < held ? it - held + k : it + (k - held);
+      if (k >= held && !(ok = bar_wait(&S.full[n % SLOTS], (n / SLOTS) & 1, dead))) break;
+      uint4 q[CU];
+      take(c, n, q);
+      __syncwarp();
+      if (lane == 0) bar_arrive(&S.empty[n % SLOTS]);
+#pragma unroll
+      for (int u = 0; u < CU; ++u) {
+        const int first = c * CV + u * CT + w * 32, v = first + lane;
+        uint64_t h[A / 2];
+        float g[A];
+        VT::pairs(q[u], h);
+#pragma unroll
+        for (int j = 0; j < A / 2; ++j)
+          split(mul2(ex2_2(mul2(add2(h[j], neg_m), scale2)), coef), g[2 * j], g[2 * j + 1]);
+        for (uint32_t word = mk[first / 32]; word; word &= word - 1) {  // listed elements
+          const int l = __ffs(word) - 1;
+          for (int j0 = 0; j0 < P.k; j0 += 32) {
+            const int at = j0 + lane < P.k ? S.at[b][j0 + lane] : -1;
+            unsigned who = __ballot_sync(FULL, at >= 0 && at / A == first + l);
+            for (; who; who &= who - 1) {
+              const int j = j0 + __ffs(who) - 1;
+              const int e = S.at[b][j] & (A - 1);
+              if (lane == l) {
+#pragma unroll
+                for (int a = 0; a < A; ++a)
+                  if (a == e) g[a] = S.listg[b][j];
+              }
+            }
+          }
+        }
+        if (v < R.nv) put(v, g);
+      }
+    }
+    if (!ok) break;
+    it += again;
+    __syncwarp();
+    if (lane == 0) bar_arrive(&S.list_empty[b]);
+    ++live;
+  }
+}
+
 // Parts of a row: enough CTAs to fill the 148 SMs several times over, at least two vectors a
 // thread in each.
 int distill_parts(int64_t rows_, int64_t vocab, int dtype) {
@@ -353,6 +673,12 @@ int distill_parts(int64_t rows_, int64_t vocab, int dtype) {
   int64_t p = (148 * 8 + rows_ - 1) / rows_;
   p = std::min<int64_t>(p, (nv + 2 * NT - 1) / (2 * NT));
   return (int)std::max<int64_t>(1, std::min<int64_t>(p, MAX_PARTS));
+}
+
+// Rows taken whole by one CTA each, where there are enough and they are long.
+bool step_in_one(const DistP& P, int dtype) {
+  const int64_t bytes = (int64_t)P.V * (dtype == VINFER_DTYPE_BF16 ? 2 : 4);
+  return P.rows >= 2 * 148 && bytes >= (64 << 10);
 }
 
 int check(const VinferDistillArgs* a) {
@@ -397,6 +723,19 @@ int launch_loss(const DistP& P, cudaStream_t st) {
 template <typename T>
 int launch_grad(const DistP& P, cudaStream_t st, bool dependent) {
   return launch(k_distill_grad<T>, (unsigned)(P.rows * P.parts), NT, 0, st, dependent, P);
+}
+
+size_t step_smem(int V, int A) {
+  return (size_t)SLOTS * CV * 16 + sizeof(StepS) + 2 * (size_t)step_chunks(V, A) * (CV / 8);
+}
+
+template <typename T>
+int launch_step(const DistP& P, int* next_row, cudaStream_t st) {
+  const size_t smem = step_smem(P.V, Vec<T>::A);
+  if (opt_in(k_distill_step<T>, smem) != VINFER_OK) return VINFER_E_CUDA;
+  if (result(cudaMemsetAsync(next_row, 0, sizeof(int), st)) != VINFER_OK) return VINFER_E_CUDA;
+  return launch(k_distill_step<T>, (unsigned)std::min<int64_t>(P.rows, 148), STEP_T, smem, st, false,
+                P, next_row);
 }
 
 size_t align_up(size_t n) { return (n + 255) / 256 * 256; }
@@ -476,6 +815,9 @@ int vinfer_distill_step(const VinferDistillArgs* a, float* loss, void* grad, int
   P.grad = grad;
   P.ldg = ld_grad;
   cudaStream_t st = (cudaStream_t)stream;
+  if (step_in_one(P, a->dtype))
+    return a->dtype == VINFER_DTYPE_BF16 ? launch_step<__nv_bfloat16>(P, (int*)workspace, st)
+                                         : launch_step<float>(P, (int*)workspace, st);
   if (a->dtype == VINFER_DTYPE_BF16) {
     rc = launch_loss<__nv_bfloat16>(P, st);
     return rc != VINFER_OK ? rc : launch_grad<__nv_bfloat16>(P, st, true);
