@@ -127,14 +127,15 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
 
 // A row's list as one warp works on it, four entries a lane.
 struct ListS {
-  double z[MAXK];     // listed logits; behind the join distances from the row's largest, in log2
+  double e[MAXK];     // 2^((z - top) * scale): all that takes exponentials is ready before the sum is
   double p[MAXK];     // masses as listed
   double psum[MAXK];  // ... summed over the entries of the same id
+  float z[MAXK];      // listed logits
   float l[MAXK];      // log-probabilities
   int id[MAXK];       // -1: empty
-  bool lead[MAXK];    // the first entry of its id
   double mass;        // sum of p
-  double top;         // largest z
+  double esum;        // sum of e, each id once
+  float top;          // largest z
   int distinct;       // ids
   bool bad;           // an id or a log-probability out of range
 };
@@ -145,12 +146,15 @@ __device__ __forceinline__ void list_begin(const DistP& P, int64_t row, ListS& L
   const int lane = threadIdx.x & 31;
   const T* x = static_cast<const T*>(P.logits) + row * P.ld;
   int id[4];
+  float z[4];
   bool bad = false;
-  double mass = 0, top = (double)neg_inf();
+  double mass = 0;
+  float top = neg_inf();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int j = lane + 32 * i;
     id[i] = -1;
+    z[i] = neg_inf();
     if (j < P.k) {
       id[i] = P.ids[row * P.k + j];
       float l = P.lp[row * P.k + j];
@@ -160,15 +164,20 @@ __device__ __forceinline__ void list_begin(const DistP& P, int64_t row, ListS& L
       }
       const bool off = id[i] >= P.V || !(l < -neg_inf());
       bad = bad || off;
-      const double z = id[i] >= 0 && !off ? (double)Vec<T>::load(x + id[i]) : (double)neg_inf();
+      if (id[i] >= 0 && !off) z[i] = Vec<T>::load(x + id[i]);
       const double p = id[i] >= 0 ? exp((double)l) : 0.0;
       L.id[j] = id[i];
       L.l[j] = l;
-      L.z[j] = z;
+      L.z[j] = z[i];
       L.p[j] = p;
       mass += p;
-      if (z > top || z != z) top = z;
+      if (z[i] > top || z[i] != z[i]) top = z[i];
     }
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float t = __shfl_xor_sync(FULL, top, o);
+    if (t > top || t != t) top = t;
   }
   __syncwarp();
   double psum[4] = {0, 0, 0, 0};
@@ -184,25 +193,28 @@ __device__ __forceinline__ void list_begin(const DistP& P, int64_t row, ListS& L
       }
   }
   int distinct = 0;
+  double esum = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int j = lane + 32 * i;
     if (j < P.k) {
+      const double e =
+          z[i] == neg_inf() ? 0.0 : exp2(((double)z[i] - (double)top) * P.scale_d);
+      L.e[j] = e;
       L.psum[j] = psum[i];
-      L.lead[j] = lead[i];
-      distinct += lead[i];
+      if (lead[i]) {
+        esum += e;
+        ++distinct;
+      }
     }
   }
   mass = warp_sum(mass);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const double t = __shfl_xor_sync(FULL, top, o);
-    if (t > top || t != t) top = t;
-  }
+  esum = warp_sum(esum);
   distinct = (int)__reduce_add_sync(FULL, (unsigned)distinct);
   bad = __any_sync(FULL, bad);
   if (lane == 0) {
     L.mass = mass;
+    L.esum = esum;
     L.top = top;
     L.distinct = distinct;
     L.bad = bad;
@@ -210,72 +222,77 @@ __device__ __forceinline__ void list_begin(const DistP& P, int64_t row, ListS& L
   __syncwarp();
 }
 
-// The row solved: all in distances from its largest logit, whatever its magnitude, and in log2.
+// The row solved, in distances from its largest logit `ref`, whatever its magnitude.
 struct Solved {
-  double lse;    // log-sum
-  double rest;   // ... of what is outside the list
-  double mass;   // the target's mass M
-  double pt;     // its tail
-  double norm, lnorm;  // a listed mass is p * norm, its logarithm l - lnorm
+  double ref;
+  double total;        // sum of 2^((x - ref) * scale) over the row
+  double listed;       // 2^((top - ref) * scale) / total: q of a listed element is e * listed
+  double rest;         // share of what is outside the list
+  double mass;         // the target's mass M
+  double pt;           // its tail
+  double norm;         // a listed mass is p * norm
   bool bad;
 };
 
-// From the list and the sum outside it, (m, r) with r in units of 2^(m * scale). Leaves ln q in L.z
-// (as log2 q).
-__device__ __forceinline__ Solved list_solve(const DistP& P, ListS& L, float m, double r) {
-  const int lane = threadIdx.x & 31;
-  const double inf = (double)-neg_inf();
-  Solved S = {0, 0, 0, 0, 1, 0, L.bad};
-  if (L.bad) {
-    if (lane == 0 && P.status) atomicOr(P.status, (int)VINFER_ST_BAD_LIST);
-    return S;
-  }
-  double ref = L.top;
-  if (r != 0 && !(ref != ref) && (double)m > ref) ref = m;
-  double total = 0;
-  for (int j = lane; j < P.k; j += 32) {
-    L.z[j] = (L.z[j] - ref) * P.scale_d;
-    if (L.lead[j]) total += exp2(L.z[j]);
-  }
-  S.rest = r == 0 ? -inf : ((double)m - ref) * P.scale_d + log2(r);
-  total = warp_sum(total) + (r == 0 ? 0.0 : exp2(S.rest));
-  S.lse = log2(total);
-  for (int j = lane; j < P.k; j += 32) L.z[j] -= S.lse;
-  if (lane == 0 && P.status && !(fabs(S.lse) < inf))
-    atomicOr(P.status, (int)VINFER_ST_NONFINITE);
+// From the list and the sum outside it, (m, r) with r in units of 2^(m * scale). This is what the
+// gradient waits for: two exponentials and a division.
+__device__ __forceinline__ Solved list_solve(const DistP& P, const ListS& L, float m, double r) {
+  const float top = L.top;
+  Solved S;
+  S.bad = L.bad;
+  S.ref = r != 0 && m > top ? m : top;  // a NaN top stays
+  const double ft = exp2(((double)top - S.ref) * P.scale_d);
+  const double fr = r == 0 ? 0.0 : r * exp2(((double)m - S.ref) * P.scale_d);
+  S.total = (L.esum == 0 ? 0.0 : L.esum * ft) + fr;
+  if (S.ref != S.ref || S.ref == (double)neg_inf()) S.total = (double)__int_as_float(0x7fffffff);
+  const double inv = 1.0 / S.total;
+  S.listed = L.esum == 0 ? 0.0 : ft * inv;
+  S.rest = fr * inv;
   S.mass = L.mass;
+  S.pt = 0;
+  S.norm = 1;
   if (P.tail) {
     S.pt = L.distinct < P.V ? fmax(0.0, 1.0 - S.mass) : 0.0;
   } else if (S.mass > 0) {
     S.norm = 1.0 / S.mass;
-    S.lnorm = log(S.mass);
     S.mass = 1.0;
   }
   S.mass += S.pt;
   return S;
+}
+__device__ __forceinline__ bool lost(const Solved& S) {
+  return S.bad || !(S.total < (double)-neg_inf());
 }
 
 // The gradient's terms, times f: of the listed elements, and of those outside.
 __device__ __forceinline__ Stat list_grads(const DistP& P, const ListS& L, const Solved& S, float m,
                                            double r, float f, float* listg) {
   const float nan = __int_as_float(0x7fffffff);
-  const bool lost = S.bad || S.lse != S.lse;
   for (int j = threadIdx.x & 31; j < P.k; j += 32)
-    listg[j] = lost          ? nan
+    listg[j] = lost(S)       ? nan
                : L.id[j] < 0 ? 0.f
-                             : f * (float)(S.mass * exp2(L.z[j]) - L.psum[j] * S.norm);
-  if (lost) return Stat{nan, nan};
+                             : f * (float)(S.mass * (L.e[j] * S.listed) - L.psum[j] * S.norm);
+  if (lost(S)) return Stat{nan, nan};
   if (r == 0) return Stat{0.f, 0.f};
-  return Stat{m, f * (float)((S.mass * exp2(S.rest - S.lse) - S.pt) / r)};
+  return Stat{m, f * (float)((S.mass * S.rest - S.pt) / r)};
 }
 
 __device__ __forceinline__ float list_loss(const DistP& P, const ListS& L, const Solved& S) {
-  if (S.bad || S.lse != S.lse) return __int_as_float(0x7fffffff);
+  const int lane = threadIdx.x & 31;
+  if (lost(S)) {
+    if (lane == 0 && P.status)
+      atomicOr(P.status, (int)(S.bad ? VINFER_ST_BAD_LIST : VINFER_ST_NONFINITE));
+    return __int_as_float(0x7fffffff);
+  }
+  const double lse = log(S.total), lnorm = S.norm == 1 ? 0.0 : -log(S.norm);
+  const double unit = P.scale_d * LN2_D;
   double loss = 0;
-  for (int j = threadIdx.x & 31; j < P.k; j += 32)
-    if (L.p[j] > 0) loss += L.p[j] * S.norm * (((double)L.l[j] - S.lnorm) - L.z[j] * LN2_D);
+  for (int j = lane; j < P.k; j += 32)
+    if (L.p[j] > 0)
+      loss += L.p[j] * S.norm *
+              (((double)L.l[j] - lnorm) - (((double)L.z[j] - S.ref) * unit - lse));
   loss = warp_sum(loss);
-  if (S.pt > 0) loss += S.pt * (log(S.pt) - (S.rest - S.lse) * LN2_D);
+  if (S.pt > 0) loss += S.pt * (log(S.pt) - log(S.rest));
   return (float)loss;
 }
 
@@ -389,6 +406,7 @@ constexpr int CW = 16, CT = CW * 32;      // warps and threads that sum and writ
 constexpr int CU = 4;                     // vectors a thread takes of a chunk
 constexpr int CV = CT * CU;               // vectors of a chunk: 32 KiB
 constexpr int SLOTS = 6;                  // chunks of the ring
+constexpr int STEP_CTAS = 1;              // CTAs of an SM
 constexpr int ROWQ = 4;                   // rows handed out ahead of the warps
 constexpr int STEP_T = CT + 64;           // and a warp each for the producer and the lists
 
@@ -411,7 +429,7 @@ struct StepS {
 __host__ __device__ inline int step_chunks(int V, int A) { return (V + A - 1 + A - 1 + CV * A - 1) / (CV * A); }
 
 template <typename T>
-__global__ void __launch_bounds__(STEP_T, 1) k_distill_step(const DistP P, int* next_row) {
+__global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const DistP P, int* next_row) {
   using VT = Vec<T>;
   constexpr int A = VT::A;
   extern __shared__ __align__(128) unsigned char dyn[];
@@ -520,7 +538,7 @@ __global__ void __launch_bounds__(STEP_T, 1) k_distill_step(const DistP P, int* 
       const float pm = lane < CW ? S.part_m[lane] : neg_inf(), ps = lane < CW ? S.part_s[lane] : 0.f;
       const float m = warp_max(pm);
       const double r =
-          warp_sum(ps == 0.f ? 0.0 : (double)ps * exp2(((double)pm - (double)m) * (double)P.scale));
+          warp_sum(ps == 0.f ? 0.0 : (double)ps * (double)exp2f((pm - m) * P.scale));
       const Solved sol = list_solve(P, S.list, m, r);
       const Stat st = list_grads(P, S.list, sol, m, r, weight * P.inv_t, S.listg[b]);
       if (lane == 0) S.out = StepRow{st.m, st.coef};
@@ -678,7 +696,7 @@ int distill_parts(int64_t rows_, int64_t vocab, int dtype) {
 // Rows taken whole by one CTA each, where there are enough and they are long.
 bool step_in_one(const DistP& P, int dtype) {
   const int64_t bytes = (int64_t)P.V * (dtype == VINFER_DTYPE_BF16 ? 2 : 4);
-  return P.rows >= 2 * 148 && bytes >= (64 << 10);
+  return P.rows >= 2 * 148 * STEP_CTAS && bytes >= (64 << 10);
 }
 
 int check(const VinferDistillArgs* a) {
@@ -734,7 +752,7 @@ int launch_step(const DistP& P, int* next_row, cudaStream_t st) {
   const size_t smem = step_smem(P.V, Vec<T>::A);
   if (opt_in(k_distill_step<T>, smem) != VINFER_OK) return VINFER_E_CUDA;
   if (result(cudaMemsetAsync(next_row, 0, sizeof(int), st)) != VINFER_OK) return VINFER_E_CUDA;
-  return launch(k_distill_step<T>, (unsigned)std::min<int64_t>(P.rows, 148), STEP_T, smem, st, false,
+  return launch(k_distill_step<T>, (unsigned)std::min<int64_t>(P.rows, 148 * STEP_CTAS), STEP_T, smem, st, false,
                 P, next_row);
 }
 
