@@ -117,7 +117,8 @@ def test_matches_the_formulas(backend, N, V, k, T, pad, tail, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=["f32", "bf16"])
 @pytest.mark.parametrize("N,V,k,pad", [(301, 32776, 9, 0), (310, 33001, 128, 0), (297, 50003, 33, 5),
-                                       (299, 120007, 20, 1), (610, 65536, 4, 0)])
+                                       (299, 120007, 20, 1), (610, 65536, 4, 0), (100, 262144, 6, 0),
+                                       (97, 248319, 128, 0)])
 def test_many_long_rows(backend, N, V, k, pad, dtype):
     """Rows taken whole by one CTA: more than the CTAs, ragged, masked, with bad lists among them."""
     x, ids, lp, w = make(N, V, k, dtype, 1.5)

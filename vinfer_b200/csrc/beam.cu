@@ -621,9 +621,9 @@ int launch_beam(const PickP& Q, int64_t requests, cudaStream_t st) {
   const size_t sm_pick = pick_smem(Q.W, Q.r.n, Q.r.parts);
   if (opt_in(k_beam_rows<T>, sm_rows) != VINFER_OK || opt_in(k_beam_pick<T>, sm_pick) != VINFER_OK)
     return VINFER_E_CUDA;
-  const int rc = launch(k_beam_rows<T>, (unsigned)(rows_ * Q.r.parts), NT, sm_rows, st, false, Q.r);
+  const int rc = launch(k_beam_rows<T>, (unsigned)(rows_ * Q.r.parts), NT, sm_rows, st, false, 1, Q.r);
   if (rc != VINFER_OK) return rc;
-  return launch(k_beam_pick<T>, (unsigned)requests, PT, sm_pick, st, true, Q);
+  return launch(k_beam_pick<T>, (unsigned)requests, PT, sm_pick, st, true, 1, Q);
 }
 
 }  // namespace

@@ -18,6 +18,7 @@
 #include "rows.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace {
 
@@ -67,10 +68,10 @@ __device__ __forceinline__ uint32_t listed_in(const int* at, int n, int v) {
   return __reduce_or_sync(FULL, bits);
 }
 
-// Takes the listed elements out of the warp's vectors: lane l holds vector v0 + l, `word` has the
-// bit of each that holds one.
+// The warp's vectors with their listed elements taken out: lane l holds vector v0 + l as q, `word` has
+// the bit of each that holds one. Rarely called, and kept out of the streaming loops' code.
 template <typename T>
-__device__ __forceinline__ void take_out(uint4& q, uint32_t word, const int* at, int n, int v0) {
+__device__ __noinline__ uint4 take_out(uint4 q, uint32_t word, const int* at, int n, int v0) {
   for (; word; word &= word - 1) {
     const int l = __ffs(word) - 1;
     const uint32_t bits = listed_in<Vec<T>::A>(at, n, v0 + l);
@@ -80,6 +81,33 @@ __device__ __forceinline__ void take_out(uint4& q, uint32_t word, const int* at,
         if (bits >> j & 1) Vec<T>::put(q, j, Vec<T>::NEG_INF_BITS);
     }
   }
+  return q;
+}
+
+// Stores the gradients of the listed elements of the warp's vectors, each by the lane that has just
+// stored its vector. `first`: where the element counted as place 0 goes.
+template <typename T>
+__device__ __noinline__ void store_listed(T* first, uint32_t word, const int* at,
+                                          const float* listg, int n, int v0) {
+  constexpr int A = Vec<T>::A;
+  for (; word; word &= word - 1) {
+    const int l = __ffs(word) - 1;
+    for (int j0 = 0; j0 < n; j0 += 32) {
+      const int mine = j0 + (threadIdx.x & 31) < n ? at[j0 + (threadIdx.x & 31)] : -1;
+      unsigned who = __ballot_sync(FULL, mine >= 0 && mine / A == v0 + l);
+      for (; who; who &= who - 1) {
+        const int j = j0 + __ffs(who) - 1;
+        if ((threadIdx.x & 31) == l) first[at[j]] = Vec<T>::round(listg[j]);
+      }
+    }
+  }
+}
+
+// Stores the elements of one vector that lie in [0, V): the vector's first is element e0.
+template <typename T>
+__device__ __noinline__ void store_ragged(T* out, uint4 q, int e0, int V) {
+  for (int j = 0; j < Vec<T>::A; ++j)
+    if (e0 + j >= 0 && e0 + j < V) out[e0 + j] = Vec<T>::round(Vec<T>::get(q, j));
 }
 
 // Dynamic shared memory: one bit for each vector of the part's rounds, set where it holds a listed
@@ -117,7 +145,8 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {  // a warp's 32 vectors are one word (and zeros behind the part)
       const int first = vb - v0 + u * NT + (tid & ~31);
-      if (const uint32_t word = marked[first / 32]) take_out<T>(q[u], word, hit, hits, first);
+      if (const uint32_t word = marked[first / 32])
+        q[u] = take_out<T>(q[u], word, hit, hits, first);
     }
     add_exps<T>(q, VT::max(q), P.scale, m, s);
   }
@@ -374,13 +403,8 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
           for (int j = 0; j < A; ++j) g[j] = 0.f;
         }
         const int64_t e0 = (int64_t)v * A - R.off;
-        if (aligned && R.whole(v)) {
-          *reinterpret_cast<uint4*>(out + e0) = VT::pack(g);
-        } else {
-#pragma unroll
-          for (int j = 0; j < A; ++j)
-            if (e0 + j >= 0 && e0 + j < P.V) out[e0 + j] = VT::round(g[j]);
-        }
+        if (aligned && R.whole(v)) *reinterpret_cast<uint4*>(out + e0) = VT::pack(g);
+        else store_ragged(out, VT::pack(g), (int)e0, P.V);
       }
     }
   }
@@ -395,49 +419,109 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
 }
 
 // ---- loss and gradient in one pass ------------------------------------------------------------
-// One persistent CTA an SM takes whole rows. A producer thread streams a row's chunks into a ring of
-// shared memory by bulk copies; CW warps sum them, releasing each chunk until the ring can hold the
-// rest of the row; the list's warp solves the row; the CW warps then write the gradient of the
-// chunks the ring still holds, and of the others, which the producer brings once more (from L2:
-// every SM re-reads what it read some microseconds before). HBM sees each row read once and written
-// once. While a row is solved and written, the producer fills the ring with the next row, and
-// the list's warp prepares the next list.
-constexpr int CW = 16, CT = CW * 32;      // warps and threads that sum and write
+// A cluster of CTAs takes a row at a time, each CTA a slice of it. In each CTA a producer thread
+// streams the slice into a ring of chunks by bulk copies; CW warps sum the chunks, releasing
+// each until the ring can hold the rest of the slice, and write the gradient once the row is
+// solved: first of the chunks the ring still holds, then of the others, which the producer brings
+// once more, from L2 (the slices are cut so that few are, and nothing else is kept there). HBM sees
+// every row read once and written once. Two warps solve rows in turn: each prepares its row's list
+// ahead, joins the CTA's sum with the other CTAs' (each sends its own to all), and hands out the
+// gradient's terms. Two CTAs an SM, so that one streams while the other solves.
+constexpr int STEP_CTAS = 2;              // CTAs of an SM
+constexpr int CW = 11, CT = CW * 32;      // warps and threads that sum and write
 constexpr int CU = 4;                     // vectors a thread takes of a chunk
-constexpr int CV = CT * CU;               // vectors of a chunk: 32 KiB
-constexpr int SLOTS = 6;                  // chunks of the ring
-constexpr int STEP_CTAS = 1;              // CTAs of an SM
-constexpr int ROWQ = 4;                   // rows handed out ahead of the warps
-constexpr int STEP_T = CT + 64;           // and a warp each for the producer and the lists
+constexpr int CV = CT * CU;               // vectors of a chunk: 22 KiB
+constexpr int SLOTS = 4;                  // chunks of the ring
+constexpr int SLICE = 14;                 // chunks of a slice at most
+constexpr int MINC = 1, MAXC = 16;        // CTAs of a cluster
+constexpr int LW = 2;                     // warps that solve, and rows under way
+constexpr int STEP_T = CT + 32 + LW * 32;
 
-struct StepRow {  // what the warps need to write a row
+static_assert(CU == 4, "a warp's marks of a chunk are one 16-byte word");
+// word and bit of vector v of a slice
+__device__ __forceinline__ uint32_t* mark(uint4* marks, int v) {
+  const int c = v / CV, u = v % CV / CT, w = v % CT / 32;
+  return reinterpret_cast<uint32_t*>(marks + c * CW + w) + u;
+}
+
+// What belongs to one row under way. Buffer j serves the live rows i with i % LW == j. It is safe
+// to refill: a CTA sends its sum of row i + 2 after its gradient of row i + 1, which needs every
+// CTA's sum of row i + 1, taken there after row i was solved and written.
+static_assert(LW == 2, "a buffer's last reader is done two rows later");
+struct StepRow {
+  uint64_t list_full, list_empty;  // marks and places are set; ... and no longer needed
+  uint64_t summed;                 // the CTA's warps have left their sums
+  uint64_t joined;                 // every CTA's sum has arrived
+  uint64_t solved;                 // m, coef and listg are set
+  uint64_t part[MAXC];             // the CTAs' sums (m, s)
+  float part_m[CW], part_s[CW];    // this CTA's warps'
   float m, coef;
+  float listg[MAXK];
+  int at[MAXK];                    // places of the listed elements in the slice, -1: not in it
+  uint4 marks[SLICE * CW];         // a bit for each vector that holds one: a warp's CU of a chunk
+  ListS list;
 };
+constexpr int ROWQ = 4;            // rows handed out ahead, the next two of them before they are loaded
 struct StepS {
   uint64_t full[SLOTS], empty[SLOTS];
   uint64_t row_full[ROWQ], row_empty[ROWQ];
-  uint64_t list_full[2], list_empty[2];  // lists and marks of this row and the next
-  uint64_t summed, solved;
-  int row[ROWQ];
-  float part_m[CW], part_s[CW];
-  StepRow out;
-  float listg[2][MAXK];
-  int at[2][MAXK];                       // places of the listed elements, -1: empty
-  ListS list;
+  int64_t next_row[ROWQ];          // -1: no more
+  float next_weight[ROWQ];
+  StepRow row[LW];
   int dead;
 };
-__host__ __device__ inline int step_chunks(int V, int A) { return (V + A - 1 + A - 1 + CV * A - 1) / (CV * A); }
+
+// The rows of a cluster, as every CTA's producer walks them: the live rows (weight not 0) are dealt
+// out in turn, and so are the others, so that every cluster gets as many of each.
+struct RowWalk {
+  const float* weights;
+  int64_t rows, base;    // the 32 rows under the lanes
+  float w, ahead;        // this lane's weight, and that of the next 32
+  unsigned mine;         // rows of the 32 that are the cluster's and still to come
+  uint32_t live, dead;   // live and other rows before base, modulo the clusters
+  int me, all;
+  __device__ __forceinline__ RowWalk(const DistP& P, int cluster, int clusters)
+      : weights(P.weights), rows(P.rows), base(-32), w(0), ahead(0), mine(0), live(0), dead(0),
+        me(cluster), all(clusters) {
+    ahead = at(0);
+  }
+  __device__ __forceinline__ float at(int64_t b) const {
+    const int64_t r = b + (threadIdx.x & 31);
+    return r < rows ? (weights ? weights[r] : 1.f) : 0.f;
+  }
+  // The next row and its weight; false behind the last. The whole warp calls it.
+  __device__ __forceinline__ bool next(int64_t& row, float& weight) {
+    while (!mine) {
+      base += 32;
+      if (base >= rows) return false;
+      w = ahead;
+      ahead = at(base + 32);
+      const int lane = threadIdx.x & 31;
+      const bool there = base + lane < rows, l = there && w != 0.f, d = there && w == 0.f;
+      const unsigned lm = __ballot_sync(FULL, l), dm = __ballot_sync(FULL, d);
+      const unsigned below = (1u << lane) - 1;
+      const uint32_t turn = l ? live + __popc(lm & below) : dead + __popc(dm & below);
+      mine = __ballot_sync(FULL, there && (int)(turn % all) == me);
+      live = (live + __popc(lm)) % all;
+      dead = (dead + __popc(dm)) % all;
+    }
+    const int l = __ffs(mine) - 1;
+    mine &= mine - 1;
+    row = base + l;
+    weight = __shfl_sync(FULL, w, l);
+    return true;
+  }
+};
 
 template <typename T>
-__global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const DistP P, int* next_row) {
+__global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid_constant__ DistP P) {
   using VT = Vec<T>;
   constexpr int A = VT::A;
   extern __shared__ __align__(128) unsigned char dyn[];
   uint4* ring = reinterpret_cast<uint4*>(dyn);
   StepS& S = *reinterpret_cast<StepS*>(dyn + (size_t)SLOTS * CV * 16);
-  uint32_t* marks = reinterpret_cast<uint32_t*>(&S + 1);  // [2][chunks * CV / 32]
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int words = step_chunks(P.V, A) * (CV / 32);
+  const int size = (int)cluster_size(), rank = (int)cluster_rank();
   if (tid == 0) {
     for (int i = 0; i < SLOTS; ++i) {
       bar_init(&S.full[i], 1);
@@ -445,242 +529,275 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const DistP 
     }
     for (int i = 0; i < ROWQ; ++i) {
       bar_init(&S.row_full[i], 1);
-      bar_init(&S.row_empty[i], CW + 1);
+      bar_init(&S.row_empty[i], CW + LW);
     }
-    for (int i = 0; i < 2; ++i) {
-      bar_init(&S.list_full[i], 1);
-      bar_init(&S.list_empty[i], CW);
+    for (int i = 0; i < LW; ++i) {
+      bar_init(&S.row[i].list_full, 1);
+      bar_init(&S.row[i].list_empty, CW);
+      bar_init(&S.row[i].summed, CW);
+      bar_init(&S.row[i].joined, 1);
+      bar_init(&S.row[i].solved, 1);
     }
-    bar_init(&S.summed, CW);
-    bar_init(&S.solved, 1);
     S.dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int i = tid; i < 2 * words; i += STEP_T) marks[i] = 0;
-  for (int i = tid; i < 2 * MAXK; i += STEP_T) (&S.at[0][0])[i] = -1;
+  for (int j = w; j < LW; j += STEP_T / 32) {
+    for (int i = lane; i < MAXK; i += 32) S.row[j].at[i] = -1;
+    for (int i = lane; i < SLICE * CW; i += 32) S.row[j].marks[i] = make_uint4(0, 0, 0, 0);
+  }
   __syncthreads();
+  if (size > 1) cluster_sync();  // every CTA's barriers are ready for the others' sums
   volatile int* dead = &S.dead;
+  const uint64_t once = evict_first();
+  // a warp's next row and its weight; false behind the last
+  uint32_t taken = 0;
+  auto next_row = [&](int64_t& row, float& weight) {
+    const int i = taken % ROWQ;
+    if (!bar_wait(&S.row_full[i], (taken / ROWQ) & 1, dead)) return false;
+    row = S.next_row[i];
+    weight = S.next_weight[i];
+    __syncwarp();
+    if (lane == 0) bar_arrive(&S.row_empty[i]);
+    ++taken;
+    return row >= 0;
+  };
+  int64_t row;
+  float weight;
 
   if (w == CW) {  // ---- the producer
-    if (lane == 0) {
-      uint32_t it = 0;  // chunks so far
-      int row = blockIdx.x;
-      for (uint32_t i = 0;; ++i) {
-        const int qi = i % ROWQ;
-        if (i >= ROWQ && !bar_wait(&S.row_empty[qi], (i / ROWQ - 1) & 1, dead)) break;
-        S.row[qi] = row < P.rows ? row : -1;
-        bar_arrive(&S.row_full[qi]);
-        if (row >= P.rows) break;
-        if (!P.weights || P.weights[row] != 0.f) {
-          const Row<T> R(static_cast<const T*>(P.logits) + (int64_t)row * P.ld, P.V);
-          const int C = (R.nv + CV - 1) / CV, again = C > SLOTS ? C - SLOTS : 0;
-          const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;  // whole vectors
-          bool ok = true;
-          for (int c = 0; c < C + again && ok; ++c, ++it) {
-            const int slot = it % SLOTS, chunk = c < C ? c : c - C;
-            if (it >= SLOTS) ok = bar_wait(&S.empty[slot], (it / SLOTS - 1) & 1, dead);
-            if (!ok) break;
-            const int a = max(chunk * CV, lo), b = min((chunk + 1) * CV, hi);
-            if (b > a) {
-              bar_expect(&S.full[slot], (uint32_t)(b - a) * 16);
-              bulk_load(ring + (size_t)slot * CV + (a - chunk * CV),
-                        R.p + ((int64_t)a * A - R.off), (uint32_t)(b - a) * 16, &S.full[slot]);
-            } else {
-              bar_arrive(&S.full[slot]);
-            }
-          }
-          if (!ok) break;
-        }
-        row = gridDim.x + atomicAdd(next_row, 1);
+    RowWalk walk(P, blockIdx.x / size, gridDim.x / size);
+    uint32_t it = 0, handed = 0;  // chunks and rows so far
+    int ok = 1;
+    auto hand = [&](int64_t& r, float& wt) {
+      if (!walk.next(r, wt)) r = -1;
+      if (lane == 0) {
+        const int i = handed % ROWQ;
+        if (handed >= ROWQ) ok = bar_wait(&S.row_empty[i], (handed / ROWQ - 1) & 1, dead);
+        S.next_row[i] = r;
+        S.next_weight[i] = wt;
+        bar_arrive(&S.row_full[i]);
       }
-      // no copy of this CTA may land behind its end
-      if (*dead)
-        for (uint32_t k = it > SLOTS ? it - SLOTS : 0; k < it; ++k) {
-          int none = 0;
-          bar_wait(&S.full[k % SLOTS], (k / SLOTS) & 1, &none);
+      ++handed;
+      ok = __shfl_sync(FULL, ok, 0);
+    };
+    int64_t row1 = -1, row2 = -1;
+    float weight1 = 0.f, weight2 = 0.f;
+    hand(row, weight);
+    if (row >= 0) hand(row1, weight1);
+    for (; ok && row >= 0; row = row1, weight = weight1, row1 = row2, weight1 = weight2) {
+      row2 = -1;
+      if (row1 >= 0) hand(row2, weight2);
+      if (!ok) break;
+      if (weight == 0.f) continue;
+      if (lane == 0) {
+        const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
+        const int v0 = (int)((int64_t)R.nv * rank / size);
+        const int v1 = (int)((int64_t)R.nv * (rank + 1) / size);
+        const int lo = max(v0, R.off ? 1 : 0), hi = min(v1, (R.V + R.off) / A);  // whole vectors
+        const int C = (v1 - v0 + CV - 1) / CV, again = max(C - SLOTS, 0);
+        for (int c = 0; c < C + again; ++c, ++it) {
+          const int slot = it % SLOTS, v = v0 + (c < C ? c : c - C) * CV;
+          if (it >= SLOTS && !(ok = bar_wait(&S.empty[slot], (it / SLOTS - 1) & 1, dead))) break;
+          const int a = max(v, lo), b = min(v + CV, hi);
+          if (b > a) {
+            bar_expect(&S.full[slot], (uint32_t)(b - a) * 16);
+            bulk_load(ring + (size_t)slot * CV + (a - v), R.p + ((int64_t)a * A - R.off),
+                      (uint32_t)(b - a) * 16, &S.full[slot], c >= again, once);
+          } else {
+            bar_arrive(&S.full[slot]);
+          }
         }
+      }
+      ok = __shfl_sync(FULL, ok, 0);
     }
-    return;
-  }
-
-  if (w == CW + 1) {  // ---- the list's warp
+    // no copy of this CTA may land behind its end
+    if (lane == 0 && *dead)
+      for (uint32_t k = it > SLOTS ? it - SLOTS : 0; k < it; ++k) {
+        int none = 0;
+        bar_wait(&S.full[k % SLOTS], (k / SLOTS) & 1, &none);
+      }
+  } else if (w > CW) {  // ---- the lists' warps
+    const int mine = w - CW - 1;
+    StepRow& B = S.row[mine];
     uint32_t live = 0;
-    for (uint32_t i = 0;; ++i) {
-      if (!bar_wait(&S.row_full[i % ROWQ], (i / ROWQ) & 1, dead)) break;
-      const int row = S.row[i % ROWQ];
-      __syncwarp();
-      if (lane == 0) bar_arrive(&S.row_empty[i % ROWQ]);
-      if (row < 0) break;
-      const float weight = P.weights ? P.weights[row] : 1.f;
+    while (next_row(row, weight)) {
       if (weight == 0.f) {
-        if (lane == 0) P.loss[row] = 0.f;
+        if (mine == 0 && rank == 0 && lane == 0) P.loss[row] = 0.f;
         continue;
       }
-      const int b = live & 1;
-      list_begin<T>(P, row, S.list);
-      if (live >= 2 && !bar_wait(&S.list_empty[b], (live / 2 - 1) & 1, dead)) break;
-      const int off = (int)(((uintptr_t)(static_cast<const T*>(P.logits) + (int64_t)row * P.ld) & 15) /
-                            sizeof(T));
-      uint32_t* mk = marks + b * words;
+      const uint32_t use = live / LW;
+      if ((int)(live++ % LW) != mine) continue;
+      const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
+      const int v0 = (int)((int64_t)R.nv * rank / size);
+      const int v1 = (int)((int64_t)R.nv * (rank + 1) / size);
+      list_begin<T>(P, row, B.list);
+      if (use > 0 && !bar_wait(&B.list_empty, (use - 1) & 1, dead)) break;
       for (int j = lane; j < P.k; j += 32)
-        if (S.at[b][j] >= 0) mk[S.at[b][j] / A / 32] = 0;
+        if (B.at[j] >= 0) *mark(B.marks, B.at[j] / A) = 0;
       __syncwarp();
       for (int j = lane; j < P.k; j += 32) {
-        const int id = S.list.id[j];
-        const int at = id >= 0 && id < P.V ? id + off : -1;
-        S.at[b][j] = at;
-        if (at >= 0) atomicOr(&mk[at / A / 32], 1u << (at / A & 31));
+        const int id = B.list.id[j], at = id + R.off - v0 * A;
+        const bool in = id >= 0 && id < P.V && at >= 0 && at < (v1 - v0) * A;
+        B.at[j] = in ? at : -1;
+        if (in) atomicOr(mark(B.marks, at / A), 1u << (at / A & 31));
       }
       __syncwarp();
-      if (lane == 0) bar_arrive(&S.list_full[b]);
-      if (!bar_wait(&S.summed, live & 1, dead)) break;
-      // the warps' sums, joined in a fixed order
-      const float pm = lane < CW ? S.part_m[lane] : neg_inf(), ps = lane < CW ? S.part_s[lane] : 0.f;
-      const float m = warp_max(pm);
-      const double r =
-          warp_sum(ps == 0.f ? 0.0 : (double)ps * (double)exp2f((pm - m) * P.scale));
-      const Solved sol = list_solve(P, S.list, m, r);
-      const Stat st = list_grads(P, S.list, sol, m, r, weight * P.inv_t, S.listg[b]);
-      if (lane == 0) S.out = StepRow{st.m, st.coef};
+      if (lane == 0) bar_arrive(&B.list_full);
+      if (!bar_wait(&B.summed, use & 1, dead)) break;
+      // this CTA's sum to all, and all joined: in a fixed order, the same in every CTA
+      float pm = lane < CW ? B.part_m[lane] : neg_inf(), ps = lane < CW ? B.part_s[lane] : 0.f;
+      float m = warp_max(pm);
+      float s = ps == 0.f ? 0.f : ps * exp2f((pm - m) * P.scale);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
+      double r = s;
+      if (size > 1) {
+        if (lane == 0) bar_expect(&B.joined, size * 8);
+        __syncwarp();
+        if (lane < size)
+          send(&B.part[rank], &B.joined, lane,
+               (uint64_t)__float_as_uint(s) << 32 | __float_as_uint(m));
+        if (!bar_wait<true>(&B.joined, use & 1, dead)) break;
+        const uint64_t got = lane < size ? B.part[lane] : 0;
+        pm = __uint_as_float((uint32_t)got);
+        ps = __uint_as_float((uint32_t)(got >> 32));
+        if (ps == 0.f) pm = neg_inf();
+        m = warp_max(pm);
+        r = warp_sum(ps == 0.f ? 0.0 : (double)ps * (double)exp2f((pm - m) * P.scale));
+      }
+      const Solved sol = list_solve(P, B.list, m, r);
+      const Stat st = list_grads(P, B.list, sol, m, r, weight * P.inv_t, B.listg);
+      if (lane == 0) {
+        B.m = st.m;
+        B.coef = st.coef;
+      }
       __syncwarp();
-      if (lane == 0) bar_arrive(&S.solved);
-      const float loss = list_loss(P, S.list, sol);
-      if (lane == 0) P.loss[row] = loss * weight;
+      if (lane == 0) bar_arrive(&B.solved);
+      const float loss = list_loss(P, B.list, sol);
+      if (rank == 0 && lane == 0) P.loss[row] = loss * weight;
       __syncwarp();
-      ++live;
     }
     if (lane == 0 && *dead && P.status) atomicOr(P.status, (int)VINFER_ST_INTERNAL);
-    return;
-  }
-
-  // ---- the warps that sum and write
-  uint32_t it = 0, live = 0;  // chunks and rows so far
-  const uint64_t scale2 = pair(P.scale, P.scale);
-  for (uint32_t i = 0;; ++i) {
-    if (!bar_wait(&S.row_full[i % ROWQ], (i / ROWQ) & 1, dead)) break;
-    const int row = S.row[i % ROWQ];
-    __syncwarp();
-    if (lane == 0) bar_arrive(&S.row_empty[i % ROWQ]);
-    if (row < 0) break;
-    const Row<T> R(static_cast<const T*>(P.logits) + (int64_t)row * P.ld, P.V);
-    T* out = static_cast<T*>(P.grad) + (int64_t)row * P.ldg;
-    const bool aligned = (int)(((uintptr_t)out & 15) / sizeof(T)) == R.off;
-    const int C = (R.nv + CV - 1) / CV, again = C > SLOTS ? C - SLOTS : 0;
-    const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;
-
-    // the thread's vectors of a chunk: in the ring, at the row's ragged ends from memory
-    auto take = [&](int chunk, uint32_t n, uint4 (&q)[CU]) {
+  } else {  // ---- the warps that sum and write
+    const uint64_t scale2 = pair(P.scale, P.scale);
+    // the thread's vectors of the chunk that begins at v: in the ring, at the row's ragged ends (or
+    // behind the slice) from memory
+    auto take = [&](const Row<T>& R, int v, int v1, bool inside, uint32_t n, uint4 (&q)[CU]) {
       const uint4* src = ring + (size_t)(n % SLOTS) * CV + tid;
 #pragma unroll
       for (int u = 0; u < CU; ++u) q[u] = src[u * CT];
-      const int v0 = chunk * CV;
-      if (v0 < lo || v0 + CV > hi) {
+      if (!inside) {
+        const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;
 #pragma unroll
         for (int u = 0; u < CU; ++u) {
-          const int v = v0 + u * CT + tid;
-          const uint32_t ni = VT::NEG_INF_WORD;
-          if (v >= R.nv) q[u] = make_uint4(ni, ni, ni, ni);
-          else if (v < lo || v >= hi) q[u] = R.edge(R.p, R.V, v * A - R.off);
+          const int x = v + u * CT + tid;
+          if (x < lo || x >= min(hi, v1))
+            q[u] = R.edge(R.p, x < v1 ? R.V : 0, x * A - R.off);  // all -inf behind the slice
         }
-      }
-    };
-    auto put = [&](int v, const float (&g)[A]) {
-      const int64_t e0 = (int64_t)v * A - R.off;
-      if (aligned && v >= lo && v < hi) {
-        *reinterpret_cast<uint4*>(out + e0) = VT::pack(g);
-      } else {
-#pragma unroll
-        for (int j = 0; j < A; ++j)
-          if (e0 + j >= 0 && e0 + j < P.V) out[e0 + j] = VT::round(g[j]);
       }
     };
 
-    if (P.weights && P.weights[row] == 0.f) {
-      float g[A];
-#pragma unroll
-      for (int j = 0; j < A; ++j) g[j] = 0.f;
-      for (int v = tid; v < R.nv; v += CT) put(v, g);
-      continue;
-    }
-    const int b = live & 1;
-    const uint32_t* mk = marks + b * words;
-    if (!bar_wait(&S.list_full[b], (live / 2) & 1, dead)) break;
-    float m = neg_inf(), s = 0.f;
+    uint32_t it = 0, live = 0;  // chunks and rows so far
     bool ok = true;
-    for (int c = 0; c < C; ++c, ++it) {
-      if (!(ok = bar_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead))) break;
-      uint4 q[CU];
-      take(c, it, q);
-      if (c < C - SLOTS) {  // not held for the gradient
-        __syncwarp();
-        if (lane == 0) bar_arrive(&S.empty[it % SLOTS]);
+    while (ok && next_row(row, weight)) {
+      T* out = static_cast<T*>(P.grad) + row * P.ldg;
+      if (weight == 0.f) {
+        const int a = (int)((int64_t)P.V * rank / size), b = (int)((int64_t)P.V * (rank + 1) / size);
+        const int head = min(b, a + (int)((16 - ((uintptr_t)(out + a) & 15)) % 16 / sizeof(T)));
+        const int body = head + (b - head) / A * A;
+        for (int e = a + tid; e < head; e += CT) out[e] = VT::round(0.f);
+        for (int e = head + tid * A; e < body; e += CT * A)
+          store_once(out + e, make_uint4(0, 0, 0, 0), once);
+        for (int e = body + tid; e < b; e += CT) out[e] = VT::round(0.f);
+        continue;
       }
-#pragma unroll
-      for (int u = 0; u < CU; ++u) {
-        const int first = c * CV + u * CT + w * 32;
-        if (const uint32_t word = mk[first / 32]) take_out<T>(q[u], word, S.at[b], P.k, first);
-      }
-      add_exps<T>(q, VT::max(q), P.scale, m, s);
-    }
-    if (!ok) break;
-    if (s == 0.f) m = neg_inf();
-    const float mw = warp_max(m);
-    float sw = s == 0.f ? 0.f : s * ex2((m - mw) * P.scale);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sw += __shfl_xor_sync(FULL, sw, o);
-    if (lane == 0) {
-      S.part_m[w] = mw;
-      S.part_s[w] = sw;
-      bar_arrive(&S.summed);
-    }
-    __syncwarp();
-    if (!bar_wait(&S.solved, live & 1, dead)) break;
-    const StepRow o = S.out;
-    const uint64_t neg_m = pair(-o.m, -o.m), coef = pair(o.coef, o.coef);
-    // chunks the ring still holds, in order, then the others once more
-    const int held = C - again;
-    for (int k = 0; k < C; ++k) {
-      const int c = k < held ? again + k : k - held;
-      const uint32_t n = k < held ? it - held + k : it + (k - held);
-      if (k >= held && !(ok = bar_wait(&S.full[n % SLOTS], (n / SLOTS) & 1, dead))) break;
-      uint4 q[CU];
-      take(c, n, q);
-      __syncwarp();
-      if (lane == 0) bar_arrive(&S.empty[n % SLOTS]);
-#pragma unroll
-      for (int u = 0; u < CU; ++u) {
-        const int first = c * CV + u * CT + w * 32, v = first + lane;
-        uint64_t h[A / 2];
-        float g[A];
-        VT::pairs(q[u], h);
-#pragma unroll
-        for (int j = 0; j < A / 2; ++j)
-          split(mul2(ex2_2(mul2(add2(h[j], neg_m), scale2)), coef), g[2 * j], g[2 * j + 1]);
-        for (uint32_t word = mk[first / 32]; word; word &= word - 1) {  // listed elements
-          const int l = __ffs(word) - 1;
-          for (int j0 = 0; j0 < P.k; j0 += 32) {
-            const int at = j0 + lane < P.k ? S.at[b][j0 + lane] : -1;
-            unsigned who = __ballot_sync(FULL, at >= 0 && at / A == first + l);
-            for (; who; who &= who - 1) {
-              const int j = j0 + __ffs(who) - 1;
-              const int e = S.at[b][j] & (A - 1);
-              if (lane == l) {
-#pragma unroll
-                for (int a = 0; a < A; ++a)
-                  if (a == e) g[a] = S.listg[b][j];
-              }
-            }
-          }
+      const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
+      const bool aligned = (int)(((uintptr_t)out & 15) / sizeof(T)) == R.off;
+      const int v0 = (int)((int64_t)R.nv * rank / size);
+      const int v1 = (int)((int64_t)R.nv * (rank + 1) / size);
+      const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;
+      const int C = (v1 - v0 + CV - 1) / CV, again = max(C - SLOTS, 0);
+      StepRow& B = S.row[live % LW];
+      const uint32_t use = live++ / LW;
+      if (!(ok = bar_wait(&B.list_full, use & 1, dead))) break;
+      float m = neg_inf(), s = 0.f;
+      for (int c = 0; c < C; ++c, ++it) {
+        if (!(ok = bar_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead))) break;
+        const int v = v0 + c * CV;
+        uint4 q[CU];
+        take(R, v, v1, v >= lo && v + CV <= min(hi, v1), it, q);
+        if (c < again) {  // not held for the gradient
+          __syncwarp();
+          if (lane == 0) bar_arrive(&S.empty[it % SLOTS]);
         }
-        if (v < R.nv) put(v, g);
+        const uint4 mk = B.marks[c * CW + w];
+        if (mk.x | mk.y | mk.z | mk.w) {
+          const int f = c * CV + w * 32;
+          if (mk.x) q[0] = take_out<T>(q[0], mk.x, B.at, P.k, f);
+          if (mk.y) q[1] = take_out<T>(q[1], mk.y, B.at, P.k, f + CT);
+          if (mk.z) q[2] = take_out<T>(q[2], mk.z, B.at, P.k, f + 2 * CT);
+          if (mk.w) q[3] = take_out<T>(q[3], mk.w, B.at, P.k, f + 3 * CT);
+        }
+        add_exps<T>(q, VT::max(q), P.scale, m, s);
       }
+      if (!ok) break;
+      if (s == 0.f) m = neg_inf();
+      const float mw = warp_max(m);
+      float sw = s == 0.f ? 0.f : s * ex2((m - mw) * P.scale);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sw += __shfl_xor_sync(FULL, sw, o);
+      if (lane == 0) {
+        B.part_m[w] = mw;
+        B.part_s[w] = sw;
+        bar_arrive(&B.summed);
+      }
+      __syncwarp();
+      if (!(ok = bar_wait(&B.solved, use & 1, dead))) break;
+      const uint64_t neg_m = pair(-B.m, -B.m), coef = pair(B.coef, B.coef);
+      // the chunks the ring still holds, in order, then the others once more
+      const int held = C - again;
+      const uint32_t n0 = it - held;
+      for (int k = 0; k < C; ++k) {
+        const int c = k < held ? again + k : k - held;
+        const uint32_t n = n0 + k;
+        if (k >= held && !(ok = bar_wait(&S.full[n % SLOTS], (n / SLOTS) & 1, dead))) break;
+        const int v = v0 + c * CV;
+        const bool inside = v >= lo && v + CV <= min(hi, v1);
+        uint4 q[CU];
+        take(R, v, v1, inside, n, q);
+        __syncwarp();
+        if (lane == 0) bar_arrive(&S.empty[n % SLOTS]);
+        const uint4 mk = B.marks[c * CW + w];
+        const uint32_t any[CU] = {mk.x, mk.y, mk.z, mk.w};
+        T* to = out + ((int64_t)(v + tid) * A - R.off);
+#pragma unroll
+        for (int u = 0; u < CU; ++u) {
+          uint64_t h[A / 2];
+          float g[A];
+          VT::pairs(q[u], h);
+#pragma unroll
+          for (int j = 0; j < A / 2; ++j)
+            split(mul2(ex2_2(mul2(add2(h[j], neg_m), scale2)), coef), g[2 * j], g[2 * j + 1]);
+          const uint4 r = VT::pack(g);
+          if (inside && aligned) {
+            store_once(to + u * CT * A, r, once);
+          } else {
+            const int x = v + u * CT + tid;
+            if (x < v1) store_ragged(out, r, x * A - R.off, P.V);
+          }
+          if (any[u])
+            store_listed(out + ((int64_t)v0 * A - R.off), any[u], B.at, B.listg, P.k,
+                         c * CV + u * CT + w * 32);
+        }
+      }
+      if (!ok) break;
+      it += again;
+      __syncwarp();
+      if (lane == 0) bar_arrive(&B.list_empty);
     }
-    if (!ok) break;
-    it += again;
-    __syncwarp();
-    if (lane == 0) bar_arrive(&S.list_empty[b]);
-    ++live;
   }
+  __syncwarp();
+  if (size > 1) cluster_sync();  // no sum is sent to a CTA that has left
 }
 
 // Parts of a row: enough CTAs to fill the 148 SMs several times over, at least two vectors a
@@ -691,12 +808,6 @@ int distill_parts(int64_t rows_, int64_t vocab, int dtype) {
   int64_t p = (148 * 8 + rows_ - 1) / rows_;
   p = std::min<int64_t>(p, (nv + 2 * NT - 1) / (2 * NT));
   return (int)std::max<int64_t>(1, std::min<int64_t>(p, MAX_PARTS));
-}
-
-// Rows taken whole by one CTA each, where there are enough and they are long.
-bool step_in_one(const DistP& P, int dtype) {
-  const int64_t bytes = (int64_t)P.V * (dtype == VINFER_DTYPE_BF16 ? 2 : 4);
-  return P.rows >= 2 * 148 * STEP_CTAS && bytes >= (64 << 10);
 }
 
 int check(const VinferDistillArgs* a) {
@@ -733,27 +844,78 @@ template <typename T>
 int launch_loss(const DistP& P, cudaStream_t st) {
   const int part_vecs = (P.V / Vec<T>::A + 2 + P.parts - 1) / P.parts + 1;
   const size_t smem = (size_t)(part_vecs + NT * U - 1) / (NT * U) * (NT * U / 8);
-  const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, smem, st, false, P);
+  const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, smem, st, false, 1, P);
   if (rc != VINFER_OK) return rc;
-  return launch(k_distill_finish<T>, (unsigned)((P.rows + FW - 1) / FW), FW * 32, 0, st, true, P);
+  return launch(k_distill_finish<T>, (unsigned)((P.rows + FW - 1) / FW), FW * 32, 0, st, true, 1, P);
 }
 
 template <typename T>
 int launch_grad(const DistP& P, cudaStream_t st, bool dependent) {
-  return launch(k_distill_grad<T>, (unsigned)(P.rows * P.parts), NT, 0, st, dependent, P);
+  return launch(k_distill_grad<T>, (unsigned)(P.rows * P.parts), NT, 0, st, dependent, 1, P);
 }
 
-size_t step_smem(int V, int A) {
-  return (size_t)SLOTS * CV * 16 + sizeof(StepS) + 2 * (size_t)step_chunks(V, A) * (CV / 8);
+// The CTAs a row is cut into, a power of two: none when even the largest cluster cannot hold one.
+// A single CTA is launched without a cluster dimension and uses nothing of one.
+int step_cluster(int64_t V, int A) {
+  const int64_t nv = (V + 2 * A - 2) / A;  // at any alignment
+  for (int c = MINC; c <= MAXC; c *= 2)
+    if ((nv + c - 1) / c <= SLICE * CV) return c;
+  return 0;
+}
+
+constexpr size_t STEP_SMEM = (size_t)SLOTS * CV * 16 + sizeof(StepS);
+static_assert(STEP_CTAS * (STEP_SMEM + 1024) <= 228 * 1024, "STEP_CTAS fit an SM");
+
+// Clusters of c CTAs that fit the current device at once (a property of the device: asked once).
+template <typename T>
+int step_clusters(int c, int* clusters) {
+  static std::atomic<int> known[64][MAXC + 1];
+  int dev = 0;
+  if (result(cudaGetDevice(&dev)) != VINFER_OK || dev < 0 || dev >= 64) return VINFER_E_CUDA;
+  *clusters = known[dev][c].load();
+  if (*clusters > 0) return VINFER_OK;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = c;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(148 * STEP_CTAS / c * c);
+  cfg.blockDim = dim3(STEP_T);
+  cfg.dynamicSmemBytes = STEP_SMEM;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (c == 1) {
+    *clusters = 148 * STEP_CTAS;
+    return VINFER_OK;
+  }
+  const int rc = result(cudaOccupancyMaxActiveClusters(clusters, k_distill_step<T>, &cfg));
+  if (rc != VINFER_OK || *clusters < 1) return VINFER_E_CUDA;
+  known[dev][c].store(*clusters);
+  return VINFER_OK;
 }
 
 template <typename T>
-int launch_step(const DistP& P, int* next_row, cudaStream_t st) {
-  const size_t smem = step_smem(P.V, Vec<T>::A);
-  if (opt_in(k_distill_step<T>, smem) != VINFER_OK) return VINFER_E_CUDA;
-  if (result(cudaMemsetAsync(next_row, 0, sizeof(int), st)) != VINFER_OK) return VINFER_E_CUDA;
-  return launch(k_distill_step<T>, (unsigned)std::min<int64_t>(P.rows, 148 * STEP_CTAS), STEP_T, smem, st, false,
-                P, next_row);
+int launch_step(const DistP& P, cudaStream_t st) {
+  const int c = step_cluster(P.V, Vec<T>::A);
+  if (opt_in(k_distill_step<T>, STEP_SMEM) != VINFER_OK) return VINFER_E_CUDA;
+  if (c > 8 && result(cudaFuncSetAttribute(k_distill_step<T>,
+                                           cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) !=
+                   VINFER_OK)
+    return VINFER_E_CUDA;
+  int clusters = 0;
+  if (step_clusters<T>(c, &clusters) != VINFER_OK) return VINFER_E_CUDA;
+  return launch(k_distill_step<T>, (unsigned)(std::min<int64_t>(P.rows, clusters) * c), STEP_T,
+                STEP_SMEM, st, false, (unsigned)c, P);
+}
+
+// One pass where rows are long and there are enough of them to fill the clusters; otherwise the three
+// kernels, whose second read of short rows comes from L2 anyway. Measured (us, one pass against
+// three kernels, rows of 151,936 bf16): 31.2 / 24.4 at 32 rows, 33.5 / 43.4 at 148, 169 / 219 at
+// 1,200; 1,200 rows of 65,536 bf16 103 / 100, of 33,000 bf16 80 / 67, of 33,000 float32 86 / 104.
+bool step_in_one(const DistP& P, int dtype) {
+  const bool bf = dtype == VINFER_DTYPE_BF16;
+  const int64_t bytes = (int64_t)P.V * (bf ? 2 : 4);
+  return P.rows >= 96 && bytes >= (bf ? 160 << 10 : 96 << 10) && step_cluster(P.V, bf ? 8 : 4) > 0;
 }
 
 size_t align_up(size_t n) { return (n + 255) / 256 * 256; }
@@ -834,8 +996,8 @@ int vinfer_distill_step(const VinferDistillArgs* a, float* loss, void* grad, int
   P.ldg = ld_grad;
   cudaStream_t st = (cudaStream_t)stream;
   if (step_in_one(P, a->dtype))
-    return a->dtype == VINFER_DTYPE_BF16 ? launch_step<__nv_bfloat16>(P, (int*)workspace, st)
-                                         : launch_step<float>(P, (int*)workspace, st);
+    return a->dtype == VINFER_DTYPE_BF16 ? launch_step<__nv_bfloat16>(P, st)
+                                         : launch_step<float>(P, st);
   if (a->dtype == VINFER_DTYPE_BF16) {
     rc = launch_loss<__nv_bfloat16>(P, st);
     return rc != VINFER_OK ? rc : launch_grad<__nv_bfloat16>(P, st, true);

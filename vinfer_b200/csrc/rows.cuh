@@ -361,31 +361,90 @@ __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
                "r"(bytes)
                : "memory");
 }
+// Each try may leave the warp suspended this long: a poll that came back at once would take issue
+// slots from the warps that compute.
+constexpr uint32_t SUSPEND_NS = 1000000;
 // Waits for the phase of this parity to end; false after a bounded number of tries (seconds), or
 // once another wait of the CTA has given up: *dead is then set, and every role leaves.
+// CLUSTER: what other CTAs of the cluster sent is seen behind it.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* dead) {
   const uint32_t a = smem_addr(b);
-  for (int i = 0; i < (1 << 22); ++i) {
+  for (int i = 0; i < 1 << 20; ++i) {
     uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(a), "r"(parity)
-        : "memory");
+    if (CLUSTER)
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(a), "r"(parity), "r"(SUSPEND_NS)
+          : "memory");
+    else
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(a), "r"(parity), "r"(SUSPEND_NS)
+          : "memory");
     if (done) return true;
     if (*dead) return false;
   }
   *dead = 1;
   return false;
 }
-// bytes: a multiple of 16, both addresses 16-byte aligned; completes on the barrier
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* b) {
-  asm volatile(
-      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_addr(dst)),
-      "l"(src), "r"(bytes), "r"(smem_addr(b))
-      : "memory");
+// L2 policy for data that is not needed again
+__device__ __forceinline__ uint64_t evict_first() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void store_once(void* dst, const uint4& q, uint64_t policy) {
+  asm volatile("st.global.L2::cache_hint.v4.b32 [%0], {%1, %2, %3, %4}, %5;" ::"l"(dst), "r"(q.x),
+               "r"(q.y), "r"(q.z), "r"(q.w), "l"(policy)
+               : "memory");
+}
+// bytes: a multiple of 16, both addresses 16-byte aligned; completes on the barrier. `once`: the
+// bytes are not read again (policy: evict_first()).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* b,
+                                          bool once, uint64_t policy) {
+  if (once)
+    asm volatile(
+        "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], "
+        "%2, [%3], %4;" ::"r"(smem_addr(dst)),
+        "l"(src), "r"(bytes), "r"(smem_addr(b)), "l"(policy)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+            smem_addr(dst)),
+        "l"(src), "r"(bytes), "r"(smem_addr(b))
+        : "memory");
+}
+
+// ---- clusters ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::
+                   : "memory");
+}
+// Stores 8 bytes in another CTA's shared memory and counts them on its barrier.
+__device__ __forceinline__ void send(void* dst, uint64_t* bar, uint32_t rank, uint64_t value) {
+  uint32_t d, b;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(dst)), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_addr(bar)), "r"(rank));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(d),
+               "l"(value), "r"(b)
+               : "memory");
 }
 
 __device__ __forceinline__ void grid_dependency_wait() {
@@ -416,21 +475,30 @@ int opt_in(K kern, size_t smem) {
   return result(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
 }
 
-// One launch; `dependent`: may begin while the stream's kernel before it drains (that kernel's
-// writes are read behind grid_dependency_wait()).
+// One launch, of clusters of `cluster` CTAs; `dependent`: may begin while the stream's kernel before
+// it drains (that kernel's writes are read behind grid_dependency_wait()).
 template <typename... KA, typename... A>
 int launch(void (*kern)(KA...), unsigned grid, unsigned block, size_t smem, cudaStream_t st,
-           bool dependent, A... args) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+           bool dependent, unsigned cluster, A... args) {
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid);
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = n;
   return result(cudaLaunchKernelEx(&cfg, kern, args...));
 }
 
