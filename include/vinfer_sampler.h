@@ -298,7 +298,8 @@ int vinfer_reorder_states(const VinferState* states, int32_t n_states, const int
  *  - vinfer_distill_loss: losses [rows]; row_stats (float [rows, 2], 8-byte aligned) and list_grads
  *    (float [rows, k]) receive what the gradient needs, both or neither.
  *  - vinfer_distill_grad: d(sum_r grad_out[r] * loss[r]) / dlogits, of the logits' type, rounded once
- *    (grad_out NULL: ones). args as for the loss. grad may be the logits (then with their ld).
+ *    (grad_out NULL: ones; its stride in elements, 0 for one value shared by all rows). args as for
+ *    the loss. grad may be the logits (then with their ld).
  *  - vinfer_distill_step: both in one call, grad_out all ones. grad may be the logits.
  * The workspace needs no initialisation and holds nothing between calls; 16-byte aligned. */
 #define VINFER_DISTILL_MAX_K 128
@@ -321,8 +322,8 @@ size_t vinfer_distill_workspace_bytes(int64_t rows, int64_t vocab, int32_t dtype
 int vinfer_distill_loss(const VinferDistillArgs* args, float* loss, float* row_stats,
                         float* list_grads, void* workspace, size_t workspace_bytes, void* stream);
 int vinfer_distill_grad(const VinferDistillArgs* args, const float* row_stats,
-                        const float* list_grads, const float* grad_out, void* grad,
-                        int64_t ld_grad, void* stream);
+                        const float* list_grads, const float* grad_out, int64_t grad_out_stride,
+                        void* grad, int64_t ld_grad, void* stream);
 int vinfer_distill_step(const VinferDistillArgs* args, float* loss, void* grad, int64_t ld_grad,
                         void* workspace, size_t workspace_bytes, void* stream);
 

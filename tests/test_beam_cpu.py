@@ -86,7 +86,8 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.vinfer_distill_loss(C.byref(d), 16, 16, None, 16, big, None) == _lib.E_ARG
     assert lib.vinfer_distill_loss(C.byref(d), 16, None, None, 16, 8, None) == _lib.E_LIMIT
     assert lib.vinfer_distill_step(C.byref(d), 16, 16, 9, 16, big, None) == _lib.E_ARG
-    assert lib.vinfer_distill_grad(C.byref(d), 16, None, None, 16, 10, None) == _lib.E_ARG
+    assert lib.vinfer_distill_grad(C.byref(d), 16, None, None, 0, 16, 10, None) == _lib.E_ARG
+    assert lib.vinfer_distill_grad(C.byref(d), 16, 16, 16, -1, 16, 10, None) == _lib.E_ARG
     for t in (0.0, -1.0, float("inf"), float("nan")):
         d.temperature = t
         assert lib.vinfer_distill_loss(C.byref(d), 16, None, None, 16, big, None) == _lib.E_ARG

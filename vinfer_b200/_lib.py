@@ -212,7 +212,7 @@ def load() -> C.CDLL:
                                         C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
     lib.vinfer_distill_grad.restype = C.c_int
     lib.vinfer_distill_grad.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p,
-                                        C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]
+                                        C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]
     lib.vinfer_distill_step.restype = C.c_int
     lib.vinfer_distill_step.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p, C.c_int64,
                                         C.c_void_p, C.c_size_t, C.c_void_p]

@@ -21,7 +21,7 @@ namespace {
 using namespace rows;
 
 constexpr int NT = 256, NW = NT / 32;
-constexpr int U = 8;              // 16-byte vectors a thread holds: 32 KiB a CTA and round
+constexpr int U = 4;              // 16-byte vectors of a thread and round: 16 KiB a CTA
 constexpr int MAX_PARTS = 64;     // parts of a row
 constexpr int MAX_JOIN = 1024;    // entries of a beam's parts together (a warp joins them)
 constexpr int MAX_STAGED = 8192;  // entries of a request's parts together (64 KiB staged)
@@ -58,11 +58,11 @@ struct RowsP {
 };
 constexpr u64 NONE = ~0ull;
 
-constexpr int DCAP = 512;  // delegates: vectors that may hold one of the part's n best
+constexpr int DCAP = 1024; // delegates: threads' rounds that may hold one of the part's n best
 constexpr int LCAP = 1024; // their elements that still may
 struct Delegates {         // dynamic shared memory of k_beam_rows
-  uint4 q[DCAP];
-  int e0[DCAP];            // id of the vector's first element
+  int v[DCAP];             // the round's first vector of the thread
+  float mx[DCAP];          // the largest element
   u64 list[LCAP];
 };
 struct RowsS {
@@ -225,12 +225,12 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
   extern __shared__ __align__(16) unsigned char dyn[];
   Delegates& D = *reinterpret_cast<Delegates*>(dyn);
   __shared__ RowsS S;
-  const int row = blockIdx.x / P.parts, part = blockIdx.x - row * P.parts;
+  const uint32_t row = blockIdx.x / (uint32_t)P.parts, part = blockIdx.x - row * P.parts;
   const float b = P.scores[row];
   if (!(b > neg_inf() && b < -neg_inf())) return;  // dead, or refused by k_beam_pick
   const Row<T> R(static_cast<const T*>(P.logits) + (int64_t)row * P.ld, P.V);
-  const int v0 = (int)((int64_t)R.nv * part / P.parts);
-  const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
+  const int v0 = (int)(R.nv * part / P.parts);  // below 2^18 * 64
+  const int v1 = (int)(R.nv * (part + 1) / P.parts);
   const int n = P.n, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   if (tid == 0) {
     S.nd = 0;
@@ -238,17 +238,16 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
   }
 
   // The bar: a logit that at least n lanes' maxima, so at least n elements, reach: the smallest of
-  // the warps' k-th largest lane maxima (8k >= n). A vector below it holds none of the n best; the
-  // others (about 3n a round) are kept as delegates. The warps raise it as their maxima rise;
-  // a warp that still sees the older, lower one keeps a few vectors more.
-  float m = neg_inf(), s = 0.f;
+  // the warps' k-th largest lane maxima (8k >= n). A thread's round below it holds none of the n
+  // best; the others (about 3n in the first round) are noted as delegates. The warps raise it as
+  // their maxima rise; a warp that still sees an older, lower one notes a few more.
+  Exps sum(L2E);
   float seen = neg_inf();  // this lane's largest element so far
   const int k = (n + NW - 1) / NW;
   volatile float* kth = S.kth;
+  float bar = neg_inf();
   int round = 0;
-  for (int vb = v0; vb < v1; vb += NT * U, ++round) {
-    uint4 q[U];
-    R.template load_round<U, NT>(vb, v1, q);
+  auto work = [&](const uint4 (&q)[U], int vb) {
     const float mx = V8::max(q);
     seen = fmaxf(seen, mx);
     if ((round & (round + 1)) == 0) {  // rounds 0, 1, 3, 7, ...
@@ -260,42 +259,40 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
       }
       if (lane == 0) kth[w] = from_okey(top);
       if (round == 0) __syncthreads();
+      bar = kth[0];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) bar = fminf(bar, kth[i]);
     }
-    float bar = kth[0];
-#pragma unroll
-    for (int i = 1; i < NW; ++i) bar = fminf(bar, kth[i]);
-    if (__any_sync(FULL, mx >= bar)) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const bool keep = V8::max(q[u]) >= bar;
-        const unsigned who = __ballot_sync(FULL, keep);
-        if (who) {
-          int at = 0;
-          if (lane == 0) at = atomicAdd(&S.nd, __popc(who));
-          at = __shfl_sync(FULL, at, 0) + __popc(who & ((1u << lane) - 1));
-          if (keep && at < DCAP) {
-            D.q[at] = q[u];
-            D.e0[at] = (vb + u * NT + tid) * A - R.off;
-          }
-        }
+    ++round;
+    if (mx >= bar) {
+      const int at = atomicAdd(&S.nd, 1);
+      if (at < DCAP) {
+        D.v[at] = vb + tid;
+        D.mx[at] = mx;
       }
     }
-    add_exps<T>(q, mx, L2E, m, s);
-  }
+    sum.add<T>(q, mx);
+  };
+  stream_rounds<U, NT>(R, v0, v1, work);
   __syncthreads();
 
-  // the delegates' elements that reach the final bar, one a thread
-  float bar = S.kth[0];
+  // the delegates' elements that reach the final bar: their vectors are read again, from L2
+  bar = S.kth[0];
 #pragma unroll
   for (int i = 1; i < NW; ++i) bar = fminf(bar, S.kth[i]);
   bool careful = !(bar > neg_inf()) || S.nd > DCAP;
   if (!careful) {
-    for (int i = tid; i < S.nd * A; i += NT) {
-      const T* x = reinterpret_cast<const T*>(&D.q[i / A]) + i % A;
-      const float f = V8::load(x);
-      if (f >= bar) {
-        const int at = atomicAdd(&S.cnt, 1);
-        if (at < LCAP) D.list[at] = entry(f, D.e0[i / A] + i % A);
+    for (int i = tid; i < S.nd * U; i += NT) {
+      const int v = D.v[i / U] + i % U * NT;
+      if (D.mx[i / U] < bar || v >= v1) continue;
+      const uint4 q = R.load(v);
+      if (V8::max(q) < bar) continue;
+      for (int j = 0; j < A; ++j) {
+        const float f = V8::get(q, j);
+        if (f >= bar) {
+          const int at = atomicAdd(&S.cnt, 1);
+          if (at < LCAP) D.list[at] = entry(f, v * A - R.off + j);
+        }
       }
     }
     __syncthreads();
@@ -324,8 +321,8 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
     if (rank < n) out[rank] = e;
   }
   for (int i = have + tid; i < n; i += NT) out[i] = NONE;
-  block_join<NW>(m, s, L2E, S.f);
-  if (tid == 0) P.hdr[at] = PartHdr{m, s, {0, 0}};
+  block_join<NW>(sum.m, sum.s, L2E, S.f);
+  if (tid == 0) P.hdr[at] = PartHdr{sum.m, sum.s, {0, 0}};
 }
 
 struct PickP {
@@ -593,15 +590,11 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
   }
 }
 
-// Parts of a row: enough CTAs to fill the 148 SMs several times over, at least two vectors a
-// thread in each, and no more entries than a warp joins.
-int beam_parts(int64_t rows, int W, int64_t vocab, int dtype, int n) {
+// Parts of a row, no more entries than a warp joins or a request stages.
+int beam_parts(int64_t rows_, int W, int64_t vocab, int dtype, int n) {
   const int64_t A = dtype == VINFER_DTYPE_BF16 ? 8 : 4;
-  const int64_t nv = (vocab + A - 1) / A;
-  int64_t p = (148 * 8 + rows - 1) / rows;
-  p = std::min<int64_t>(p, (nv + 2 * NT - 1) / (2 * NT));
-  p = std::min<int64_t>(p, std::min(MAX_PARTS, std::min(MAX_JOIN / n, MAX_STAGED / (W * n))));
-  return (int)std::max<int64_t>(1, p);
+  const int limit = std::min(MAX_PARTS, std::min(MAX_JOIN / n, MAX_STAGED / (W * n)));
+  return plan_parts(rows_, (vocab + A - 1) / A, NT * U, limit);
 }
 
 size_t pick_smem(int W, int n, int parts) {

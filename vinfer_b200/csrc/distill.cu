@@ -25,7 +25,8 @@ namespace {
 using namespace rows;
 
 constexpr int NT = 256, NW = NT / 32;
-constexpr int U = 8;            // 16-byte vectors a thread holds: 32 KiB a CTA and round
+constexpr int RU = 4;           // 16-byte vectors of a thread and round while summing: 16 KiB a CTA
+constexpr int U = 8;            // ... and while writing the gradient
 constexpr int MAX_PARTS = 64;
 constexpr int MAXK = VINFER_DISTILL_MAX_K;
 static_assert(MAXK <= NT && MAXK <= 128, "one thread an entry; four entries a lane");
@@ -54,9 +55,19 @@ struct DistP {
   float* listg;      // [rows, k]: dloss/dz of the listed elements
   int* status;
   const float* grad_out;
+  int64_t go_stride;
   void* grad;
   int64_t ldg;
 };
+
+// The word of marks that has the bit of vector v, where rounds are of U vectors for each of N threads
+// and a warp's U words of a round lie side by side.
+template <int N, int U>
+__device__ __forceinline__ uint32_t* mark_word(uint4* marks, int v) {
+  static_assert(U == 4, "the words are one 16-byte load");
+  const int c = v / (N * U), u = v % (N * U) / N, w = v % N / 32;
+  return reinterpret_cast<uint32_t*>(marks + c * (N / 32) + w) + u;
+}
 
 // Which elements of vector v are among the n places `at` (a place: element counted from the first
 // vector, -1: none): one bit each. The whole warp calls it with the same v.
@@ -69,9 +80,9 @@ __device__ __forceinline__ uint32_t listed_in(const int* at, int n, int v) {
 }
 
 // The warp's vectors with their listed elements taken out: lane l holds vector v0 + l as q, `word` has
-// the bit of each that holds one. Rarely called, and kept out of the streaming loops' code.
+// the bit of each that holds one.
 template <typename T>
-__device__ __noinline__ uint4 take_out(uint4 q, uint32_t word, const int* at, int n, int v0) {
+__device__ __forceinline__ uint4 take_out(uint4 q, uint32_t word, const int* at, int n, int v0) {
   for (; word; word &= word - 1) {
     const int l = __ffs(word) - 1;
     const uint32_t bits = listed_in<Vec<T>::A>(at, n, v0 + l);
@@ -82,6 +93,12 @@ __device__ __noinline__ uint4 take_out(uint4 q, uint32_t word, const int* at, in
     }
   }
   return q;
+}
+
+// The same out of line, where the loop's code is long and its registers few.
+template <typename T>
+__device__ __noinline__ uint4 take_out_call(uint4 q, uint32_t word, const int* at, int n, int v0) {
+  return take_out<T>(q, word, at, n, v0);
 }
 
 // Stores the gradients of the listed elements of the warp's vectors, each by the lane that has just
@@ -116,42 +133,43 @@ template <typename T>
 __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   using VT = Vec<T>;
   constexpr int A = VT::A;
-  extern __shared__ uint32_t marked[];
+  extern __shared__ uint4 marked[];  // a warp's RU words of a round side by side
   __shared__ float sm[2 * NW];
   __shared__ int hit[MAXK];
   __shared__ int hits;
-  const int64_t row = blockIdx.x / P.parts;
-  const int part = (int)(blockIdx.x - row * P.parts), tid = threadIdx.x;
+  const uint32_t row = blockIdx.x / (uint32_t)P.parts, part = blockIdx.x - row * P.parts;
+  const int tid = threadIdx.x;
   if (P.weights && P.weights[row] == 0.f) return;
   const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
-  const int v0 = (int)((int64_t)R.nv * part / P.parts);
-  const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
+  const int v0 = (int)(R.nv * part / P.parts);  // below 2^18 * 64
+  const int v1 = (int)(R.nv * (part + 1) / P.parts);
   const int id = tid < P.k ? P.ids[row * P.k + tid] : -1;
-  for (int i = tid; i < (v1 - v0 + NT * U - 1) / (NT * U) * (NT * U / 32); i += NT) marked[i] = 0;
+  for (int i = tid; i < (v1 - v0 + NT * RU - 1) / (NT * RU) * NW; i += NT)
+    marked[i] = make_uint4(0, 0, 0, 0);
   if (tid == 0) hits = 0;
   __syncthreads();
   {
     const int e = id + R.off - v0 * A;  // the part's elements, counted from its first vector
     if (id >= 0 && id < P.V && e >= 0 && e < (v1 - v0) * A) {
       hit[atomicAdd(&hits, 1)] = e;
-      atomicOr(&marked[e / A / 32], 1u << (e / A & 31));
+      atomicOr(mark_word<NT, RU>(marked, e / A), 1u << (e / A & 31));
     }
   }
   __syncthreads();
-  float m = neg_inf(), s = 0.f;
-  for (int vb = v0; vb < v1; vb += NT * U) {
-    uint4 q[U];
-    R.template load_round<U, NT>(vb, v1, q);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {  // a warp's 32 vectors are one word (and zeros behind the part)
-      const int first = vb - v0 + u * NT + (tid & ~31);
-      if (const uint32_t word = marked[first / 32])
-        q[u] = take_out<T>(q[u], word, hit, hits, first);
+  Exps sum(P.scale);
+  stream_rounds<RU, NT>(R, v0, v1, [&](uint4 (&q)[RU], int vb) {
+    const uint4 mk = marked[(vb - v0) / (NT * RU) * NW + tid / 32];
+    if (mk.x | mk.y | mk.z | mk.w) {
+      const int f = vb - v0 + (tid & ~31);
+      if (mk.x) q[0] = take_out<T>(q[0], mk.x, hit, hits, f);
+      if (mk.y) q[1] = take_out<T>(q[1], mk.y, hit, hits, f + NT);
+      if (mk.z) q[2] = take_out<T>(q[2], mk.z, hit, hits, f + 2 * NT);
+      if (mk.w) q[3] = take_out<T>(q[3], mk.w, hit, hits, f + 3 * NT);
     }
-    add_exps<T>(q, VT::max(q), P.scale, m, s);
-  }
-  block_join<NW>(m, s, P.scale, sm);
-  if (tid == 0) P.part[blockIdx.x] = Part{m, s};
+    sum.add<T>(q, VT::max(q));
+  });
+  block_join<NW>(sum.m, sum.s, P.scale, sm);
+  if (tid == 0) P.part[blockIdx.x] = Part{sum.m, sum.s};
 }
 
 // A row's list as one warp works on it, four entries a lane.
@@ -368,17 +386,17 @@ template <typename T>
 __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
   using VT = Vec<T>;
   constexpr int A = VT::A;
-  const int64_t row = blockIdx.x / P.parts;
-  const int part = (int)(blockIdx.x - row * P.parts), tid = threadIdx.x;
+  const uint32_t row = blockIdx.x / (uint32_t)P.parts, part = blockIdx.x - row * P.parts;
+  const int tid = threadIdx.x;
   const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
   T* out = static_cast<T*>(P.grad) + row * P.ldg;
   const bool aligned = (int)(((uintptr_t)out & 15) / sizeof(T)) == R.off;
-  const int v0 = (int)((int64_t)R.nv * part / P.parts);
-  const int v1 = (int)((int64_t)R.nv * (part + 1) / P.parts);
+  const int v0 = (int)(R.nv * part / P.parts);  // below 2^18 * 64
+  const int v1 = (int)(R.nv * (part + 1) / P.parts);
   const float weight = P.weights ? P.weights[row] : 1.f;
   grid_dependency_wait();
   const float f =
-      weight == 0.f ? 0.f : weight * P.inv_t * (P.grad_out ? P.grad_out[row] : 1.f);
+      weight == 0.f ? 0.f : weight * P.inv_t * (P.grad_out ? P.grad_out[row * P.go_stride] : 1.f);
   Stat st = {0.f, 0.f};
   if (f != 0.f) st = P.stat[row];
   const float coef = f * st.coef;
@@ -436,13 +454,6 @@ constexpr int SLICE = 14;                 // chunks of a slice at most
 constexpr int MINC = 1, MAXC = 16;        // CTAs of a cluster
 constexpr int LW = 2;                     // warps that solve, and rows under way
 constexpr int STEP_T = CT + 32 + LW * 32;
-
-static_assert(CU == 4, "a warp's marks of a chunk are one 16-byte word");
-// word and bit of vector v of a slice
-__device__ __forceinline__ uint32_t* mark(uint4* marks, int v) {
-  const int c = v / CV, u = v % CV / CT, w = v % CT / 32;
-  return reinterpret_cast<uint32_t*>(marks + c * CW + w) + u;
-}
 
 // What belongs to one row under way. Buffer j serves the live rows i with i % LW == j. It is safe
 // to refill: a CTA sends its sum of row i + 2 after its gradient of row i + 1, which needs every
@@ -591,8 +602,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       if (weight == 0.f) continue;
       if (lane == 0) {
         const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
-        const int v0 = (int)((int64_t)R.nv * rank / size);
-        const int v1 = (int)((int64_t)R.nv * (rank + 1) / size);
+        const int v0 = R.nv * rank / size, v1 = R.nv * (rank + 1) / size;
         const int lo = max(v0, R.off ? 1 : 0), hi = min(v1, (R.V + R.off) / A);  // whole vectors
         const int C = (v1 - v0 + CV - 1) / CV, again = max(C - SLOTS, 0);
         for (int c = 0; c < C + again; ++c, ++it) {
@@ -628,18 +638,17 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       const uint32_t use = live / LW;
       if ((int)(live++ % LW) != mine) continue;
       const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
-      const int v0 = (int)((int64_t)R.nv * rank / size);
-      const int v1 = (int)((int64_t)R.nv * (rank + 1) / size);
+      const int v0 = R.nv * rank / size, v1 = R.nv * (rank + 1) / size;
       list_begin<T>(P, row, B.list);
       if (use > 0 && !bar_wait(&B.list_empty, (use - 1) & 1, dead)) break;
       for (int j = lane; j < P.k; j += 32)
-        if (B.at[j] >= 0) *mark(B.marks, B.at[j] / A) = 0;
+        if (B.at[j] >= 0) *mark_word<CT, CU>(B.marks, B.at[j] / A) = 0;
       __syncwarp();
       for (int j = lane; j < P.k; j += 32) {
         const int id = B.list.id[j], at = id + R.off - v0 * A;
         const bool in = id >= 0 && id < P.V && at >= 0 && at < (v1 - v0) * A;
         B.at[j] = in ? at : -1;
-        if (in) atomicOr(mark(B.marks, at / A), 1u << (at / A & 31));
+        if (in) atomicOr(mark_word<CT, CU>(B.marks, at / A), 1u << (at / A & 31));
       }
       __syncwarp();
       if (lane == 0) bar_arrive(&B.list_full);
@@ -713,14 +722,13 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       }
       const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
       const bool aligned = (int)(((uintptr_t)out & 15) / sizeof(T)) == R.off;
-      const int v0 = (int)((int64_t)R.nv * rank / size);
-      const int v1 = (int)((int64_t)R.nv * (rank + 1) / size);
+      const int v0 = R.nv * rank / size, v1 = R.nv * (rank + 1) / size;
       const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;
       const int C = (v1 - v0 + CV - 1) / CV, again = max(C - SLOTS, 0);
       StepRow& B = S.row[live % LW];
       const uint32_t use = live++ / LW;
       if (!(ok = bar_wait(&B.list_full, use & 1, dead))) break;
-      float m = neg_inf(), s = 0.f;
+      Exps sum(P.scale);
       for (int c = 0; c < C; ++c, ++it) {
         if (!(ok = bar_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead))) break;
         const int v = v0 + c * CV;
@@ -733,14 +741,16 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
         const uint4 mk = B.marks[c * CW + w];
         if (mk.x | mk.y | mk.z | mk.w) {
           const int f = c * CV + w * 32;
-          if (mk.x) q[0] = take_out<T>(q[0], mk.x, B.at, P.k, f);
-          if (mk.y) q[1] = take_out<T>(q[1], mk.y, B.at, P.k, f + CT);
-          if (mk.z) q[2] = take_out<T>(q[2], mk.z, B.at, P.k, f + 2 * CT);
-          if (mk.w) q[3] = take_out<T>(q[3], mk.w, B.at, P.k, f + 3 * CT);
+          if (mk.x) q[0] = take_out_call<T>(q[0], mk.x, B.at, P.k, f);
+          if (mk.y) q[1] = take_out_call<T>(q[1], mk.y, B.at, P.k, f + CT);
+          if (mk.z) q[2] = take_out_call<T>(q[2], mk.z, B.at, P.k, f + 2 * CT);
+          if (mk.w) q[3] = take_out_call<T>(q[3], mk.w, B.at, P.k, f + 3 * CT);
         }
-        add_exps<T>(q, VT::max(q), P.scale, m, s);
+        sum.add<T>(q, VT::max(q));
       }
       if (!ok) break;
+      float m = sum.m;
+      const float s = sum.s;
       if (s == 0.f) m = neg_inf();
       const float mw = warp_max(m);
       float sw = s == 0.f ? 0.f : s * ex2((m - mw) * P.scale);
@@ -800,14 +810,9 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
   if (size > 1) cluster_sync();  // no sum is sent to a CTA that has left
 }
 
-// Parts of a row: enough CTAs to fill the 148 SMs several times over, at least two vectors a
-// thread in each.
 int distill_parts(int64_t rows_, int64_t vocab, int dtype) {
   const int64_t A = dtype == VINFER_DTYPE_BF16 ? 8 : 4;
-  const int64_t nv = (vocab + A - 1) / A;
-  int64_t p = (148 * 8 + rows_ - 1) / rows_;
-  p = std::min<int64_t>(p, (nv + 2 * NT - 1) / (2 * NT));
-  return (int)std::max<int64_t>(1, std::min<int64_t>(p, MAX_PARTS));
+  return plan_parts(rows_, (vocab + A - 1) / A, NT * RU, MAX_PARTS);
 }
 
 int check(const VinferDistillArgs* a) {
@@ -843,7 +848,7 @@ DistP params(const VinferDistillArgs* a) {
 template <typename T>
 int launch_loss(const DistP& P, cudaStream_t st) {
   const int part_vecs = (P.V / Vec<T>::A + 2 + P.parts - 1) / P.parts + 1;
-  const size_t smem = (size_t)(part_vecs + NT * U - 1) / (NT * U) * (NT * U / 8);
+  const size_t smem = (size_t)(part_vecs + NT * RU - 1) / (NT * RU) * (NT * RU / 8);
   const int rc = launch(k_distill_rows<T>, (unsigned)(P.rows * P.parts), NT, smem, st, false, 1, P);
   if (rc != VINFER_OK) return rc;
   return launch(k_distill_finish<T>, (unsigned)((P.rows + FW - 1) / FW), FW * 32, 0, st, true, 1, P);
@@ -957,17 +962,19 @@ int vinfer_distill_loss(const VinferDistillArgs* a, float* loss, float* row_stat
 }
 
 int vinfer_distill_grad(const VinferDistillArgs* a, const float* row_stats,
-                        const float* list_grads, const float* grad_out, void* grad,
-                        int64_t ld_grad, void* stream) {
+                        const float* list_grads, const float* grad_out, int64_t grad_out_stride,
+                        void* grad, int64_t ld_grad, void* stream) {
   NvtxRange nvtx_range("vinfer_distill_grad");
   const int rc = check(a);
   if (rc != VINFER_OK) return rc;
-  if (!row_stats || !list_grads || !grad_ok(a, grad, ld_grad)) return VINFER_E_ARG;
+  if (!row_stats || !list_grads || grad_out_stride < 0 || !grad_ok(a, grad, ld_grad))
+    return VINFER_E_ARG;
   if (((uintptr_t)row_stats) % 8) return VINFER_E_ARG;
   DistP P = params(a);
   P.stat = reinterpret_cast<Stat*>(const_cast<float*>(row_stats));
   P.listg = const_cast<float*>(list_grads);
   P.grad_out = grad_out;
+  P.go_stride = grad_out_stride;
   P.grad = grad;
   P.ldg = ld_grad;
   cudaStream_t st = (cudaStream_t)stream;

@@ -19,6 +19,9 @@ constexpr float L2E = 1.4426950408889634f;      // log2(e) rounded to float
 constexpr double L2E_D = 1.4426950408889634074;  // log2(e)
 constexpr double LN2_D = 0.69314718055994530942;
 
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return (uint32_t)__cvta_generic_to_shared(p);
+}
 __device__ __forceinline__ float neg_inf() { return __int_as_float(0xff800000); }
 
 // 2^x by the hardware's approximation (2 ulp; 0 below the normal range)
@@ -260,6 +263,23 @@ struct Row {
   }
 };
 
+// Streams vectors [v0, v1) of a row through work(q, first vector) in rounds of U a thread, each round
+// loaded while the one before it is worked on. v0 < v1.
+template <int U, int NT, typename T, typename F>
+__device__ __forceinline__ void stream_rounds(const Row<T>& R, int v0, int v1, F&& work) {
+  uint4 a[U], b[U];
+  R.template load_round<U, NT>(v0, v1, a);
+  for (int v = v0;; v += 2 * NT * U) {
+    const int v2 = v + NT * U, v3 = v2 + NT * U;
+    if (v2 < v1) R.template load_round<U, NT>(v2, v1, b);
+    work(a, v);
+    if (v2 >= v1) break;
+    if (v3 < v1) R.template load_round<U, NT>(v3, v1, a);
+    work(b, v2);
+    if (v3 >= v1) break;
+  }
+}
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(FULL, v, o));
@@ -271,54 +291,62 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// Softmax sums are held as (m, s): s in units of 2^(m * scale), m the largest logit summed, scale =
+// Softmax sums are held as (m, s): s in units of 2^(m * scale), m a logit of those summed, scale =
 // log2(e) / temperature rounded to float. m stays a logit, so sums of rows at the type's lowest
 // value (a mask) need no exponent beyond the float's range, and the rounding of `scale` only
-// stretches distances from the maximum.
-
-// Adds the U vectors q, whose largest element is mx, to the thread's sum: an ex2 an element, and a
-// multiply-add and an addition for each two. The argument x * scale - c is rounded once, and
-// what c misses of m * scale is put right in the round's sum.
-template <typename T, int U>
-__device__ __forceinline__ void add_exps(const uint4 (&q)[U], float mx, float scale, float& m,
-                                         float& s) {
-  constexpr int H = Vec<T>::A / 2;
-  if (mx > m) {
-    if (s != 0.f) s *= ex2((m - mx) * scale);
-    m = mx;
-  }
-  const float ref = m == neg_inf() ? 0.f : m;  // only -inf so far (or NaN, which the sum shows)
-  const float c = ref * scale;
-  float sum = 0.f;
-  if (fabsf(c) < 1e37f) {
-    const uint64_t k = pair(scale, scale), d = pair(-c, -c);
-    uint64_t all = pair(0.f, 0.f);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      uint64_t f[H];
-      Vec<T>::pairs(q[u], f);
-      uint64_t t = ex2_2(fma2(f[0], k, d));
-#pragma unroll
-      for (int j = 1; j < H; ++j) t = add2(t, ex2_2(fma2(f[j], k, d)));
-      all = add2(all, t);
+// stretches distances from m.
+//
+// A thread's sum while it streams: m is the largest element of its first round, and moves only when a
+// later one counts 16 times as much, so that exponents stay small and few rounds rescale: a
+// round costs an ex2 an element, and a multiply-add and an addition for each two. The argument
+// x * scale - c is rounded once, and what c misses of m * scale is put right in the round's sum.
+struct Exps {
+  float m, s;
+  float c, fix;  // m * scale rounded, and what that does to a round's sum
+  float scale;
+  __device__ __forceinline__ explicit Exps(float scale_)
+      : m(neg_inf()), s(0.f), c(0.f), fix(0.f), scale(scale_) {}
+  // the thread's vectors q, whose largest element is mx
+  template <typename T, int U>
+  __device__ __forceinline__ void add(const uint4 (&q)[U], float mx) {
+    constexpr int H = Vec<T>::A / 2;
+    if ((mx - m) * scale > 4.f) {  // the first round (m is -inf) and seldom again
+      if (s != 0.f) s *= ex2((m - mx) * scale);
+      m = mx;
+      c = m * scale;
+      fix = -fmaf(m, scale, -c) * (float)LN2_D;
     }
-    float a, b;
-    split(all, a, b);
-    sum = a + b;
-    const float lo = fmaf(ref, scale, -c);
-    sum = fmaf(sum, -lo * (float)LN2_D, sum);
-  } else {  // c near the float's range, or infinite: distances first
+    float sum;
+    if (fabsf(c) < 1e37f) {
+      const uint64_t k = pair(scale, scale), d = pair(-c, -c);
+      uint64_t all = pair(0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        uint64_t f[H];
+        Vec<T>::pairs(q[u], f);
+        uint64_t t = ex2_2(fma2(f[0], k, d));
+#pragma unroll
+        for (int j = 1; j < H; ++j) t = add2(t, ex2_2(fma2(f[j], k, d)));
+        all = add2(all, t);
+      }
+      float a, b;
+      split(all, a, b);
+      sum = a + b;
+      sum = fmaf(sum, fix, sum);
+    } else {  // c near the float's range, or infinite: distances first
+      sum = 0.f;
 #pragma unroll 1
-    for (int u = 0; u < U; ++u) {
-      uint4 v = q[0];
+      for (int u = 0; u < U; ++u) {
+        uint4 v = q[0];
 #pragma unroll
-      for (int i = 1; i < U; ++i)
-        if (i == u) v = q[i];
-      for (int j = 0; j < Vec<T>::A; ++j) sum += ex2((Vec<T>::get(v, j) - ref) * scale);
+        for (int i = 1; i < U; ++i)
+          if (i == u) v = q[i];
+        for (int j = 0; j < Vec<T>::A; ++j) sum += ex2((Vec<T>::get(v, j) - m) * scale);
+      }
     }
+    s += sum;
   }
-  s += sum;
-}
+};
 
 // Joins the sums of a block's threads: every thread gets the block's. Fixed order: the result does
 // not depend on timing. `sm`: 2 * NW floats.
@@ -347,9 +375,6 @@ __device__ __forceinline__ void block_join(float& m, float& s, float scale, floa
 }
 
 // ---- barriers in shared memory and bulk copies ----
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-  return (uint32_t)__cvta_generic_to_shared(p);
-}
 __device__ __forceinline__ void bar_init(uint64_t* b, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(b)), "r"(count) : "memory");
 }
@@ -458,6 +483,26 @@ struct NvtxRange {
   NvtxRange(const NvtxRange&) = delete;
   NvtxRange& operator=(const NvtxRange&) = delete;
 };
+
+// Parts of each row for kernels of 4 CTAs an SM that stream parts in rounds of `round` vectors: the
+// fewest waves of CTAs times the rounds of one, where beginning and ending a part costs about as
+// much as START rounds. Measured (us a beam step): 256 rows of 151,936 bf16 32.3 / 29.7 / 32.3 /
+// 31.9 with 1 / 2 / 3 / 4 parts (2 taken), 512 rows of 248,320 float32 107 / 117 / 124 with 1 / 2 / 3
+// (1 taken).
+inline int plan_parts(int64_t rows, int64_t nv, int round, int limit) {
+  constexpr int64_t SLOTS = 148 * 4, START = 2;
+  int best = 1;
+  int64_t least = INT64_MAX;
+  for (int p = 1; p <= limit && (p - 1) * (int64_t)round < nv; ++p) {
+    const int64_t cost =
+        (rows * p + SLOTS - 1) / SLOTS * ((nv + (int64_t)p * round - 1) / ((int64_t)p * round) + START);
+    if (cost < least) {
+      least = cost;
+      best = p;
+    }
+  }
+  return best;
+}
 
 // An error code for the caller; the runtime's own error state is cleared, so that a refused launch
 // does not show up in somebody else's check.

@@ -26,19 +26,19 @@ if TYPE_CHECKING:
 class _ListLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, backend, ids, logprobs, weights, temperature, tail):
-        loss, stats, lists = backend.distill_loss(
+        loss, saved = backend.distill_loss(
             logits, ids, logprobs, weights, temperature=temperature, tail=tail,
             for_grad=ctx.needs_input_grad[0])
-        ctx.save_for_backward(logits, ids, logprobs, weights, stats, lists)
+        ctx.save_for_backward(logits, ids, logprobs, weights, saved)
         ctx.backend, ctx.temperature, ctx.tail = backend, temperature, tail
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_out):
-        logits, ids, logprobs, weights, stats, lists = ctx.saved_tensors
+        logits, ids, logprobs, weights, saved = ctx.saved_tensors
         grad = ctx.backend.distill_grad(
-            logits, ids, logprobs, weights, stats, lists, grad_out.float().contiguous(),
+            logits, ids, logprobs, weights, saved, grad_out,
             temperature=ctx.temperature, tail=ctx.tail)
         return grad, None, None, None, None, None, None
 

@@ -75,7 +75,7 @@ class B200Sampler:
         return ws
 
     def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
 
     # ---- argument packing ----------------------------------------------------------------------
     def args(self, logits: torch.Tensor, params: RowParams, uniforms: torch.Tensor | None,
@@ -353,37 +353,45 @@ class B200Sampler:
     def distill_loss(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
                      weights: torch.Tensor | None = None, *, temperature: float = 1.0,
                      tail: bool = False, for_grad: bool = False
-                     ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+                     ) -> tuple[torch.Tensor, torch.Tensor | None]:
         """The rows' distillation losses (float32 ``[rows]``), and with ``for_grad`` what
-        ``distill_grad`` needs (row statistics ``[rows, 2]``, the list's gradients
-        ``[rows, k]``). ``vinfer_b200.distill.distillation_loss`` is the differentiable form."""
+        ``distill_grad`` needs of them (float32 ``[rows * (2 + k)]``).
+        ``vinfer_b200.distill.distillation_loss`` is the differentiable form."""
         a = self._distill_args(logits, ids, logprobs, weights, temperature, tail)
-        loss = torch.empty(a.rows, dtype=torch.float32, device=self.device)
-        stats = lists = None
+        n, k = a.rows, a.k
+        loss = torch.empty(n, dtype=torch.float32, device=self.device)
+        saved = stats = lists = None
         if for_grad:
-            stats = torch.empty(a.rows, 2, dtype=torch.float32, device=self.device)
-            lists = torch.empty(a.rows, a.k, dtype=torch.float32, device=self.device)
-        if a.rows:
-            nbytes = self.lib.vinfer_distill_workspace_bytes(a.rows, a.vocab, a.dtype, a.k)
+            saved = torch.empty(n * (2 + k), dtype=torch.float32, device=self.device)
+            stats = saved.data_ptr()
+            lists = stats + 8 * n
+        if n:
+            nbytes = self.lib.vinfer_distill_workspace_bytes(n, a.vocab, a.dtype, k)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             self._call(self.lib.vinfer_distill_loss, "vinfer_distill_loss", C.byref(a),
-                       loss.data_ptr(), _ptr(stats), _ptr(lists), ws.data_ptr(), nbytes)
-        return loss, stats, lists
+                       loss.data_ptr(), stats, lists, ws.data_ptr(), nbytes)
+        return loss, saved
 
     def distill_grad(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
-                     weights: torch.Tensor | None, stats: torch.Tensor, lists: torch.Tensor,
+                     weights: torch.Tensor | None, saved: torch.Tensor,
                      grad_out: torch.Tensor | None = None, *, temperature: float = 1.0,
                      tail: bool = False) -> torch.Tensor:
         """The gradient of ``sum(grad_out * loss)`` with respect to the logits, of their type
-        (``grad_out``: float32 ``[rows]``, None for ones)."""
+        (``grad_out``: float32 ``[rows]`` of any stride, None for ones), from what
+        ``distill_loss`` saved for the same arguments."""
         a = self._distill_args(logits, ids, logprobs, weights, temperature, tail)
-        sp = self._vector("stats", stats, torch.float32, a.rows, 2)
-        lp = self._vector("lists", lists, torch.float32, a.rows, a.k)
-        gp = None if grad_out is None else self._vector("grad_out", grad_out, torch.float32, a.rows)
+        stats = self._vector("saved", saved, torch.float32, a.rows * (2 + a.k))
+        gp, step = None, 0
+        if grad_out is not None:
+            if grad_out.shape != (a.rows,) or grad_out.dtype != torch.float32 or \
+                    grad_out.device != self.device:
+                raise ValueError(f"grad_out must be float32 [{a.rows}] on {self.device}")
+            gp, step = grad_out.data_ptr(), grad_out.stride(0)
         grad = self._grad_like(logits, a.ld)
         if a.rows:
-            self._call(self.lib.vinfer_distill_grad, "vinfer_distill_grad", C.byref(a), sp, lp, gp,
-                       grad.data_ptr(), grad.stride(0) if a.rows > 1 else a.vocab)
+            self._call(self.lib.vinfer_distill_grad, "vinfer_distill_grad", C.byref(a), stats,
+                       stats + 8 * a.rows, gp, step, grad.data_ptr(),
+                       grad.stride(0) if a.rows > 1 else a.vocab)
         return grad
 
     def distill_step(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
