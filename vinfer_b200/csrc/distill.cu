@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
     }
     sum.add<T>(q, VT::max(q));
   });
+  grid_dependents_may_start();
   block_join<NW>(sum.m, sum.s, P.scale, sm);
   if (tid == 0) P.part[blockIdx.x] = Part{sum.m, sum.s};
 }

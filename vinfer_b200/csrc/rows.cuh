@@ -472,6 +472,10 @@ __device__ __forceinline__ void send(void* dst, uint64_t* bar, uint32_t rank, ui
                : "memory");
 }
 
+// The dependent kernel may take its place on the SMs now; it still waits for this grid's end.
+__device__ __forceinline__ void grid_dependents_may_start() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 __device__ __forceinline__ void grid_dependency_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }

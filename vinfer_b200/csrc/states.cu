@@ -50,17 +50,17 @@ struct StatesP {
   int* status;
 };
 
-// One item: NT * UV vectors of slot `from` to slot `to`. 32-bit index arithmetic, and divisions only
-// where runs are shorter than an item or lie under several outer dimensions.
+// One item: NT * UV vectors of slot `from` to slot `to`, counted over the live part of its runs (`rv`
+// vectors each). 32-bit index arithmetic, and divisions only where runs are shorter than an item or
+// lie under several outer dimensions.
 template <typename VT>
-__device__ __forceinline__ void copy_item(const Desc& D, int from, int to, uint32_t chunk, int len) {
+__device__ __forceinline__ void copy_item(const Desc& D, int from, int to, uint32_t chunk,
+                                          uint32_t rv, uint32_t vecs, int len) {
   constexpr uint32_t SPAN = NT * UV;
   const unsigned char* src = D.src + (int64_t)from * D.src_slot;
   unsigned char* dst = D.dst + (int64_t)to * D.dst_slot;
-  const uint32_t rv = D.run_vecs, i0 = chunk * SPAN;
+  const uint32_t i0 = chunk * SPAN;
   const uint32_t o0 = D.n_outer ? i0 / rv : 0, r0 = i0 - o0 * rv;
-  const uint32_t end = D.unit_vecs ? (uint32_t)len * D.unit_vecs : rv;  // live vectors of a run
-  if (r0 >= end && r0 + SPAN <= rv) return;
   VT v[UV];
   int64_t at[UV];
 #pragma unroll
@@ -72,7 +72,7 @@ __device__ __forceinline__ void copy_item(const Desc& D, int from, int to, uint3
       o += q;
       r -= q * rv;
     }
-    bool live = i0 + step < D.vecs && r < end;
+    bool live = i0 + step < vecs;
     int64_t so = (int64_t)r * sizeof(VT), po = so;
     for (int k = OUTER - 1; k >= OUTER - D.n_outer; --k) {
       uint32_t x = o;
@@ -92,9 +92,11 @@ __device__ __forceinline__ void copy_item(const Desc& D, int from, int to, uint3
     if (at[u] >= 0) *reinterpret_cast<VT*>(dst + at[u]) = v[u];
 }
 
-// Dynamic shared memory: one packed move (source << 16 | slot) a slot.
+// Dynamic shared memory: for every slot a packed move (source << 16 | slot) and the items of the
+// moves before it.
 __global__ void __launch_bounds__(NT, CTAS) k_reorder(const __grid_constant__ StatesP P) {
   extern __shared__ uint32_t moves[];
+  uint32_t* before = moves + P.slots;  // [M + 1]
   __shared__ int wcnt[NT / 32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   uint32_t M = 0;  // the slots that move, ascending: every CTA makes the same list
@@ -119,22 +121,69 @@ __global__ void __launch_bounds__(NT, CTAS) k_reorder(const __grid_constant__ St
     if (move) moves[at] = (uint32_t)p << 16 | (uint32_t)s;
     __syncthreads();
   }
-  // items: the moves of a chunk side by side, chunk after chunk, tensor after tensor
-  uint32_t g = blockIdx.x;
+  // items: whole states chunk by chunk with the moves of a chunk side by side; states cut by lengths
+  // move by move, the live part alone; tensor after tensor
+  auto live_vecs = [&](const Desc& D, uint32_t mv) {  // of one run
+    return (uint32_t)min(max(P.lengths[mv & 0xffff], 0), D.len_max) * D.unit_vecs;
+  };
+  uint32_t g = blockIdx.x, unit = 0, run = 0, vecs = 0;  // of the tensor that `before` counts
   for (int t = 0; t < P.n; ++t) {
     const Desc& D = P.d[t];
-    const uint32_t items = D.chunks * M;
+    const bool cut = D.unit_vecs != 0;
+    if (cut && (D.unit_vecs != unit || D.run_vecs != run || D.vecs != vecs)) {
+      unit = D.unit_vecs;
+      run = D.run_vecs;
+      vecs = D.vecs;
+      uint32_t sum = 0;
+      for (uint32_t i0 = 0; i0 < M; i0 += NT) {
+        const uint32_t i = i0 + threadIdx.x;
+        const uint32_t mine =
+            i < M ? (vecs / run * live_vecs(D, moves[i]) + NT * UV - 1) / (NT * UV) : 0;
+        uint32_t incl = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+          const uint32_t up = __shfl_up_sync(FULL, incl, o);
+          if (lane >= o) incl += up;
+        }
+        __syncthreads();  // wcnt and `before` were read by all
+        if (lane == 31) wcnt[w] = incl;
+        __syncthreads();
+        uint32_t at = sum + incl - mine;
+        for (int k = 0; k < NT / 32; ++k) {
+          if (k < w) at += wcnt[k];
+          sum += wcnt[k];
+        }
+        if (i < M) before[i] = at;
+      }
+      if (threadIdx.x == 0) before[M] = sum;
+      __syncthreads();
+    }
+    const uint32_t items = cut ? before[M] : D.chunks * M;
     for (; g < items; g += gridDim.x) {
-      const uint32_t chunk = g / M, mv = moves[g - chunk * M];
+      uint32_t chunk, i;
+      if (cut) {  // the last move that begins at or before g
+        uint32_t lo = 0, hi = M;
+        while (hi - lo > 1) {
+          const uint32_t mid = (lo + hi) / 2;
+          if (before[mid] <= g) lo = mid;
+          else hi = mid;
+        }
+        i = lo;
+        chunk = g - before[i];
+      } else {
+        chunk = g / M;
+        i = g - chunk * M;
+      }
+      const uint32_t mv = moves[i];
       const int from = mv >> 16, to = mv & 0xffff;
-      int len = 0;
-      if (D.unit_vecs || D.len_outer >= 0) len = min(max(P.lengths[to], 0), D.len_max);
+      const int len = D.len_outer >= 0 ? min(max(P.lengths[to], 0), D.len_max) : 0;
+      const uint32_t rv = cut ? live_vecs(D, mv) : D.run_vecs;
+      const uint32_t n = cut ? D.vecs / D.run_vecs * rv : D.vecs;
       switch (D.vec) {
-        case 16: copy_item<uint4>(D, from, to, chunk, len); break;
-        case 8: copy_item<uint2>(D, from, to, chunk, len); break;
-        case 4: copy_item<uint32_t>(D, from, to, chunk, len); break;
-        case 2: copy_item<uint16_t>(D, from, to, chunk, len); break;
-        default: copy_item<uint8_t>(D, from, to, chunk, len); break;
+        case 16: copy_item<uint4>(D, from, to, chunk, rv, n, len); break;
+        case 8: copy_item<uint2>(D, from, to, chunk, rv, n, len); break;
+        case 4: copy_item<uint32_t>(D, from, to, chunk, rv, n, len); break;
+        case 2: copy_item<uint16_t>(D, from, to, chunk, rv, n, len); break;
+        default: copy_item<uint8_t>(D, from, to, chunk, rv, n, len); break;
       }
     }
     g -= items;
@@ -220,7 +269,7 @@ extern "C" int vinfer_reorder_states(const VinferState* states, int32_t n_states
     }
     // every slot may move: no more CTAs than items, at most what is resident
     const int64_t grid = std::min<int64_t>(148 * CTAS, chunks * slots);
-    const size_t smem = (size_t)slots * 4;
+    const size_t smem = (size_t)slots * 8 + 4;
     if (opt_in(k_reorder, smem) != VINFER_OK) return VINFER_E_CUDA;
     const int rc = launch(k_reorder, (unsigned)grid, NT, smem, (cudaStream_t)stream, false, 1, P);
     if (rc != VINFER_OK) return rc;
