@@ -64,9 +64,35 @@ struct DistP {
 // and a warp's U words of a round lie side by side.
 template <int N, int U>
 __device__ __forceinline__ uint32_t* mark_word(uint4* marks, int v) {
-  static_assert(U == 4, "the words are one 16-byte load");
+  static_assert(U % 4 == 0, "a warp's words are 16-byte loads");
   const int c = v / (N * U), u = v % (N * U) / N, w = v % N / 32;
-  return reinterpret_cast<uint32_t*>(marks + c * (N / 32) + w) + u;
+  return reinterpret_cast<uint32_t*>(marks) + (c * (N / 32) + w) * U + u;
+}
+// A warp's words of round c; whether any has a bit.
+template <int N, int U>
+__device__ __forceinline__ bool marks_of(const uint4* marks, int c, int w, uint32_t (&word)[U]) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < U / 4; ++i) {
+    const uint4 m = marks[(c * (N / 32) + w) * (U / 4) + i];
+    word[4 * i] = m.x;
+    word[4 * i + 1] = m.y;
+    word[4 * i + 2] = m.z;
+    word[4 * i + 3] = m.w;
+    any |= m.x | m.y | m.z | m.w;
+  }
+  return any != 0;
+}
+
+template <int N, int U>
+__device__ __forceinline__ bool has_marks(const uint4* marks, int c, int w) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < U / 4; ++i) {
+    const uint4 m = marks[(c * (N / 32) + w) * (U / 4) + i];
+    any |= m.x | m.y | m.z | m.w;
+  }
+  return any != 0;
 }
 
 // Which elements of vector v are among the n places `at` (a place: element counted from the first
@@ -93,12 +119,6 @@ __device__ __forceinline__ uint4 take_out(uint4 q, uint32_t word, const int* at,
     }
   }
   return q;
-}
-
-// The same out of line, where the loop's code is long and its registers few.
-template <typename T>
-__device__ __noinline__ uint4 take_out_call(uint4 q, uint32_t word, const int* at, int n, int v0) {
-  return take_out<T>(q, word, at, n, v0);
 }
 
 // Stores the gradients of the listed elements of the warp's vectors, each by the lane that has just
@@ -158,13 +178,12 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   __syncthreads();
   Exps sum(P.scale);
   stream_rounds<RU, NT>(R, v0, v1, [&](uint4 (&q)[RU], int vb) {
-    const uint4 mk = marked[(vb - v0) / (NT * RU) * NW + tid / 32];
-    if (mk.x | mk.y | mk.z | mk.w) {
-      const int f = vb - v0 + (tid & ~31);
-      if (mk.x) q[0] = take_out<T>(q[0], mk.x, hit, hits, f);
-      if (mk.y) q[1] = take_out<T>(q[1], mk.y, hit, hits, f + NT);
-      if (mk.z) q[2] = take_out<T>(q[2], mk.z, hit, hits, f + 2 * NT);
-      if (mk.w) q[3] = take_out<T>(q[3], mk.w, hit, hits, f + 3 * NT);
+    uint32_t word[RU];
+    if (marks_of<NT, RU>(marked, (vb - v0) / (NT * RU), tid / 32, word)) {
+#pragma unroll
+      for (int u = 0; u < RU; ++u)
+        if (word[u])
+          q[u] = take_out<T>(q[u], word[u], hit, hits, vb - v0 + u * NT + (tid & ~31));
     }
     sum.add<T>(q, VT::max(q));
   });
@@ -447,11 +466,11 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
 // ahead, joins the CTA's sum with the other CTAs' (each sends its own to all), and hands out the
 // gradient's terms. Two CTAs an SM, so that one streams while the other solves.
 constexpr int STEP_CTAS = 2;              // CTAs of an SM
-constexpr int CW = 11, CT = CW * 32;      // warps and threads that sum and write
+constexpr int CW = 12, CT = CW * 32;      // warps and threads that sum and write
 constexpr int CU = 4;                     // vectors a thread takes of a chunk
-constexpr int CV = CT * CU;               // vectors of a chunk: 22 KiB
+constexpr int CV = CT * CU;               // vectors of a chunk: 24 KiB
 constexpr int SLOTS = 4;                  // chunks of the ring
-constexpr int SLICE = 14;                 // chunks of a slice at most
+constexpr int SLICE = 13;                 // chunks of a slice at most
 constexpr int MINC = 1, MAXC = 16;        // CTAs of a cluster
 constexpr int LW = 2;                     // warps that solve, and rows under way
 constexpr int STEP_T = CT + 32 + LW * 32;
@@ -470,7 +489,7 @@ struct StepRow {
   float m, coef;
   float listg[MAXK];
   int at[MAXK];                    // places of the listed elements in the slice, -1: not in it
-  uint4 marks[SLICE * CW];         // a bit for each vector that holds one: a warp's CU of a chunk
+  uint4 marks[SLICE * CW * CU / 4]; // a bit for each vector that holds one: a warp's CU of a chunk
   ListS list;
 };
 constexpr int ROWQ = 4;            // rows handed out ahead, the next two of them before they are loaded
@@ -525,6 +544,66 @@ struct RowWalk {
   }
 };
 
+// What a warp needs of a chunk besides its place in the ring; the calls below are rare, and out of line
+// so that the streaming loops keep their registers.
+template <typename T>
+struct Chunk {
+  const T* p;      // the row
+  int V, off, v;   // its length, its offset from an aligned address, the chunk's first vector
+  int v0, v1;      // the slice
+};
+
+// Makes the warp's vectors of a chunk in the ring what the loops take them for: the row's ragged ends
+// filled from memory, -inf behind the slice and, with `marks`, in the place of listed elements.
+template <typename T>
+__device__ __noinline__ void mend_chunk(uint4* chunk, Chunk<T> K, const uint4* marks,
+                                        const int* at, int n) {
+  constexpr int A = Vec<T>::A;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int lo = K.off ? 1 : 0, hi = min(K.v1, (K.V + K.off) / A);
+  for (int u = 0; u < CU; ++u) {
+    const int x = K.v + u * CT + tid;
+    if (x < lo || x >= hi)
+      chunk[u * CT + tid] = Row<T>::edge(K.p, x < K.v1 ? K.V : 0, x * A - K.off);
+  }
+  __syncwarp();
+  if (marks) {
+    const int c = (K.v - K.v0) / CV;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(marks) + (c * CW + w) * CU;
+    for (int u = 0; u < CU; ++u)
+      for (uint32_t word = words[u]; word; word &= word - 1) {
+        const int l = __ffs(word) - 1;
+        const uint32_t bits = listed_in<A>(at, n, c * CV + u * CT + w * 32 + l);
+        if (lane == l) {
+          uint4 q = chunk[u * CT + tid];
+          for (int j = 0; j < A; ++j)
+            if (bits >> j & 1) Vec<T>::put(q, j, Vec<T>::NEG_INF_BITS);
+          chunk[u * CT + tid] = q;
+        }
+      }
+  }
+  // these writes before the copy that refills the chunk
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+
+// The gradient of a chunk that cannot be stored by whole vectors.
+template <typename T>
+__device__ __noinline__ void put_chunk(const uint4* chunk, Chunk<T> K, T* out, float m, float scale,
+                                       float coef) {
+  constexpr int A = Vec<T>::A;
+  for (int u = 0; u < CU; ++u) {
+    const int x = K.v + u * CT + (int)threadIdx.x;
+    if (x >= K.v1) continue;
+    const uint4 q = chunk[u * CT + threadIdx.x];
+    for (int j = 0; j < A; ++j) {
+      const int e = x * A - K.off + j;
+      if (e >= 0 && e < K.V)
+        out[e] = Vec<T>::round(coef * ex2((Vec<T>::get(q, j) - m) * scale));
+    }
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid_constant__ DistP P) {
   using VT = Vec<T>;
@@ -555,7 +634,8 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
   }
   for (int j = w; j < LW; j += STEP_T / 32) {
     for (int i = lane; i < MAXK; i += 32) S.row[j].at[i] = -1;
-    for (int i = lane; i < SLICE * CW; i += 32) S.row[j].marks[i] = make_uint4(0, 0, 0, 0);
+    for (int i = lane; i < SLICE * CW * CU / 4; i += 32)
+      S.row[j].marks[i] = make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
   if (size > 1) cluster_sync();  // every CTA's barriers are ready for the others' sums
@@ -690,23 +770,6 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
     if (lane == 0 && *dead && P.status) atomicOr(P.status, (int)VINFER_ST_INTERNAL);
   } else {  // ---- the warps that sum and write
     const uint64_t scale2 = pair(P.scale, P.scale);
-    // the thread's vectors of the chunk that begins at v: in the ring, at the row's ragged ends (or
-    // behind the slice) from memory
-    auto take = [&](const Row<T>& R, int v, int v1, bool inside, uint32_t n, uint4 (&q)[CU]) {
-      const uint4* src = ring + (size_t)(n % SLOTS) * CV + tid;
-#pragma unroll
-      for (int u = 0; u < CU; ++u) q[u] = src[u * CT];
-      if (!inside) {
-        const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;
-#pragma unroll
-        for (int u = 0; u < CU; ++u) {
-          const int x = v + u * CT + tid;
-          if (x < lo || x >= min(hi, v1))
-            q[u] = R.edge(R.p, x < v1 ? R.V : 0, x * A - R.off);  // all -inf behind the slice
-        }
-      }
-    };
-
     uint32_t it = 0, live = 0;  // chunks and rows so far
     bool ok = true;
     while (ok && next_row(row, weight)) {
@@ -724,7 +787,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
       const bool aligned = (int)(((uintptr_t)out & 15) / sizeof(T)) == R.off;
       const int v0 = R.nv * rank / size, v1 = R.nv * (rank + 1) / size;
-      const int lo = R.off ? 1 : 0, hi = (R.V + R.off) / A;
+      const int lo = R.off ? 1 : 0, end = min(v1, (R.V + R.off) / A);
       const int C = (v1 - v0 + CV - 1) / CV, again = max(C - SLOTS, 0);
       StepRow& B = S.row[live % LW];
       const uint32_t use = live++ / LW;
@@ -733,19 +796,15 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       for (int c = 0; c < C; ++c, ++it) {
         if (!(ok = bar_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead))) break;
         const int v = v0 + c * CV;
+        uint4* chunk = ring + (size_t)(it % SLOTS) * CV;
+        if (!(v >= lo && v + CV <= end) || has_marks<CT, CU>(B.marks, c, w))
+          mend_chunk<T>(chunk, Chunk<T>{R.p, R.V, R.off, v, v0, v1}, B.marks, B.at, P.k);
         uint4 q[CU];
-        take(R, v, v1, v >= lo && v + CV <= min(hi, v1), it, q);
+#pragma unroll
+        for (int u = 0; u < CU; ++u) q[u] = chunk[u * CT + tid];
         if (c < again) {  // not held for the gradient
           __syncwarp();
           if (lane == 0) bar_arrive(&S.empty[it % SLOTS]);
-        }
-        const uint4 mk = B.marks[c * CW + w];
-        if (mk.x | mk.y | mk.z | mk.w) {
-          const int f = c * CV + w * 32;
-          if (mk.x) q[0] = take_out_call<T>(q[0], mk.x, B.at, P.k, f);
-          if (mk.y) q[1] = take_out_call<T>(q[1], mk.y, B.at, P.k, f + CT);
-          if (mk.z) q[2] = take_out_call<T>(q[2], mk.z, B.at, P.k, f + 2 * CT);
-          if (mk.w) q[3] = take_out_call<T>(q[3], mk.w, B.at, P.k, f + 3 * CT);
         }
         sum.add<T>(q, VT::max(q));
       }
@@ -773,31 +832,36 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
         const uint32_t n = n0 + k;
         if (k >= held && !(ok = bar_wait(&S.full[n % SLOTS], (n / SLOTS) & 1, dead))) break;
         const int v = v0 + c * CV;
-        const bool inside = v >= lo && v + CV <= min(hi, v1);
-        uint4 q[CU];
-        take(R, v, v1, inside, n, q);
-        __syncwarp();
-        if (lane == 0) bar_arrive(&S.empty[n % SLOTS]);
-        const uint4 mk = B.marks[c * CW + w];
-        const uint32_t any[CU] = {mk.x, mk.y, mk.z, mk.w};
-        T* to = out + ((int64_t)(v + tid) * A - R.off);
+        uint4* chunk = ring + (size_t)(n % SLOTS) * CV;
+        const bool inside = v >= lo && v + CV <= end;
+        if (inside && aligned) {
+          uint4 q[CU];
 #pragma unroll
-        for (int u = 0; u < CU; ++u) {
-          uint64_t h[A / 2];
-          float g[A];
-          VT::pairs(q[u], h);
+          for (int u = 0; u < CU; ++u) q[u] = chunk[u * CT + tid];
+          __syncwarp();
+          if (lane == 0) bar_arrive(&S.empty[n % SLOTS]);
+          T* to = out + ((int64_t)(v + tid) * A - R.off);
 #pragma unroll
-          for (int j = 0; j < A / 2; ++j)
-            split(mul2(ex2_2(mul2(add2(h[j], neg_m), scale2)), coef), g[2 * j], g[2 * j + 1]);
-          const uint4 r = VT::pack(g);
-          if (inside && aligned) {
-            store_once(to + u * CT * A, r, once);
-          } else {
-            const int x = v + u * CT + tid;
-            if (x < v1) store_ragged(out, r, x * A - R.off, P.V);
+          for (int u = 0; u < CU; ++u) {
+            uint64_t h[A / 2];
+            float g[A];
+            VT::pairs(q[u], h);
+#pragma unroll
+            for (int j = 0; j < A / 2; ++j)
+              split(mul2(ex2_2(mul2(add2(h[j], neg_m), scale2)), coef), g[2 * j], g[2 * j + 1]);
+            store_once(to + u * CT * A, VT::pack(g), once);
           }
-          if (any[u])
-            store_listed(out + ((int64_t)v0 * A - R.off), any[u], B.at, B.listg, P.k,
+        } else {
+          const Chunk<T> K = {R.p, R.V, R.off, v, v0, v1};
+          if (k >= held && !inside) mend_chunk<T>(chunk, K, nullptr, nullptr, 0);
+          put_chunk<T>(chunk, K, out, B.m, P.scale, B.coef);
+          __syncwarp();
+          if (lane == 0) bar_arrive(&S.empty[n % SLOTS]);
+        }
+        if (has_marks<CT, CU>(B.marks, c, w)) {
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(B.marks) + (c * CW + w) * CU;
+          for (int u = 0; u < CU; ++u)
+            store_listed(out + ((int64_t)v0 * A - R.off), words[u], B.at, B.listg, P.k,
                          c * CV + u * CT + w * 32);
         }
       }
@@ -855,8 +919,13 @@ int launch_loss(const DistP& P, cudaStream_t st) {
   return launch(k_distill_finish<T>, (unsigned)((P.rows + FW - 1) / FW), FW * 32, 0, st, true, 1, P);
 }
 
+// The gradient's parts need no joining: many, of two vectors a thread at least (256 rows of 151,936
+// bf16: 27.6 us with 5 parts, 30.1 with 2).
 template <typename T>
-int launch_grad(const DistP& P, cudaStream_t st, bool dependent) {
+int launch_grad(DistP P, cudaStream_t st, bool dependent) {
+  const int64_t nv = (P.V + Vec<T>::A - 1) / Vec<T>::A;
+  P.parts = (int)std::max<int64_t>(
+      1, std::min<int64_t>((148 * 8 + P.rows - 1) / P.rows, (nv + 2 * NT - 1) / (2 * NT)));
   return launch(k_distill_grad<T>, (unsigned)(P.rows * P.parts), NT, 0, st, dependent, 1, P);
 }
 
