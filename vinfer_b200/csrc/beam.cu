@@ -22,6 +22,7 @@ using namespace rows;
 
 constexpr int NT = 256, NW = NT / 32;
 constexpr int U = 4;              // 16-byte vectors of a thread and round: 16 KiB a CTA
+constexpr int BUFS = 2;           // rounds in registers
 constexpr int MAX_PARTS = 64;     // parts of a row
 constexpr int MAX_JOIN = 1024;    // entries of a beam's parts together (a warp joins them)
 constexpr int MAX_STAGED = 8192;  // entries of a request's parts together (64 KiB staged)
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
     }
     sum.add<T>(q, mx);
   };
-  stream_rounds<U, NT>(R, v0, v1, work);
+  stream_rounds<U, NT, BUFS>(R, v0, v1, work);
   grid_dependents_may_start();
   __syncthreads();
 

@@ -26,6 +26,7 @@ using namespace rows;
 
 constexpr int NT = 256, NW = NT / 32;
 constexpr int RU = 4;           // 16-byte vectors of a thread and round while summing: 16 KiB a CTA
+constexpr int BUFS = 2;         // rounds in registers
 constexpr int U = 8;            // ... and while writing the gradient
 constexpr int MAX_PARTS = 64;
 constexpr int MAXK = VINFER_DISTILL_MAX_K;
@@ -64,35 +65,33 @@ struct DistP {
 // and a warp's U words of a round lie side by side.
 template <int N, int U>
 __device__ __forceinline__ uint32_t* mark_word(uint4* marks, int v) {
-  static_assert(U % 4 == 0, "a warp's words are 16-byte loads");
   const int c = v / (N * U), u = v % (N * U) / N, w = v % N / 32;
   return reinterpret_cast<uint32_t*>(marks) + (c * (N / 32) + w) * U + u;
 }
 // A warp's words of round c; whether any has a bit.
 template <int N, int U>
 __device__ __forceinline__ bool marks_of(const uint4* marks, int c, int w, uint32_t (&word)[U]) {
+  const uint32_t* at = reinterpret_cast<const uint32_t*>(marks) + (c * (N / 32) + w) * U;
   uint32_t any = 0;
 #pragma unroll
-  for (int i = 0; i < U / 4; ++i) {
-    const uint4 m = marks[(c * (N / 32) + w) * (U / 4) + i];
-    word[4 * i] = m.x;
-    word[4 * i + 1] = m.y;
-    word[4 * i + 2] = m.z;
-    word[4 * i + 3] = m.w;
-    any |= m.x | m.y | m.z | m.w;
+  for (int i = 0; i < U; ++i) {
+    if (U % 4 == 0 && i % 4 == 0) {
+      const uint4 m = *reinterpret_cast<const uint4*>(at + i);
+      word[i] = m.x;
+      word[i + 1] = m.y;
+      word[i + 2] = m.z;
+      word[i + 3] = m.w;
+    } else if (U % 4 != 0) {
+      word[i] = at[i];
+    }
+    any |= word[i];
   }
   return any != 0;
 }
-
 template <int N, int U>
 __device__ __forceinline__ bool has_marks(const uint4* marks, int c, int w) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int i = 0; i < U / 4; ++i) {
-    const uint4 m = marks[(c * (N / 32) + w) * (U / 4) + i];
-    any |= m.x | m.y | m.z | m.w;
-  }
-  return any != 0;
+  uint32_t word[U];
+  return marks_of<N, U>(marks, c, w, word);
 }
 
 // Which elements of vector v are among the n places `at` (a place: element counted from the first
@@ -164,8 +163,8 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   const int v0 = (int)(R.nv * part / P.parts);  // below 2^18 * 64
   const int v1 = (int)(R.nv * (part + 1) / P.parts);
   const int id = tid < P.k ? P.ids[row * P.k + tid] : -1;
-  for (int i = tid; i < (v1 - v0 + NT * RU - 1) / (NT * RU) * NW; i += NT)
-    marked[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < (v1 - v0 + NT * RU - 1) / (NT * RU) * NW * RU; i += NT)
+    reinterpret_cast<uint32_t*>(marked)[i] = 0;
   if (tid == 0) hits = 0;
   __syncthreads();
   {
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
   }
   __syncthreads();
   Exps sum(P.scale);
-  stream_rounds<RU, NT>(R, v0, v1, [&](uint4 (&q)[RU], int vb) {
+  stream_rounds<RU, NT, BUFS>(R, v0, v1, [&](uint4 (&q)[RU], int vb) {
     uint32_t word[RU];
     if (marks_of<NT, RU>(marked, (vb - v0) / (NT * RU), tid / 32, word)) {
 #pragma unroll

@@ -263,20 +263,22 @@ struct Row {
   }
 };
 
-// Streams vectors [v0, v1) of a row through work(q, first vector) in rounds of U a thread, each round
-// loaded while the one before it is worked on. v0 < v1.
-template <int U, int NT, typename T, typename F>
+// Streams vectors [v0, v1) of a row through work(q, first vector) in rounds of U a thread, with
+// BUFS - 1 rounds in flight while one is worked on. v0 < v1.
+template <int U, int NT, int BUFS, typename T, typename F>
 __device__ __forceinline__ void stream_rounds(const Row<T>& R, int v0, int v1, F&& work) {
-  uint4 a[U], b[U];
-  R.template load_round<U, NT>(v0, v1, a);
-  for (int v = v0;; v += 2 * NT * U) {
-    const int v2 = v + NT * U, v3 = v2 + NT * U;
-    if (v2 < v1) R.template load_round<U, NT>(v2, v1, b);
-    work(a, v);
-    if (v2 >= v1) break;
-    if (v3 < v1) R.template load_round<U, NT>(v3, v1, a);
-    work(b, v2);
-    if (v3 >= v1) break;
+  uint4 q[BUFS][U];
+#pragma unroll
+  for (int b = 0; b < BUFS - 1; ++b)
+    if (v0 + b * NT * U < v1) R.template load_round<U, NT>(v0 + b * NT * U, v1, q[b]);
+  for (int v = v0;; v += BUFS * NT * U) {
+#pragma unroll
+    for (int b = 0; b < BUFS; ++b) {
+      const int vb = v + b * NT * U, ahead = vb + (BUFS - 1) * NT * U;
+      if (ahead < v1) R.template load_round<U, NT>(ahead, v1, q[(b + BUFS - 1) % BUFS]);
+      work(q[b], vb);
+      if (vb + NT * U >= v1) return;
+    }
   }
 }
 
@@ -388,14 +390,17 @@ __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
 }
 // Each try may leave the warp suspended this long: a poll that came back at once would take issue
 // slots from the warps that compute.
-constexpr uint32_t SUSPEND_NS = 1000000;
-// Waits for the phase of this parity to end; false after a bounded number of tries (seconds), or
-// once another wait of the CTA has given up: *dead is then set, and every role leaves.
+// A try may leave the warp suspended this long, and sleeps a little behind it: a warp that polled
+// would take issue slots from those that compute (512 -> 494 us for the distillation step).
+constexpr uint32_t SUSPEND_NS = 20000;
+// Waits for the phase of this parity to end; false after a bounded number of tries (0.1 to 5 s; the
+// waits here last microseconds), or once another wait of the CTA has given up: *dead is then set,
+// and every role leaves.
 // CLUSTER: what other CTAs of the cluster sent is seen behind it.
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* dead) {
   const uint32_t a = smem_addr(b);
-  for (int i = 0; i < 1 << 20; ++i) {
+  for (int i = 0; i < 1 << 18; ++i) {
     uint32_t done;
     if (CLUSTER)
       asm volatile(
@@ -414,6 +419,7 @@ __device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile 
           : "memory");
     if (done) return true;
     if (*dead) return false;
+    __nanosleep(100);
   }
   *dead = 1;
   return false;
