@@ -315,7 +315,7 @@ typedef struct VinferDistillArgs {
   const int32_t* ids;      /* [rows, k] */
   const float* logprobs;   /* [rows, k] */
   const float* weights;    /* [rows], NULL: ones */
-  float temperature;       /* > 0 */
+  float temperature;       /* in [1e-37, 1e37] */
   int32_t tail;
   int32_t* status;         /* optional, one device int32 */
 } VinferDistillArgs;

@@ -88,7 +88,7 @@ def test_c_entries_refuse_bad_arguments():
     assert lib.vinfer_distill_step(C.byref(d), 16, 16, 9, 16, big, None) == _lib.E_ARG
     assert lib.vinfer_distill_grad(C.byref(d), 16, None, None, 0, 16, 10, None) == _lib.E_ARG
     assert lib.vinfer_distill_grad(C.byref(d), 16, 16, 16, -1, 16, 10, None) == _lib.E_ARG
-    for t in (0.0, -1.0, float("inf"), float("nan")):
+    for t in (0.0, -1.0, 1e-40, 1e38, float("inf"), float("nan")):
         d.temperature = t
         assert lib.vinfer_distill_loss(C.byref(d), 16, None, None, 16, big, None) == _lib.E_ARG
     d.temperature, d.k = 1.0, 129
@@ -130,6 +130,7 @@ def _lists(n=3, k=2):
     (dict(logprobs=torch.zeros(2, 2)), "logprobs must be"),
     (dict(weights=torch.zeros(3, 1)), "weights must be"),
     (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=1e-40), "temperature"),
 ])
 def test_distill_refuses(backend, what, err):
     ids, lp = _lists()
@@ -255,8 +256,13 @@ def test_decode_states_refuse():
         DecodeStates([t], length_dim=0)
     with pytest.raises(ValueError, match="overlaps itself"):
         DecodeStates([torch.zeros(5).expand(4, 5)])
-    with pytest.raises(ValueError, match="overlaps its state"):
+    with pytest.raises(ValueError, match="overlaps a state"):
         DecodeStates([t], out=[t])
+    u = torch.zeros(4, 3, 5)
+    with pytest.raises(ValueError, match="overlaps a state"):
+        DecodeStates([t, u], out=[u, t])
+    kv = torch.zeros(4, 2, 3, 5)  # outputs side by side in one buffer are fine
+    DecodeStates([t, u], out=[kv[:, 0], kv[:, 1]])
     with pytest.raises(ValueError, match="shape and type"):
         DecodeStates([t], out=[torch.zeros(4, 3, 4)])
     with pytest.raises(ValueError, match="too scattered"):

@@ -280,9 +280,12 @@ def test_upstream_gradients(backend):
         assert np.all(np.abs(leaf.grad.double().cpu().numpy() - want) <= tg + np.abs(want) * 2.0**-23)
 
 
-def test_captured_and_side_streams(backend):
+@pytest.mark.parametrize("N,V,dtype", [(40, 30001, torch.bfloat16), (99, 120007, torch.bfloat16),
+                                       (98, 120007, torch.float32)], ids=str)
+def test_captured_and_side_streams(backend, N, V, dtype):
     dev = backend.device
-    x, ids, lp, w = make(40, 30001, 9, torch.bfloat16)
+    x, ids, lp, w = make(N, V, 9, dtype)
+    w[::5] = 0.0
     d = [t.to(dev) for t in (x, ids, lp, w)]
     eager_l, eager_g = backend.distill_step(*d, tail=True)
     torch.cuda.synchronize()
@@ -300,6 +303,34 @@ def test_captured_and_side_streams(backend):
     torch.cuda.synchronize()
     for l, g in outs:
         assert torch.equal(l, eager_l) and torch.equal(g, eager_g)
+
+
+def test_extreme_temperatures(backend):
+    """At the ends of the range all mass is on the largest logit, or every token's is the same."""
+    dev = backend.device
+    x = torch.tensor([[3.0, 1.0, 2.0, -7.0]], device=dev)
+    ids = torch.tensor([[0, 2]], dtype=torch.int32, device=dev)
+    lp = torch.tensor([[-0.1, -5.0]], device=dev)
+    loss, grad = backend.distill_step(x, ids[:, :1].contiguous(), torch.zeros(1, 1, device=dev),
+                                      temperature=1e-37)
+    assert float(loss[0]) == 0 and torch.isfinite(grad).all()
+    loss, grad = backend.distill_step(x, ids, lp, temperature=1e37)
+    p = np.exp([-0.1, -5.0]) / np.exp([-0.1, -5.0]).sum()
+    assert abs(float(loss[0]) - (p * np.log(p)).sum() - np.log(4)) < 1e-6
+    backend.check()
+
+
+def test_an_output_given_is_seen_to_change(backend):
+    dev = backend.device
+    x, ids, lp, w = make(4, 300, 3, torch.float32)
+    h = x.to(dev).requires_grad_(True)
+    logits = h * 1.0
+    y = logits.exp()                  # saves its output
+    z = (logits ** 2).sum()           # saves logits
+    backend.distill_step(logits.detach(), ids.to(dev), lp.to(dev), out=logits.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    y.sum().backward()
 
 
 def test_no_rows(backend):

@@ -470,7 +470,7 @@ constexpr int CU = 4;                     // vectors a thread takes of a chunk
 constexpr int CV = CT * CU;               // vectors of a chunk: 24 KiB
 constexpr int SLOTS = 4;                  // chunks of the ring
 constexpr int SLICE = 13;                 // chunks of a slice at most
-constexpr int MINC = 1, MAXC = 16;        // CTAs of a cluster
+constexpr int MAXC = 4;                   // CTAs of a cluster
 constexpr int LW = 2;                     // warps that solve, and rows under way
 constexpr int STEP_T = CT + 32 + LW * 32;
 
@@ -883,7 +883,7 @@ int check(const VinferDistillArgs* a) {
   if (!a || !a->logits || !a->ids || !a->logprobs) return VINFER_E_ARG;
   if (a->dtype != VINFER_DTYPE_F32 && a->dtype != VINFER_DTYPE_BF16) return VINFER_E_ARG;
   if (a->rows < 1 || a->vocab < 1 || a->ld < a->vocab || a->k < 1) return VINFER_E_ARG;
-  if (!(a->temperature > 0.f) || !(a->temperature < INFINITY)) return VINFER_E_ARG;
+  if (!(a->temperature >= 1e-37f) || !(a->temperature <= 1e37f)) return VINFER_E_ARG;
   if (((uintptr_t)a->logits) % (a->dtype == VINFER_DTYPE_BF16 ? 2 : 4)) return VINFER_E_ARG;
   if (a->vocab > VINFER_MAX_VOCAB || a->rows > VINFER_DISTILL_MAX_ROWS || a->k > MAXK)
     return VINFER_E_LIMIT;
@@ -928,13 +928,14 @@ int launch_grad(DistP P, cudaStream_t st, bool dependent) {
   return launch(k_distill_grad<T>, (unsigned)(P.rows * P.parts), NT, 0, st, dependent, 1, P);
 }
 
-// The CTAs a row is cut into, a power of two: none when even the largest cluster cannot hold one.
-// A single CTA is launched without a cluster dimension and uses nothing of one.
+// The CTAs a row is cut into, a power of two. A single CTA is launched without a cluster dimension and
+// uses nothing of one.
+static_assert((VINFER_MAX_VOCAB + 6) / 4 <= MAXC * SLICE * CV, "every row fits a cluster");
 int step_cluster(int64_t V, int A) {
   const int64_t nv = (V + 2 * A - 2) / A;  // at any alignment
-  for (int c = MINC; c <= MAXC; c *= 2)
-    if ((nv + c - 1) / c <= SLICE * CV) return c;
-  return 0;
+  int c = 1;
+  while ((nv + c - 1) / c > SLICE * CV) c *= 2;
+  return c;
 }
 
 constexpr size_t STEP_SMEM = (size_t)SLOTS * CV * 16 + sizeof(StepS);
@@ -972,10 +973,6 @@ template <typename T>
 int launch_step(const DistP& P, cudaStream_t st) {
   const int c = step_cluster(P.V, Vec<T>::A);
   if (opt_in(k_distill_step<T>, STEP_SMEM) != VINFER_OK) return VINFER_E_CUDA;
-  if (c > 8 && result(cudaFuncSetAttribute(k_distill_step<T>,
-                                           cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) !=
-                   VINFER_OK)
-    return VINFER_E_CUDA;
   int clusters = 0;
   if (step_clusters<T>(c, &clusters) != VINFER_OK) return VINFER_E_CUDA;
   return launch(k_distill_step<T>, (unsigned)(std::min<int64_t>(P.rows, clusters) * c), STEP_T,
@@ -989,7 +986,7 @@ int launch_step(const DistP& P, cudaStream_t st) {
 bool step_in_one(const DistP& P, int dtype) {
   const bool bf = dtype == VINFER_DTYPE_BF16;
   const int64_t bytes = (int64_t)P.V * (bf ? 2 : 4);
-  return P.rows >= 96 && bytes >= (bf ? 160 << 10 : 96 << 10) && step_cluster(P.V, bf ? 8 : 4) > 0;
+  return P.rows >= 96 && bytes >= (bf ? 160 << 10 : 96 << 10);
 }
 
 size_t align_up(size_t n) { return (n + 255) / 256 * 256; }

@@ -329,8 +329,8 @@ class B200Sampler:
         k = ids.shape[1] if ids.dim() == 2 else 0
         if not 1 <= k <= _lib.DISTILL_MAX_K:
             raise ValueError(f"ids must be [rows, k] with k in [1, {_lib.DISTILL_MAX_K}]")
-        if not 0 < temperature < float("inf"):
-            raise ValueError(f"temperature must be finite and > 0, got {temperature}")
+        if not 1e-37 <= temperature <= 1e37:
+            raise ValueError(f"temperature must be in [1e-37, 1e37], got {temperature}")
         a = _lib.DistillArgs()
         a.ids = self._vector("ids", ids, torch.int32, n, k)
         a.logprobs = self._vector("logprobs", logprobs, torch.float32, n, k)
@@ -401,9 +401,10 @@ class B200Sampler:
         """The rows' losses and the gradient of their sum with respect to the logits in one call,
         for a training step whose row weights are known ahead (``logits.backward(grad)``
         carries on). ``out`` receives the gradient; it may be ``logits`` itself, whose memory
-        the step then reuses."""
+        the step then reuses. Nothing is recorded for autograd."""
         a = self._distill_args(logits, ids, logprobs, weights, temperature, tail)
-        if out is None:
+        given = out is not None
+        if not given:
             out = self._grad_like(logits, a.ld)
         elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != self.device or \
                 (out.stride(1) != 1 and a.vocab > 1) or (a.rows > 1 and out.stride(0) < a.vocab):
@@ -418,6 +419,8 @@ class B200Sampler:
             self._call(self.lib.vinfer_distill_step, "vinfer_distill_step", C.byref(a),
                        loss.data_ptr(), out.data_ptr(),
                        out.stride(0) if a.rows > 1 else a.vocab, ws.data_ptr(), nbytes)
+        if given:  # whoever saved it for a backward pass learns that it changed
+            torch.autograd.graph.increment_version(out)
         return loss, out
 
     def sample(self, logits: torch.Tensor, params: SamplingParams, seed: int,

@@ -312,8 +312,8 @@ class DecodeStates:
             ld = None if length_dim is None else self._dim(t, length_dim, "length_dim")[0]
             if ld == sd:
                 raise ValueError("length_dim must not be slot_dim")
-            if out is not None and _overlap(t, u):
-                raise ValueError(f"output {i} overlaps its state")
+            if out is not None and any(_overlap(v, u) for v in self.tensors):
+                raise ValueError(f"output {i} overlaps a state")
             if t.numel():
                 found.append(_describe(i, t, u, sd, ld))
         self.count = len(found)
