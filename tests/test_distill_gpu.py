@@ -305,6 +305,32 @@ def test_captured_and_side_streams(backend, N, V, dtype):
         assert torch.equal(l, eager_l) and torch.equal(g, eager_g)
 
 
+def test_a_captured_backward_pass(backend):
+    """Loss and gradient through autograd inside a captured graph, replayed on new inputs."""
+    dev = backend.device
+    x, ids, lp, w = make(64, 9001, 9, torch.bfloat16)
+    d = [t.to(dev) for t in (ids, lp, w)]
+    leaf = x.to(dev).requires_grad_(True)
+    s = torch.cuda.Stream(dev)
+    s.wait_stream(torch.cuda.current_stream())
+    gr = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(gr, stream=s):
+        loss = distillation_loss(backend, leaf, *d, tail=True)
+        (grad,) = torch.autograd.grad(loss.mean(), leaf)
+    for seed in (0, 1):
+        y, ids2, lp2, w2 = make(64, 9001, 9, torch.bfloat16, seed=seed)
+        with torch.no_grad():
+            for to, t in zip((leaf, *d), (y, ids2, lp2, w2)):
+                to.copy_(t)
+        gr.replay()
+        torch.cuda.synchronize()
+        compare(y, ids2, lp2, w2, 1.0, True, loss.detach())
+        _, want = backend.distill_step(leaf.detach(), d[0], d[1], d[2] / 64, tail=True)
+        # two roundings of the same value, the weight's to float32 between them: one bf16 step
+        assert torch.allclose(grad.float(), want.float(), rtol=2.0**-7, atol=1e-9)
+
+
 def test_extreme_temperatures(backend):
     """At the ends of the range all mass is on the largest logit, or every token's is the same."""
     dev = backend.device

@@ -50,5 +50,7 @@ def distillation_loss(backend: B200Sampler, logits: torch.Tensor, ids: torch.Ten
     row stride), ``ids`` int32 and ``logprobs`` float32 ``[rows, k]`` with ``k <= 128``,
     ``weights`` float32 ``[rows]`` (a row of weight 0 is not read and gets loss and gradient 0).
     Gradients flow to ``logits`` alone, once: there is no second derivative. Where the weights of the
-    sum are known ahead, ``backend.distill_step`` computes loss and gradient in one call."""
+    sum are known ahead, ``backend.distill_step`` computes loss and gradient in one call. As with every
+    torch operation, a backward pass is captured into a CUDA graph only while no eager graph of the
+    same leaves is alive; ``distill_step`` knows no leaves."""
     return _ListLoss.apply(logits, backend, ids, logprobs, weights, temperature, tail)
