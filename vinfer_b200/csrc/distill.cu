@@ -15,6 +15,13 @@
 //   * k_distill_finish, one warp a row: joins the parts and the list's k terms in double.
 //   * k_distill_grad reads the row again and writes the gradient, one exponential an element; the
 //     listed elements are stored behind it.
+//   * k_distill_step does all of it for long rows, which it reads from HBM once (below).
+//
+// What bounds them: HBM, then the exponentials' instructions. Measured on one B200, in us, with the share
+// of the measured copy bandwidth: losses of 1,024 rows of 151,936 bf16 58.8 (0.81); of 256 rows 27; the
+// gradient alone of 1,024 rows 104 (6.0 TB/s, 0.91); loss and gradient in one call of 4,096 rows of
+// 151,936 bf16, 512 of them masked, 494 (0.72) against 591 by the three kernels, of 512 rows of 248,320
+// float32 with lists of 128 229 (0.68) against 307.
 #include "rows.cuh"
 
 #include <algorithm>
@@ -27,7 +34,7 @@ using namespace rows;
 constexpr int NT = 256, NW = NT / 32;
 constexpr int RU = 4;           // 16-byte vectors of a thread and round while summing: 16 KiB a CTA
 constexpr int BUFS = 2;         // rounds in registers
-constexpr int U = 8;            // ... and while writing the gradient
+constexpr int U = 8;            // vectors of a thread and round while writing the gradient
 constexpr int MAX_PARTS = 64;
 constexpr int MAXK = VINFER_DISTILL_MAX_K;
 static_assert(MAXK <= NT && MAXK <= 128, "one thread an entry; four entries a lane");
@@ -402,7 +409,7 @@ __global__ void __launch_bounds__(FW * 32) k_distill_finish(const DistP P) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
+__global__ void __launch_bounds__(NT, 3) k_distill_grad(const DistP P) {
   using VT = Vec<T>;
   constexpr int A = VT::A;
   const uint32_t row = blockIdx.x / (uint32_t)P.parts, part = blockIdx.x - row * P.parts;
@@ -460,10 +467,18 @@ __global__ void __launch_bounds__(NT, 4) k_distill_grad(const DistP P) {
 // streams the slice into a ring of chunks by bulk copies; CW warps sum the chunks, releasing
 // each until the ring can hold the rest of the slice, and write the gradient once the row is
 // solved: first of the chunks the ring still holds, then of the others, which the producer brings
-// once more, from L2 (the slices are cut so that few are, and nothing else is kept there). HBM sees
-// every row read once and written once. Two warps solve rows in turn: each prepares its row's list
-// ahead, joins the CTA's sum with the other CTAs' (each sends its own to all), and hands out the
-// gradient's terms. Two CTAs an SM, so that one streams while the other solves.
+// once more, from L2 (policies keep nothing else there: without them half of these bytes came from
+// HBM again). HBM sees every row read once and written once. Two warps solve rows in turn: each
+// prepares its row's list ahead, joins the CTA's sum with the other CTAs' (each sends its own to
+// all), and hands out the gradient's terms. Two CTAs an SM, so that one streams while the other
+// solves.
+//
+// Measured for 4,096 rows of 151,936 bf16 (512 masked): 494 us; the same kernel without any
+// arithmetic 452, so it is the pipeline of copies that bounds it, at 5.2 TB/s of a mix of reads and
+// writes that a plain streaming kernel takes at 6.0. One CTA an SM with a ring twice as large 545; a
+// row whole in the shared memory of four CTAs, the next one summed before it is written, 894 (what
+// a slice waits for, the solution and the copies, takes longer than the slice); chunks of 8
+// vectors a thread 569; three or four CTAs an SM 606 (their slices no longer stay in L2).
 constexpr int STEP_CTAS = 2;              // CTAs of an SM
 constexpr int CW = 12, CT = CW * 32;      // warps and threads that sum and write
 constexpr int CU = 4;                     // vectors a thread takes of a chunk
