@@ -349,8 +349,17 @@ struct PickP {
   int* status;
 };
 
+// 8 bytes from global to shared memory, without waiting; all of a thread's: copies_async_wait.
+__device__ __forceinline__ void copy_async8(u64* dst, const u64* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_async_wait() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 struct PickS {
   double m[MAXW], lns[MAXW];  // log-sum of each beam's row: m + lns
+  double sum[MAXW];           // lns = log(sum)
   float b[MAXW];              // beam scores
   int cnt[MAXW];              // entries of each beam's list
   int head[MAXN];             // ranked candidates: beam << 16 | place in its list
@@ -400,7 +409,7 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
   grid_dependency_wait();
 
   const u64* E = P.list + (int64_t)req * W * per;
-  for (int i = tid; i < W * per; i += PT) staged[i] = E[i];  // dead beams': whatever is there
+  for (int i = tid; i < W * per; i += PT) copy_async8(staged + i, E + i);  // dead beams': whatever is there
   for (int beam = w; beam < W; beam += PW) {
     const PartHdr* H = P.hdr + ((int64_t)req * W + beam) * P.parts;
     float m = neg_inf(), m2 = neg_inf(), s0 = 0, s1 = 0;  // MAX_PARTS is two a lane
@@ -420,14 +429,16 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
     s = warp_sum(s);
     if (lane == 0) {
       S.m[beam] = top;
-      S.lns[beam] = s;  // its logarithm below
+      S.sum[beam] = s;
+      S.lns[beam] = log(s);
     }
   }
+  copies_async_wait();
   __syncthreads();
 
   for (int beam = w; beam < W; beam += PW) {
     const float b = S.b[beam];
-    const double s = S.lns[beam];
+    const double s = S.sum[beam];
     int cnt = 0;
     unsigned bad = 0;
     if (!(b > neg_inf() && b < -neg_inf())) {
@@ -444,15 +455,17 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
       const u64 h1 = lane + 32 < P.parts ? mine[(lane + 32) * n + d] : 0;
       u64 bound = h0 > h1 ? h0 : h1;
       if (d == 0 && P.parts > n) {
+        const uint32_t k0 = (uint32_t)(h0 >> 32), k1 = (uint32_t)(h1 >> 32);  // by their logits
         int r0 = 0, r1 = 0;
+#pragma unroll 8
         for (int o = 0; o < P.parts; ++o) {
-          const u64 h = mine[o * n];
-          r0 += h < h0 || (h == h0 && o < lane);
-          r1 += h < h1 || (h == h1 && o < lane + 32);
+          const uint32_t k = (uint32_t)(mine[o * n] >> 32);
+          r0 += k < k0 || (k == k0 && o < lane);
+          r1 += k < k1 || (k == k1 && o < lane + 32);
         }
         bound = 0;
-        if (lane < P.parts && r0 == n - 1) bound = h0;
-        if (lane + 32 < P.parts && r1 == n - 1) bound = h1;
+        if (lane < P.parts && r0 == n - 1) bound = h0 | 0xffffffffu;
+        if (lane + 32 < P.parts && r1 == n - 1) bound = h1 | 0xffffffffu;
       }
 #pragma unroll
       for (int o = 16; o; o >>= 1) {
@@ -460,12 +473,22 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
         bound = other > bound ? other : bound;
       }
       int alive = 0;
-      for (int i0 = 0; i0 < per; i0 += 32) {
-        const u64 e = i0 + lane < per ? mine[i0 + lane] : NONE;
-        const bool keep = e <= bound && e != NONE;
-        const unsigned who = __ballot_sync(FULL, keep);  // all have read; places are behind i0
-        if (keep) mine[alive + __popc(who & ((1u << lane) - 1))] = e;
-        alive += __popc(who);
+      for (int i0 = 0; i0 < per; i0 += 128) {
+        u64 e[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = i0 + x * 32 + lane;
+          e[x] = i < per ? mine[i] : NONE;
+        }
+        __syncwarp();  // all have read; places are behind what is read next
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const bool keep = e[x] <= bound && e[x] != NONE;
+          const unsigned who = __ballot_sync(FULL, keep);
+          if (keep) mine[alive + __popc(who & ((1u << lane) - 1))] = e[x];
+          alive += __popc(who);
+        }
+        __syncwarp();
       }
       __syncwarp();
       for (int i = lane; i < alive; i += 32) {
@@ -479,7 +502,6 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
     if (lane == 0) {
       if (bad && Q.status) atomicOr(Q.status, (int)bad);
       S.cnt[beam] = cnt;
-      if (cnt) S.lns[beam] = log(s);
     }
   }
   __syncthreads();
@@ -505,6 +527,7 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
       const int bi = i / n, ji = i - bi * n;
       if (ji >= S.cnt[bi]) continue;
       const long long mine = order[i];
+      const double my = sc[i];
       int rank = ji;
       uint32_t close = 0;
       for (int k0 = 0; k0 < W && rank < n; k0 += 4) {
@@ -512,19 +535,22 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
         for (int step = top_step; step; step >>= 1) {
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
+            // no branches: the loads of the four are in flight together
             const int k = k0 + x, at = lo[x] + step - 1;
-            if (k < W && at < n && order[k * n + at] >= mine + (k < bi ? 0 : 1)) lo[x] += step;
+            const long long o = order[min(k, W - 1) * n + min(at, n - 1)];
+            lo[x] += at < n && o >= mine + (k < bi ? 0 : 1) ? step : 0;
           }
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int k = k0 + x;
-          if (k >= W || k == bi) continue;
-          rank += lo[x];
-          const double* o = sc + k * n;
-          if ((lo[x] > 0 && o[lo[x] - 1] - sc[i] <= NEAR) ||
-              (lo[x] < S.cnt[k] && sc[i] - o[lo[x]] <= NEAR))
-            close |= 1u << k;
+          const double* o = sc + min(k, W - 1) * n;
+          const double up = o[max(lo[x] - 1, 0)], down = o[min(lo[x], n - 1)];
+          const bool near = (lo[x] > 0 && up - my <= NEAR) || (lo[x] < n && my - down <= NEAR);
+          if (k < W && k != bi) {
+            rank += lo[x];
+            close |= near ? 1u << k : 0u;
+          }
         }
       }
       if (rank < n) {
@@ -560,7 +586,7 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
     }
   }
   // the beams that go on: the first W candidates whose token is no stop id
-  if (tid < 32 && Q.parents) {
+  if (w == PW - 1 && Q.parents) {  // beside the warps that write the list
     int nsel = 0;
     for (int i0 = 0; i0 < have && nsel < W; i0 += 32) {
       const int i = i0 + lane;
