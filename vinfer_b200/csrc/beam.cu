@@ -15,8 +15,8 @@
 //
 // What bounds it: reading the logits once, then the instructions of the exponentials (8 an element
 // with all overheads; the ex2 unit alone is half busy). Measured on one B200, us a step: 32
-// requests of 16 beams, 248,320 float32 logits 97.7 (508 MB: 5.2 TB/s, 0.80 of the measured copy
-// bandwidth); 64 of 4, 151,936 bf16 29.3 (77.8 MB: 0.41); one of 4 11.0, most of it the two kernels'
+// requests of 16 beams, 248,320 float32 logits 96.2 (508 MB: 5.3 TB/s, 0.81 of the measured copy
+// bandwidth); 64 of 4, 151,936 bf16 28.5 (77.8 MB: 0.42); one of 4 9.8, most of it the two kernels'
 // latency. Selecting costs little because it is not sorting: a part of a row finds a bar that n of
 // its elements reach from its lanes' maxima, and looks again only at the 16-vector rounds of the
 // threads that reach it (keeping the vectors themselves in shared memory cost 3 us more of 32).
