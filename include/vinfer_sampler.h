@@ -255,9 +255,9 @@ int vinfer_beam_select(const VinferBeamArgs* args, void* workspace, size_t works
  * every state takes the contents of slot parents[s]. A state is described by its runs of
  * contiguous bytes: slot s holds, for every index of the outer dimensions, run_bytes bytes at
  * base + s * slot_stride + sum(index * outer_stride) (strides in bytes).
- *  - In place (dst == src, in all states or in none): parents[s] == s leaves the slot alone; any
- *    other parent must keep its own state (parents[parents[s]] == parents[s], as vinfer_beam_select
- *    lays beams out), else the slot is left alone and VINFER_ST_BAD_PARENT set.
+ *  - In place (dst == src and equal strides, in all states or in none): parents[s] == s leaves the
+ *    slot alone; any other parent must keep its own state (parents[parents[s]] == parents[s], as
+ *    vinfer_beam_select lays beams out), else the slot is left alone and VINFER_ST_BAD_PARENT set.
  *  - Into another buffer (which must not overlap the source): every slot is copied, from any parent.
  *  - lengths (device int32 [slots]) with len_unit_bytes > 0 copies only the first lengths[s]
  *    positions (of len_unit_bytes each) of every run, with len_outer >= 0 only the first lengths[s]

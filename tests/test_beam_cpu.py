@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from vinfer_b200 import _lib
+from vinfer_b200.beam import BeamSearch
 from vinfer_b200.build import build
 from vinfer_b200.kernels.sampler.b200 import B200Sampler
 from vinfer_b200.sampling import BeamStep, DecodeStates, SlotHistogram
@@ -77,6 +78,11 @@ def test_c_entries_refuse_bad_arguments():
     s[0].len_unit_bytes = 24                                                      # no divisor
     assert lib.vinfer_reorder_states(s, 1, 16, 4, 16, None, None) == _lib.E_ARG
     s[0].len_unit_bytes = 16                                                      # no lengths
+    assert lib.vinfer_reorder_states(s, 1, 16, 4, None, None, None) == _lib.E_ARG
+    s[0].len_unit_bytes, s[0].src_slot_stride, s[0].dst_slot_stride = 0, 64, 128   # one tensor, two layouts
+    assert lib.vinfer_reorder_states(s, 1, 16, 4, None, None, None) == _lib.E_ARG
+    s[0].dst_slot_stride, s[0].n_outer = 64, 1
+    s[0].outer_size[0], s[0].src_outer_stride[0], s[0].dst_outer_stride[0] = 2, 256, 512
     assert lib.vinfer_reorder_states(s, 1, 16, 4, None, None, None) == _lib.E_ARG
 
     d = _lib.DistillArgs()
@@ -268,6 +274,24 @@ def test_decode_states_refuse():
     with pytest.raises(ValueError, match="too scattered"):
         DecodeStates([torch.zeros(4, 4, 4, 4, 4, 4, 4)[:, ::2, ::2, ::2, ::2, ::2, ::2]])
     assert DecodeStates([torch.zeros(4, 0)]).count == 0
+
+
+def test_outputs_are_given_once():
+    t, u, out = torch.zeros(4, 3), torch.ones(4, 3), torch.zeros(4, 3)
+    with pytest.raises(ValueError, match="given twice"):
+        DecodeStates([t, u], out=[out, out])
+    e = torch.zeros(4, 0)
+    assert DecodeStates([e, e], out=[torch.zeros(4, 0)] * 2).count == 0
+
+
+def test_search_refuses_states(backend):
+    t = torch.zeros(4, 3, 5)
+    with pytest.raises(ValueError, match="in place"):
+        BeamSearch(backend, 2, 2, 3, states=[DecodeStates([t], out=[torch.zeros(4, 3, 5)])])
+    search = BeamSearch(backend, 2, 2, 3, states=[DecodeStates([t], length_dim=1)])
+    with pytest.raises(ValueError, match="need lengths"):
+        search.step(torch.zeros(4, 10))
+    assert search.steps == 0 and search.scores[:, 0].eq(0).all()
 
 
 def test_reorder_refuses(backend):

@@ -46,6 +46,8 @@ class BeamSearch:
         for s in states:
             if s.slots != requests * width:
                 raise ValueError(f"states have {s.slots} slots for {requests} * {width} beams")
+            if not s.in_place:
+                raise ValueError("the states that follow the beams are copied in place, without out")
         self.backend, self.requests, self.width = backend, requests, width
         self.max_tokens, self.length_penalty, self.states = max_tokens, length_penalty, list(states)
         dev = backend.device
@@ -88,6 +90,8 @@ class BeamSearch:
         ``lengths`` (int32 ``[R * W]``): the positions of the states that hold data."""
         if self.steps >= self.max_tokens:
             raise ValueError(f"the search has taken its {self.max_tokens} tokens")
+        if lengths is None and any(s.has_lengths for s in self.states):
+            raise ValueError("states with a length_dim need lengths")
         b = self.backend.beam_select(logits, self.scores, self.n, eos=self.eos, out=self.out)
         self.steps += 1
         if self.eos is not None:

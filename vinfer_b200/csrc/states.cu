@@ -267,8 +267,10 @@ extern "C" int vinfer_reorder_states(const VinferState* states, int32_t n_states
     if (s.len_unit_bytes < 0 || (s.len_unit_bytes > 0 && (s.run_bytes % s.len_unit_bytes || s.len_outer >= 0)))
       return VINFER_E_ARG;
     if ((s.len_unit_bytes > 0 || s.len_outer >= 0) && !lengths) return VINFER_E_ARG;
+    if (in_place && s.src_slot_stride != s.dst_slot_stride) return VINFER_E_ARG;
     for (int k = 0; k < s.n_outer; ++k)
-      if (s.outer_size[k] < 1) return VINFER_E_ARG;
+      if (s.outer_size[k] < 1 || (in_place && s.src_outer_stride[k] != s.dst_outer_stride[k]))
+        return VINFER_E_ARG;
   }
   Desc d;
   for (int i = 0; i < n_states; ++i) {  // nothing is copied unless everything can be

@@ -314,9 +314,13 @@ class DecodeStates:
                 raise ValueError("length_dim must not be slot_dim")
             if out is not None and any(_overlap(v, u) for v in self.tensors):
                 raise ValueError(f"output {i} overlaps a state")
+            if out is not None and t.numel() and any(u.data_ptr() == v.data_ptr()
+                                                     for v in self.out[:i] if v.numel()):
+                raise ValueError(f"output {i} is given twice")
             if t.numel():
                 found.append(_describe(i, t, u, sd, ld))
         self.count = len(found)
+        self.in_place = all(d.src == d.dst for d in found)
         self.array = (_lib.State * max(1, self.count))(*found)
 
     @staticmethod
