@@ -383,3 +383,19 @@ def test_the_teachers_lists_come_from_the_sampler(backend):
     for tail in (False, True):
         _, _, loss, grad, _ = run_all(backend, x, ids, lp, w, 2.0, tail)
         compare(x, ids, lp, w, 2.0, tail, loss, grad)
+
+
+def test_a_loss_without_gradient_records_nothing(backend):
+    x, ids, lp, w = (t.to(backend.device) for t in make(4, 300, 3, torch.float32))
+    leaf = x.clone().requires_grad_(True)
+    recorded = distillation_loss(backend, leaf, ids, lp, w)
+    with torch.no_grad():
+        alone = distillation_loss(backend, leaf, ids, lp, w)
+    assert recorded.requires_grad and not alone.requires_grad
+    assert not distillation_loss(backend, x, ids, lp, w).requires_grad
+    assert torch.equal(recorded.detach(), alone)
+    with torch.autograd.forward_ad.dual_level():  # a tangent is refused, not dropped
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            distillation_loss(backend, dual, ids, lp, w)
+    backend.check()

@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import TYPE_CHECKING
 
 import torch
+from torch.autograd import forward_ad
 
 if TYPE_CHECKING:
     from vinfer_b200.kernels.sampler.b200 import B200Sampler
@@ -53,4 +54,8 @@ def distillation_loss(backend: B200Sampler, logits: torch.Tensor, ids: torch.Ten
     sum are known ahead, ``backend.distill_step`` computes loss and gradient in one call. As with every
     torch operation, a backward pass is captured into a CUDA graph only while no eager graph of the
     same leaves is alive; ``distill_step`` knows no leaves."""
+    if not (logits.requires_grad and torch.is_grad_enabled()) and forward_ad._current_level < 0:
+        # nothing to record (the autograd function costs a call 6 us): the loss alone
+        return backend.distill_loss(logits, ids, logprobs, weights, temperature=temperature,
+                                    tail=tail)[0]
     return _ListLoss.apply(logits, backend, ids, logprobs, weights, temperature, tail)

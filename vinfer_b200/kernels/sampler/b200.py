@@ -411,9 +411,9 @@ class B200Sampler:
             raise ValueError("out must have the logits' shape and type, with unit column stride")
         loss = torch.empty(a.rows, dtype=torch.float32, device=self.device)
         if a.rows:
-            if out.data_ptr() != logits.data_ptr() or (a.rows > 1 and out.stride(0) != a.ld):
-                if _overlap(logits, out):
-                    raise ValueError("out must be the logits themselves or not overlap them")
+            if given and (out.data_ptr() != logits.data_ptr()
+                          or (a.rows > 1 and out.stride(0) != a.ld)) and _overlap(logits, out):
+                raise ValueError("out must be the logits themselves or not overlap them")
             nbytes = self.lib.vinfer_distill_workspace_bytes(a.rows, a.vocab, a.dtype, a.k)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
             self._call(self.lib.vinfer_distill_step, "vinfer_distill_step", C.byref(a),
