@@ -54,7 +54,7 @@ extern "C" {
 #define VINFER_ST_BAD_PARAM 1u   /* a row's parameters are invalid; its id is -1 */
 #define VINFER_ST_NONFINITE 2u   /* a row has no finite maximum after processing */
 #define VINFER_ST_HIST_FULL 4u   /* vinfer_hist_append: a slot had no room for a new token */
-#define VINFER_ST_INTERNAL 8u    /* an internal consistency check failed */
+#define VINFER_ST_INTERNAL 8u    /* an internal check failed, or a kernel's wait reached its limit */
 #define VINFER_ST_BAD_SCORE 16u  /* vinfer_beam_select: a beam's score is NaN or +inf */
 #define VINFER_ST_BAD_PARENT 32u /* vinfer_reorder_states: a parent that cannot be copied from */
 #define VINFER_ST_BAD_LIST 64u   /* vinfer_distill_*: an id or a log-probability out of range */
@@ -301,7 +301,11 @@ int vinfer_reorder_states(const VinferState* states, int32_t n_states, const int
  *  - vinfer_distill_grad: d(sum_r grad_out[r] * loss[r]) / dlogits, of the logits' type, rounded once
  *    (grad_out NULL: ones; its stride in elements, 0 for one value shared by all rows). args as for
  *    the loss. grad may be the logits (then with their ld).
- *  - vinfer_distill_step: both in one call, grad_out all ones. grad may be the logits.
+ *  - vinfer_distill_step: both in one call, grad_out all ones. grad may be the logits. Its one-pass
+ *    kernel waits for its own copies and partners; a wait that reaches its limit (seconds) sets
+ *    VINFER_ST_INTERNAL, and what that call leaves in loss and grad is not to be used.
+ *  - vinfer_distill_step_within: the same with a limit of about wait_ns for each wait (0: one look;
+ *    negative: the usual limit).
  * The workspace needs no initialisation and holds nothing between calls; 16-byte aligned. */
 #define VINFER_DISTILL_MAX_K 128
 #define VINFER_DISTILL_MAX_ROWS (1 << 22)
@@ -327,6 +331,9 @@ int vinfer_distill_grad(const VinferDistillArgs* args, const float* row_stats,
                         void* grad, int64_t ld_grad, void* stream);
 int vinfer_distill_step(const VinferDistillArgs* args, float* loss, void* grad, int64_t ld_grad,
                         void* workspace, size_t workspace_bytes, void* stream);
+int vinfer_distill_step_within(const VinferDistillArgs* args, float* loss, void* grad,
+                               int64_t ld_grad, void* workspace, size_t workspace_bytes,
+                               int64_t wait_ns, void* stream);
 
 #ifdef __cplusplus
 }

@@ -55,6 +55,7 @@ EXPORTS = (
     "vinfer_distill_loss",
     "vinfer_distill_grad",
     "vinfer_distill_step",
+    "vinfer_distill_step_within",
 )
 
 _ERRORS = {E_ARG: "invalid argument", E_LIMIT: "limit exceeded", E_CUDA: "CUDA error"}
@@ -216,6 +217,10 @@ def load() -> C.CDLL:
     lib.vinfer_distill_step.restype = C.c_int
     lib.vinfer_distill_step.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p, C.c_int64,
                                         C.c_void_p, C.c_size_t, C.c_void_p]
+    lib.vinfer_distill_step_within.restype = C.c_int
+    lib.vinfer_distill_step_within.argtypes = [C.POINTER(DistillArgs), C.c_void_p, C.c_void_p,
+                                               C.c_int64, C.c_void_p, C.c_size_t, C.c_int64,
+                                               C.c_void_p]
     version = lib.vinfer_sampler_abi_version()
     if version != ABI_VERSION:
         raise RuntimeError(f"sampler library ABI {version}, expected {ABI_VERSION}")
@@ -237,7 +242,7 @@ def status_message(bits: int) -> str:
     if bits & ST_HIST_FULL:
         names.append("a history slot was full (a token was not counted)")
     if bits & ST_INTERNAL:
-        names.append("internal consistency check failed")
+        names.append("internal consistency check failed, or a wait reached its limit")
     if bits & ST_BAD_SCORE:
         names.append("a beam's score is NaN or +inf")
     if bits & ST_BAD_PARENT:

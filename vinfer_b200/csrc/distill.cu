@@ -66,6 +66,7 @@ struct DistP {
   int64_t go_stride;
   void* grad;
   int64_t ldg;
+  WaitLimit limit;   // of the waits of k_distill_step
 };
 
 // The word of marks that has the bit of vector v, where rounds are of U vectors for each of N threads
@@ -650,7 +651,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       bar_init(&S.row[i].list_full, 1);
       bar_init(&S.row[i].list_empty, CW);
       bar_init(&S.row[i].summed, CW);
-      bar_init(&S.row[i].joined, 1);
+      bar_init(&S.row[i].joined, size);
       bar_init(&S.row[i].solved, 1);
     }
     S.dead = 0;
@@ -669,7 +670,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
   uint32_t taken = 0;
   auto next_row = [&](int64_t& row, float& weight) {
     const int i = taken % ROWQ;
-    if (!bar_wait(&S.row_full[i], (taken / ROWQ) & 1, dead)) return false;
+    if (!warp_wait(&S.row_full[i], (taken / ROWQ) & 1, dead, P.limit)) return false;
     row = S.next_row[i];
     weight = S.next_weight[i];
     __syncwarp();
@@ -679,19 +680,23 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
   };
   int64_t row;
   float weight;
+  uint32_t it = 0;  // chunks so far
 
   if (w == CW) {  // ---- the producer
     RowWalk walk(P, blockIdx.x / size, gridDim.x / size);
-    uint32_t it = 0, handed = 0;  // chunks and rows so far
+    uint32_t handed = 0;  // rows so far
     int ok = 1;
     auto hand = [&](int64_t& r, float& wt) {
       if (!walk.next(r, wt)) r = -1;
       if (lane == 0) {
         const int i = handed % ROWQ;
-        if (handed >= ROWQ) ok = bar_wait(&S.row_empty[i], (handed / ROWQ - 1) & 1, dead);
-        S.next_row[i] = r;
-        S.next_weight[i] = wt;
-        bar_arrive(&S.row_full[i]);
+        if (handed >= ROWQ)
+          ok = bar_wait(&S.row_empty[i], (handed / ROWQ - 1) & 1, dead, P.limit);
+        if (ok) {
+          S.next_row[i] = r;
+          S.next_weight[i] = wt;
+          bar_arrive(&S.row_full[i]);
+        }
       }
       ++handed;
       ok = __shfl_sync(FULL, ok, 0);
@@ -699,7 +704,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
     int64_t row1 = -1, row2 = -1;
     float weight1 = 0.f, weight2 = 0.f;
     hand(row, weight);
-    if (row >= 0) hand(row1, weight1);
+    if (ok && row >= 0) hand(row1, weight1);
     for (; ok && row >= 0; row = row1, weight = weight1, row1 = row2, weight1 = weight2) {
       row2 = -1;
       if (row1 >= 0) hand(row2, weight2);
@@ -712,7 +717,8 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
         const int C = (v1 - v0 + CV - 1) / CV, again = max(C - SLOTS, 0);
         for (int c = 0; c < C + again; ++c, ++it) {
           const int slot = it % SLOTS, v = v0 + (c < C ? c : c - C) * CV;
-          if (it >= SLOTS && !(ok = bar_wait(&S.empty[slot], (it / SLOTS - 1) & 1, dead))) break;
+          if (it >= SLOTS && !(ok = bar_wait(&S.empty[slot], (it / SLOTS - 1) & 1, dead, P.limit)))
+            break;
           const int a = max(v, lo), b = min(v + CV, hi);
           if (b > a) {
             bar_expect(&S.full[slot], (uint32_t)(b - a) * 16);
@@ -725,12 +731,6 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       }
       ok = __shfl_sync(FULL, ok, 0);
     }
-    // no copy of this CTA may land behind its end
-    if (lane == 0 && *dead)
-      for (uint32_t k = it > SLOTS ? it - SLOTS : 0; k < it; ++k) {
-        int none = 0;
-        bar_wait(&S.full[k % SLOTS], (k / SLOTS) & 1, &none);
-      }
   } else if (w > CW) {  // ---- the lists' warps
     const int mine = w - CW - 1;
     StepRow& B = S.row[mine];
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       const Row<T> R(static_cast<const T*>(P.logits) + row * P.ld, P.V);
       const int v0 = R.nv * rank / size, v1 = R.nv * (rank + 1) / size;
       list_begin<T>(P, row, B.list);
-      if (use > 0 && !bar_wait(&B.list_empty, (use - 1) & 1, dead)) break;
+      if (use > 0 && !warp_wait(&B.list_empty, (use - 1) & 1, dead, P.limit)) break;
       for (int j = lane; j < P.k; j += 32)
         if (B.at[j] >= 0) *mark_word<CT, CU>(B.marks, B.at[j] / A) = 0;
       __syncwarp();
@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       }
       __syncwarp();
       if (lane == 0) bar_arrive(&B.list_full);
-      if (!bar_wait(&B.summed, use & 1, dead)) break;
+      if (!warp_wait(&B.summed, use & 1, dead, P.limit)) break;
       // this CTA's sum to all, and all joined: in a fixed order, the same in every CTA
       float pm = lane < CW ? B.part_m[lane] : neg_inf(), ps = lane < CW ? B.part_s[lane] : 0.f;
       float m = warp_max(pm);
@@ -766,12 +766,11 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(FULL, s, o);
       double r = s;
       if (size > 1) {
-        if (lane == 0) bar_expect(&B.joined, size * 8);
-        __syncwarp();
         if (lane < size)
           send(&B.part[rank], &B.joined, lane,
                (uint64_t)__float_as_uint(s) << 32 | __float_as_uint(m));
-        if (!bar_wait<true>(&B.joined, use & 1, dead)) break;
+        __syncwarp();
+        if (!warp_wait<true>(&B.joined, use & 1, dead, P.limit)) break;
         const uint64_t got = lane < size ? B.part[lane] : 0;
         pm = __uint_as_float((uint32_t)got);
         ps = __uint_as_float((uint32_t)(got >> 32));
@@ -791,10 +790,9 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       if (rank == 0 && lane == 0) P.loss[row] = loss * weight;
       __syncwarp();
     }
-    if (lane == 0 && *dead && P.status) atomicOr(P.status, (int)VINFER_ST_INTERNAL);
   } else {  // ---- the warps that sum and write
     const uint64_t scale2 = pair(P.scale, P.scale);
-    uint32_t it = 0, live = 0;  // chunks and rows so far
+    uint32_t live = 0;  // rows so far
     bool ok = true;
     while (ok && next_row(row, weight)) {
       T* out = static_cast<T*>(P.grad) + row * P.ldg;
@@ -815,10 +813,10 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       const int C = (v1 - v0 + CV - 1) / CV, again = max(C - SLOTS, 0);
       StepRow& B = S.row[live % LW];
       const uint32_t use = live++ / LW;
-      if (!(ok = bar_wait(&B.list_full, use & 1, dead))) break;
+      if (!(ok = warp_wait(&B.list_full, use & 1, dead, P.limit))) break;
       Exps sum(P.scale);
       for (int c = 0; c < C; ++c, ++it) {
-        if (!(ok = bar_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead))) break;
+        if (!(ok = warp_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead, P.limit))) break;
         const int v = v0 + c * CV;
         uint4* chunk = ring + (size_t)(it % SLOTS) * CV;
         if (!(v >= lo && v + CV <= end) || has_marks<CT, CU>(B.marks, c, w))
@@ -843,7 +841,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
         bar_arrive(&B.summed);
       }
       __syncwarp();
-      if (!(ok = bar_wait(&B.solved, use & 1, dead))) break;
+      if (!(ok = warp_wait(&B.solved, use & 1, dead, P.limit))) break;
       const uint64_t neg_m = pair(-B.m, -B.m), coef = pair(B.coef, B.coef);
       // the chunks the ring still holds, in order, then the others once more
       const int held = C - again;
@@ -851,7 +849,8 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       for (int k = 0; k < C; ++k) {
         const int c = k < held ? again + k : k - held;
         const uint32_t n = n0 + k;
-        if (k >= held && !(ok = bar_wait(&S.full[n % SLOTS], (n / SLOTS) & 1, dead))) break;
+        if (k >= held && !(ok = warp_wait(&S.full[n % SLOTS], (n / SLOTS) & 1, dead, P.limit)))
+          break;
         const int v = v0 + c * CV;
         uint4* chunk = ring + (size_t)(n % SLOTS) * CV;
         const bool inside = v >= lo && v + CV <= end;
@@ -890,7 +889,16 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       if (lane == 0) bar_arrive(&B.list_empty);
     }
   }
-  __syncwarp();
+  __syncthreads();
+  if (*dead) {  // a wait has given up, whichever and however late
+    if (tid == 0 && P.status) atomicOr(P.status, (int)VINFER_ST_INTERNAL);
+    if (w == CW && lane == 0)  // no copy of this CTA may land behind its end
+      for (uint32_t k = it > SLOTS ? it - SLOTS : 0; k < it; ++k) {
+        int none = 0;
+        bar_wait(&S.full[k % SLOTS], (k / SLOTS) & 1, &none, WAIT_LIMIT);
+      }
+    __syncwarp();
+  }
   if (size > 1) cluster_sync();  // no sum is sent to a CTA that has left
 }
 
@@ -926,6 +934,7 @@ DistP params(const VinferDistillArgs* a) {
   P.lp = a->logprobs;
   P.weights = a->weights;
   P.status = a->status;
+  P.limit = WAIT_LIMIT;
   return P;
 }
 
@@ -1070,6 +1079,12 @@ int vinfer_distill_grad(const VinferDistillArgs* a, const float* row_stats,
 
 int vinfer_distill_step(const VinferDistillArgs* a, float* loss, void* grad, int64_t ld_grad,
                         void* workspace, size_t workspace_bytes, void* stream) {
+  return vinfer_distill_step_within(a, loss, grad, ld_grad, workspace, workspace_bytes, -1, stream);
+}
+
+int vinfer_distill_step_within(const VinferDistillArgs* a, float* loss, void* grad, int64_t ld_grad,
+                               void* workspace, size_t workspace_bytes, int64_t wait_ns,
+                               void* stream) {
   NvtxRange nvtx_range("vinfer_distill_step");
   int rc = check(a);
   if (rc != VINFER_OK) return rc;
@@ -1078,6 +1093,11 @@ int vinfer_distill_step(const VinferDistillArgs* a, float* loss, void* grad, int
   if (workspace_bytes < vinfer_distill_workspace_bytes(a->rows, a->vocab, a->dtype, a->k))
     return VINFER_E_LIMIT;
   DistP P = params(a);
+  if (wait_ns >= 0) {  // at least one try; at most the usual number
+    P.limit.suspend_ns = (uint32_t)std::min<int64_t>(wait_ns, WAIT_LIMIT.suspend_ns);
+    P.limit.tries = (int32_t)std::min<int64_t>(
+        std::max<int64_t>(wait_ns / WAIT_LIMIT.suspend_ns, 1), WAIT_LIMIT.tries);
+  }
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   P.part = reinterpret_cast<Part*>(ws);
   ws += align_up((size_t)P.rows * P.parts * sizeof(Part));

@@ -388,37 +388,54 @@ __device__ __forceinline__ void bar_expect(uint64_t* b, uint32_t bytes) {
                "r"(bytes)
                : "memory");
 }
-// Each try may leave the warp suspended this long: a poll that came back at once would take issue
-// slots from the warps that compute.
-// A try may leave the warp suspended this long, and sleeps a little behind it: a warp that polled
-// would take issue slots from those that compute (512 -> 494 us for the distillation step).
-constexpr uint32_t SUSPEND_NS = 20000;
-// Waits for the phase of this parity to end; false after a bounded number of tries (0.1 to 5 s; the
-// waits here last microseconds), or once another wait of the CTA has given up: *dead is then set,
-// and every role leaves.
+// The limit of a wait: tries that may each leave the warp suspended for suspend_ns, and sleep a little
+// behind it: a warp that polled would take issue slots from those that compute (512 -> 494 us for the
+// distillation step).
+struct WaitLimit {
+  int32_t tries;
+  uint32_t suspend_ns;
+};
+constexpr WaitLimit WAIT_LIMIT = {1 << 18, 20000};  // 0.1 to 5 s; the waits here last microseconds
 // CLUSTER: what other CTAs of the cluster sent is seen behind it.
-template <bool CLUSTER = false>
-__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* dead) {
-  const uint32_t a = smem_addr(b);
-  for (int i = 0; i < 1 << 18; ++i) {
-    uint32_t done;
-    if (CLUSTER)
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(done)
-          : "r"(a), "r"(parity), "r"(SUSPEND_NS)
-          : "memory");
-    else
-      asm volatile(
-          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}"
-          : "=r"(done)
-          : "r"(a), "r"(parity), "r"(SUSPEND_NS)
-          : "memory");
-    if (done) return true;
+template <bool CLUSTER>
+__device__ __forceinline__ bool bar_try(uint64_t* b, uint32_t parity, uint32_t suspend_ns) {
+  uint32_t done;
+  if (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(b)), "r"(parity), "r"(suspend_ns)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_addr(b)), "r"(parity), "r"(suspend_ns)
+        : "memory");
+  return done;
+}
+// Waits for the phase of this parity to end; false when the limit is reached, or once another wait of
+// the CTA has given up: *dead is then set, and every role leaves. One thread's wait.
+__device__ __forceinline__ bool bar_wait(uint64_t* b, uint32_t parity, volatile int* dead,
+                                         WaitLimit limit) {
+  for (int i = 0; i < limit.tries; ++i) {
+    if (bar_try<false>(b, parity, limit.suspend_ns)) return true;
     if (*dead) return false;
+    __nanosleep(100);
+  }
+  *dead = 1;
+  return false;
+}
+// The same for a whole warp, whose lanes all get the same answer.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint64_t* b, uint32_t parity, volatile int* dead,
+                                          WaitLimit limit) {
+  for (int i = 0; i < limit.tries; ++i) {
+    if (__all_sync(FULL, bar_try<CLUSTER>(b, parity, limit.suspend_ns))) return true;
+    if (__any_sync(FULL, *dead)) return false;
     __nanosleep(100);
   }
   *dead = 1;
@@ -468,14 +485,15 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::
                    : "memory");
 }
-// Stores 8 bytes in another CTA's shared memory and counts them on its barrier.
+// Stores 8 bytes in another CTA's shared memory and arrives on its barrier. Both are done before this
+// thread's next cluster_sync() is (a copy that completes by itself might land behind it, in a CTA that
+// has left without waiting for it).
 __device__ __forceinline__ void send(void* dst, uint64_t* bar, uint32_t rank, uint64_t value) {
   uint32_t d, b;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(d) : "r"(smem_addr(dst)), "r"(rank));
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_addr(bar)), "r"(rank));
-  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(d),
-               "l"(value), "r"(b)
-               : "memory");
+  asm volatile("st.shared::cluster.b64 [%0], %1;" ::"r"(d), "l"(value) : "memory");
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(b) : "memory");
 }
 
 // The dependent kernel may take its place on the SMs now; it still waits for this grid's end.
