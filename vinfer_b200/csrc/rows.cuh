@@ -301,8 +301,12 @@ __device__ __forceinline__ double warp_sum(double v) {
 // A thread's sum while it streams: m is the largest element of its first round, and moves only when a
 // later one counts 16 times as much, so that exponents stay small and few rounds rescale: a
 // round costs an ex2 an element, and a multiply-add and an addition for each two. The argument
-// x * scale - c is rounded once, and what c misses of m * scale is put right in the round's sum.
+// x * scale - c is rounded once, and what c misses of m * scale (a small d) is put right in the round's
+// sum, by 2^-d - 1 taken as a series. From |c| = NEAR_ZERO on, where d is no longer small (2^-3 below
+// it), distances from m are formed first: they are exact there, since elements that count are within
+// a factor of two of m.
 struct Exps {
+  static constexpr float NEAR_ZERO = 4194304.f;  // 2^22
   float m, s;
   float c, fix;  // m * scale rounded, and what that does to a round's sum
   float scale;
@@ -316,10 +320,11 @@ struct Exps {
       if (s != 0.f) s *= ex2((m - mx) * scale);
       m = mx;
       c = m * scale;
-      fix = -fmaf(m, scale, -c) * (float)LN2_D;
+      const float y = -fmaf(m, scale, -c) * (float)LN2_D;  // e^y - 1; y^6 / 720 is left out, below 1e-9
+      fix = y * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.f / 120, 1.f / 24), 1.f / 6), 0.5f), 1.f);
     }
     float sum;
-    if (fabsf(c) < 1e37f) {
+    if (fabsf(c) < NEAR_ZERO) {
       const uint64_t k = pair(scale, scale), d = pair(-c, -c);
       uint64_t all = pair(0.f, 0.f);
 #pragma unroll
@@ -335,7 +340,7 @@ struct Exps {
       split(all, a, b);
       sum = a + b;
       sum = fmaf(sum, fix, sum);
-    } else {  // c near the float's range, or infinite: distances first
+    } else {  // distances first
       sum = 0.f;
 #pragma unroll 1
       for (int u = 0; u < U; ++u) {
