@@ -219,8 +219,8 @@ int vinfer_sample_decode(const VinferSampleArgs* args, int32_t* hist_len, int32_
  *    beams * (1 + n_eos) always finds every continuation. next_scores may be the scores array.
  *  - A score that is NaN or +inf sets VINFER_ST_BAD_SCORE, a live row whose logits hold a NaN or
  *    +inf or nothing above -inf VINFER_ST_NONFINITE; such a beam has no candidates.
- * The order is that of exact scores: scores closer than 2e-6 are compared with sums
- * taken in double.
+ * The order is that of exact scores: scores too close for their streamed sums (2.5e-6) are
+ * compared with sums taken in double.
  * The workspace needs no initialisation, holds nothing between calls and serves one call at a
  * time; 16-byte aligned. requests * beams <= VINFER_MAX_BATCH. */
 #define VINFER_BEAM_MAX_WIDTH 32

@@ -15,8 +15,8 @@
 //
 // What bounds it: reading the logits once, then the instructions of the exponentials (8 an element
 // with all overheads; the ex2 unit alone is half busy). Measured on one B200, us a step: 32
-// requests of 16 beams, 248,320 float32 logits 96.2 (508 MB: 5.3 TB/s, 0.81 of the measured copy
-// bandwidth); 64 of 4, 151,936 bf16 28.5 (77.8 MB: 0.42); one of 4 9.8, most of it the two kernels'
+// requests of 16 beams, 248,320 float32 logits 98.1 (508 MB: 5.2 TB/s, 0.79 of the measured copy
+// bandwidth); 64 of 4, 151,936 bf16 29.0 (77.8 MB: 0.41); one of 4 10.0, most of it the two kernels'
 // latency. Selecting costs little because it is not sorting: a part of a row finds a bar that n of
 // its elements reach from its lanes' maxima, and looks again only at the 16-vector rounds of the
 // threads that reach it (keeping the vectors themselves in shared memory cost 3 us more of 32).
@@ -36,11 +36,18 @@ constexpr int MAX_JOIN = 1024;    // entries of a beam's parts together (a warp 
 constexpr int MAX_STAGED = 8192;  // entries of a request's parts together (64 KiB staged)
 constexpr int PT = 512, PW = PT / 32;  // threads of k_beam_pick
 constexpr int MAXN = VINFER_BEAM_MAX_N, MAXW = VINFER_BEAM_MAX_WIDTH;
-// Scores of different beams within this distance are compared with sums taken in double. A streamed
-// log-sum is off by at most 6e-7 (1.2e-7 root mean square) over 66,000 rows of 1,000 to 248,320 float32
-// and bf16 logits of five distributions: mostly the argument's rounding and ex2 on the few tokens
-// that hold the mass.
-constexpr double NEAR = 2e-6;
+// Scores of different beams within this distance are compared with sums taken again in double. A streamed
+// sum is off, relative to itself and in units of 2^-24, by at most
+//   4    ex2 (2^-22, the instruction's bound),
+//   5.7  an exponent's argument, rounded once: half a step at 8 to 16 below the thread's reference;
+//        farther down a thread has at most 2^10 elements, 2^-6 of its sum,
+//   8    the additions within a round (3 + 3 + 1, and the correction); everything behind it is in double,
+//   0.5  the correction's own rounding,
+// so two sums differ by at most 36.4 of these from what they should. log2(e) as a float stretches all
+// exponents alike, by 1.4e-8 of them; a sum's mean exponent is at most its log2(V) = 18, another 2.8. In
+// all 2.4e-6. (Rounds added in float, one chain of 61 for a row of 248,320: scores off by 3.7e-6
+// either way, seen with 256 tokens raised above a constant rest.)
+constexpr double NEAR = 2.5e-6;
 
 static_assert(MAXN <= 128 && MAXW <= 32, "lists fit the picking kernel's shared memory");
 
@@ -54,8 +61,9 @@ __device__ __forceinline__ float entry_x(u64 e) { return from_okey(~(uint32_t)(e
 __device__ __forceinline__ int entry_id(u64 e) { return (int)(uint32_t)e; }
 
 struct PartHdr {
-  float m, s;  // softmax sum of the part, (m, s) at scale L2E
-  int pad[2];
+  double s;    // softmax sum of the part, (m, s) at scale L2E
+  float m;
+  int pad;
 };
 
 struct RowsP {
@@ -77,7 +85,8 @@ struct Delegates {         // dynamic shared memory of k_beam_rows
 };
 struct RowsS {
   u64 best[MAXN];
-  float f[2 * NW];
+  double sum[NW];
+  float f[NW];
   float kth[NW];
   int cnt, got, nd;
   uint32_t hist[256];
@@ -251,7 +260,7 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
   // the warps' k-th largest lane maxima (8k >= n). A thread's round below it holds none of the n
   // best; the others (about 3n in the first round) are noted as delegates. The warps raise it as
   // their maxima rise; a warp that still sees an older, lower one notes a few more.
-  Exps sum(L2E);
+  Exps<double> sum(L2E);
   float seen = neg_inf();  // this lane's largest element so far
   const int k = (n + NW - 1) / NW;
   volatile float* kth = S.kth;
@@ -332,8 +341,8 @@ __global__ void __launch_bounds__(NT, 4) k_beam_rows(const RowsP P) {
     if (rank < n) out[rank] = e;
   }
   for (int i = have + tid; i < n; i += NT) out[i] = NONE;
-  block_join<NW>(sum.m, sum.s, L2E, S.f);
-  if (tid == 0) P.hdr[at] = PartHdr{sum.m, sum.s, {0, 0}};
+  block_join<NW>(sum.m, sum.s, L2E, S.sum, S.f);
+  if (tid == 0) P.hdr[at] = PartHdr{sum.s, sum.m, 0};
 }
 
 struct PickP {
@@ -412,7 +421,8 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
   for (int i = tid; i < W * per; i += PT) copy_async8(staged + i, E + i);  // dead beams': whatever is there
   for (int beam = w; beam < W; beam += PW) {
     const PartHdr* H = P.hdr + ((int64_t)req * W + beam) * P.parts;
-    float m = neg_inf(), m2 = neg_inf(), s0 = 0, s1 = 0;  // MAX_PARTS is two a lane
+    float m = neg_inf(), m2 = neg_inf();  // MAX_PARTS is two a lane
+    double s0 = 0, s1 = 0;
     if (lane < P.parts) {
       m = H[lane].m;
       s0 = H[lane].s;
@@ -422,10 +432,9 @@ __global__ void __launch_bounds__(PT, 1) k_beam_pick(const PickP Q) {
       s1 = H[lane + 32].s;
     }
     const float top = warp_max(fmaxf(m, m2));
-    // in double: the sum of at most 64 floats, each scaled by a power of two
     double s = 0;
-    if (s0 != 0.f) s += (double)s0 * exp2(((double)m - (double)top) * (double)L2E);
-    if (s1 != 0.f) s += (double)s1 * exp2(((double)m2 - (double)top) * (double)L2E);
+    if (s0 != 0) s += s0 * exp2(((double)m - (double)top) * (double)L2E);
+    if (s1 != 0) s += s1 * exp2(((double)m2 - (double)top) * (double)L2E);
     s = warp_sum(s);
     if (lane == 0) {
       S.m[beam] = top;

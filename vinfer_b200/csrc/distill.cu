@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(NT, 4) k_distill_rows(const DistP P) {
     }
   }
   __syncthreads();
-  Exps sum(P.scale);
+  Exps<float> sum(P.scale);
   stream_rounds<RU, NT, BUFS>(R, v0, v1, [&](uint4 (&q)[RU], int vb) {
     uint32_t word[RU];
     if (marks_of<NT, RU>(marked, (vb - v0) / (NT * RU), tid / 32, word)) {
@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       StepRow& B = S.row[live % LW];
       const uint32_t use = live++ / LW;
       if (!(ok = warp_wait(&B.list_full, use & 1, dead, P.limit))) break;
-      Exps sum(P.scale);
+      Exps<float> sum(P.scale);
       for (int c = 0; c < C; ++c, ++it) {
         if (!(ok = warp_wait(&S.full[it % SLOTS], (it / SLOTS) & 1, dead, P.limit))) break;
         const int v = v0 + c * CV;
