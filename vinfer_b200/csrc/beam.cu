@@ -92,7 +92,7 @@ struct RowsS {
   uint32_t hist[256];
   uint32_t bin, before;
 };
-__host__ __device__ inline int list_cap(int n, int A) { return U * A * n + 2 * n + 64; }
+__host__ __device__ constexpr int list_cap(int n, int A) { return U * A * n + 2 * n + 64; }
 
 // The n smallest of list[0, L) into best (any order); L > n. Radix select by bytes: keys are
 // unique, so it ends with exactly n.
@@ -652,6 +652,10 @@ int beam_parts(int64_t rows_, int W, int64_t vocab, int dtype, int n) {
 size_t pick_smem(int W, int n, int parts) {
   return (size_t)W * n * (8 * (size_t)parts + 8 + 8 + 8);
 }
+// the most of both kernels: the longest lists, and MAX_STAGED entries beside lists of all beams
+constexpr size_t ROWS_SMEM = std::max(sizeof(Delegates), (size_t)list_cap(MAXN, 8) * 8);
+constexpr size_t PICK_SMEM = 8 * (size_t)MAX_STAGED + (size_t)MAXW * MAXN * 24;
+static_assert(MAX_STAGED >= MAXW * MAXN && PICK_SMEM <= 220 * 1024, "every request fits an SM");
 
 bool beam_shape_ok(int64_t requests, int32_t beams, int64_t vocab, int32_t dtype, int32_t n) {
   return requests >= 1 && beams >= 1 && beams <= MAXW && vocab >= 1 && vocab <= VINFER_MAX_VOCAB &&
@@ -664,7 +668,7 @@ int launch_beam(const PickP& Q, int64_t requests, cudaStream_t st) {
   const int64_t rows_ = requests * Q.W;
   const size_t sm_rows = std::max(sizeof(Delegates), (size_t)list_cap(Q.r.n, Vec<T>::A) * 8);
   const size_t sm_pick = pick_smem(Q.W, Q.r.n, Q.r.parts);
-  if (opt_in(k_beam_rows<T>, sm_rows) != VINFER_OK || opt_in(k_beam_pick<T>, sm_pick) != VINFER_OK)
+  if (opt_in<k_beam_rows<T>>(ROWS_SMEM) != VINFER_OK || opt_in<k_beam_pick<T>>(PICK_SMEM) != VINFER_OK)
     return VINFER_E_CUDA;
   const int rc = launch(k_beam_rows<T>, (unsigned)(rows_ * Q.r.parts), NT, sm_rows, st, false, 1, Q.r);
   if (rc != VINFER_OK) return rc;

@@ -1001,7 +1001,7 @@ int step_clusters(int c, int* clusters) {
 template <typename T>
 int launch_step(const DistP& P, cudaStream_t st) {
   const int c = step_cluster(P.V, Vec<T>::A);
-  if (opt_in(k_distill_step<T>, STEP_SMEM) != VINFER_OK) return VINFER_E_CUDA;
+  if (opt_in<k_distill_step<T>>(STEP_SMEM) != VINFER_OK) return VINFER_E_CUDA;
   int clusters = 0;
   if (step_clusters<T>(c, &clusters) != VINFER_OK) return VINFER_E_CUDA;
   return launch(k_distill_step<T>, (unsigned)(std::min<int64_t>(P.rows, clusters) * c), STEP_T,

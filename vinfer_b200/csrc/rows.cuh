@@ -8,6 +8,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include <nvtx3/nvToolsExt.h>
 
 #include "vinfer_sampler.h"
@@ -576,12 +578,19 @@ inline int result(cudaError_t e) {
   return VINFER_E_CUDA;
 }
 
-// Shared memory above 48 KB, static included (below 4 KB here), has to be asked for (a host-side
-// setting of the kernel on the current device, no work on a stream).
-template <typename K>
-int opt_in(K kern, size_t smem) {
-  if (smem <= 44 * 1024) return VINFER_OK;
-  return result(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+// Shared memory above 48 KB has to be asked for (a host-side setting of the kernel on the current
+// device, no work on a stream): the most that any launch of KERN takes, once for each device. A call
+// that asked for its own need would lower the limit under another thread's launch.
+template <auto KERN>
+int opt_in(size_t most) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (result(cudaGetDevice(&dev)) != VINFER_OK || dev < 0 || dev >= 64) return VINFER_E_CUDA;
+  if (done[dev].load(std::memory_order_acquire)) return VINFER_OK;
+  const int rc =
+      result(cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most));
+  if (rc == VINFER_OK) done[dev].store(true, std::memory_order_release);
+  return rc;
 }
 
 // One launch, of clusters of `cluster` CTAs; `dependent`: may begin while the stream's kernel before

@@ -293,7 +293,7 @@ extern "C" int vinfer_reorder_states(const VinferState* states, int32_t n_states
     // every slot may move: no more CTAs than items, at most what is resident
     const int64_t grid = std::min<int64_t>(148 * CTAS, chunks * slots);
     const size_t smem = (size_t)slots * 8 + 4;
-    if (opt_in(k_reorder, smem) != VINFER_OK) return VINFER_E_CUDA;
+    if (opt_in<k_reorder>(VINFER_STATE_MAX_SLOTS * 8 + 4) != VINFER_OK) return VINFER_E_CUDA;
     const int rc = launch(k_reorder, (unsigned)grid, NT, smem, (cudaStream_t)stream, false, 1, P);
     if (rc != VINFER_OK) return rc;
   }
