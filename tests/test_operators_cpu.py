@@ -8,8 +8,10 @@ import pytest
 import torch
 
 from vinfer_b200 import _lib
+from vinfer_b200.beam import BeamSearch
 from vinfer_b200.build import build
 from vinfer_b200.kernels.sampler.b200 import B200Sampler
+from vinfer_b200.sampling import DecodeStates
 
 
 @pytest.fixture(scope="module")
@@ -32,3 +34,40 @@ def test_the_step_with_a_limit_refuses_as_the_step_does(backend):
     d.dtype, d.k, d.rows, d.vocab, d.ld, d.temperature = 0, 4, 2, 10, 10, 1.0
     assert f(C.byref(d), 16, 16, 9, 16, 1 << 30, 0, None) == _lib.E_ARG
     assert f(C.byref(d), 16, 16, 10, 16, 8, 0, None) == _lib.E_LIMIT
+
+
+# ---- the search ----------------------------------------------------------------------------------
+class Untouched:
+    """Stands for a search's state: all that a refused step must leave as it was."""
+
+    def __init__(self, search):
+        self.search = search
+        self.before = {k: v.clone() if torch.is_tensor(v) else v for k, v in vars(search).items()
+                       if torch.is_tensor(v) or isinstance(v, int)}
+
+    def check(self):
+        for k, v in self.before.items():
+            now = getattr(self.search, k)
+            assert torch.equal(now, v) if torch.is_tensor(v) else now == v, k
+
+
+@pytest.mark.parametrize("lengths", [
+    torch.zeros(4, dtype=torch.int64), torch.zeros(3, dtype=torch.int32), [1, 1, 1, 1],
+    torch.zeros(8, dtype=torch.int32)[::2], torch.zeros(4, dtype=torch.int32, device="meta")],
+    ids=["int64", "three slots", "a list", "strided", "elsewhere"])
+def test_a_step_with_wrong_lengths_changes_nothing(backend, lengths):
+    launched = []
+
+    class Recorder(B200Sampler):
+        def beam_select(self, *a, **k):
+            launched.append("beam_select")
+            raise AssertionError("launched")
+
+    b = object.__new__(Recorder)
+    vars(b).update(vars(backend))
+    search = BeamSearch(b, 2, 2, 3, states=[DecodeStates([torch.zeros(4, 3, 5)], length_dim=1)])
+    kept = Untouched(search)
+    with pytest.raises((ValueError, TypeError)):
+        search.step(torch.zeros(4, 10), lengths)
+    assert not launched
+    kept.check()

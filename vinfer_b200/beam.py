@@ -90,8 +90,10 @@ class BeamSearch:
         ``lengths`` (int32 ``[R * W]``): the positions of the states that hold data."""
         if self.steps >= self.max_tokens:
             raise ValueError(f"the search has taken its {self.max_tokens} tokens")
-        if lengths is None and any(s.has_lengths for s in self.states):
-            raise ValueError("states with a length_dim need lengths")
+        if any(s.has_lengths for s in self.states):  # before anything of the search changes
+            if lengths is None:
+                raise ValueError("states with a length_dim need lengths")
+            self.backend._slot_values("lengths", lengths, self.requests * self.width)
         b = self.backend.beam_select(logits, self.scores, self.n, eos=self.eos, out=self.out)
         self.steps += 1
         if self.eos is not None:

@@ -297,6 +297,13 @@ class B200Sampler:
                    nbytes)
         return out
 
+    def _slot_values(self, name: str, t: torch.Tensor, slots: int) -> None:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t.dtype != torch.int32 or t.numel() != slots or not t.is_contiguous() or \
+                t.device != self.device:
+            raise ValueError(f"{name} must be a contiguous int32 of {slots} slots on {self.device}")
+
     def reorder_states(self, states: DecodeStates, parents: torch.Tensor,
                        lengths: torch.Tensor | None = None) -> None:
         """Slot ``s`` of every state takes the contents of slot ``parents[s]`` (int32, one for each
@@ -306,11 +313,9 @@ class B200Sampler:
         out of range, or one that moves itself, leaves the slot alone and sets a status bit."""
         if states.device != self.device:
             raise ValueError(f"states are on {states.device}, backend on {self.device}")
-        for name, t in (("parents", parents), ("lengths", lengths)):
-            if t is not None and (t.dtype != torch.int32 or t.numel() != states.slots
-                                  or not t.is_contiguous() or t.device != self.device):
-                raise ValueError(f"{name} must be a contiguous int32 of {states.slots} slots on "
-                                 f"{self.device}")
+        self._slot_values("parents", parents, states.slots)
+        if lengths is not None:
+            self._slot_values("lengths", lengths, states.slots)
         if (lengths is not None) != states.has_lengths:
             raise ValueError("lengths and a length_dim of the states go together")
         if states.count == 0:
