@@ -71,3 +71,12 @@ def test_a_step_with_wrong_lengths_changes_nothing(backend, lengths):
         search.step(torch.zeros(4, 10), lengths)
     assert not launched
     kept.check()
+
+
+def test_a_search_refuses_what_its_steps_would(backend):
+    """Found when the search is made, not by the first step after it has replaced the scores."""
+    with pytest.raises(ValueError, match="states are on meta"):
+        BeamSearch(backend, 2, 2, 3, states=[DecodeStates([torch.zeros(4, 3, device="meta")])])
+    with pytest.raises(ValueError, match="stop ids"):
+        BeamSearch(backend, 1, 1, 3, eos=range(17))
+    BeamSearch(backend, 1, 1, 3, eos=range(16))

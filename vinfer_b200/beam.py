@@ -41,6 +41,8 @@ class BeamSearch:
         if not 1 <= width <= _lib.BEAM_MAX_WIDTH:
             raise ValueError(f"width must be in [1, {_lib.BEAM_MAX_WIDTH}], got {width}")
         eos = sorted(set(eos))
+        if len(eos) > _lib.BEAM_MAX_EOS:
+            raise ValueError(f"at most {_lib.BEAM_MAX_EOS} stop ids are supported, got {len(eos)}")
         if width * (1 + len(eos)) > _lib.BEAM_MAX_N:
             raise ValueError(f"width * (1 + stop ids) must be at most {_lib.BEAM_MAX_N}")
         for s in states:
@@ -48,6 +50,8 @@ class BeamSearch:
                 raise ValueError(f"states have {s.slots} slots for {requests} * {width} beams")
             if not s.in_place:
                 raise ValueError("the states that follow the beams are copied in place, without out")
+            if s.device != backend.device:
+                raise ValueError(f"states are on {s.device}, backend on {backend.device}")
         self.backend, self.requests, self.width = backend, requests, width
         self.max_tokens, self.length_penalty, self.states = max_tokens, length_penalty, list(states)
         dev = backend.device
