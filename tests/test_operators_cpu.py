@@ -80,3 +80,15 @@ def test_a_search_refuses_what_its_steps_would(backend):
     with pytest.raises(ValueError, match="stop ids"):
         BeamSearch(backend, 1, 1, 3, eos=range(17))
     BeamSearch(backend, 1, 1, 3, eos=range(16))
+
+
+@pytest.mark.parametrize("w,stops", [(32, 4), (16, 8), (1, 16)])
+def test_the_default_number_of_candidates_finds_all_beams_or_is_refused(backend, w, stops):
+    """n = W * (1 + stop ids) always holds W that do not end; 128 of them where that is more would not."""
+    call = dict(logits=torch.zeros(w, 300), scores=torch.zeros(1, w),
+                eos=torch.zeros(stops, dtype=torch.int32))
+    if w * (1 + stops) > _lib.BEAM_MAX_N:
+        with pytest.raises(ValueError, match="n must be given"):
+            backend.beam_select(**call)
+    with pytest.raises(TypeError):  # past the checks: there is no launch here
+        backend.beam_select(**call, n=100)

@@ -255,8 +255,9 @@ class B200Sampler:
         vocabulary (descending score; ties by beam, then token) and lays the W best that do not
         end in one of ``eos`` (int32 stop ids on the device) into its slots: the best child of a
         beam stays in the beam's slot, so ``reorder_states`` only copies the others. ``n``
-        defaults to ``W * (1 + len(eos))``, which always finds W. ``out.next_scores`` may be
-        ``scores``. Nothing leaves the device."""
+        defaults to ``W * (1 + len(eos))``, which always finds W; where that exceeds 128 it has to
+        be given, and with fewer a slot may go without a beam although one was left.
+        ``out.next_scores`` may be ``scores``. Nothing leaves the device."""
         rows, v, ld = self._rows(logits)
         if scores.dim() != 2 or scores.shape[0] * scores.shape[1] != rows:
             raise ValueError(f"scores must be [requests, beams] for {rows} rows of logits")
@@ -269,7 +270,10 @@ class B200Sampler:
         if stops > _lib.BEAM_MAX_EOS:
             raise ValueError(f"at most {_lib.BEAM_MAX_EOS} stop ids are supported, got {stops}")
         if n is None:
-            n = min(w * (1 + stops), _lib.BEAM_MAX_N)
+            n = w * (1 + stops)
+            if n > _lib.BEAM_MAX_N:
+                raise ValueError(f"n must be given for {w} beams and {stops} stop ids: the {n} that "
+                                 f"always find {w} beams are more than {_lib.BEAM_MAX_N}")
         if not 1 <= n <= _lib.BEAM_MAX_N:
             raise ValueError(f"n must be in [1, {_lib.BEAM_MAX_N}], got {n}")
         a = _lib.BeamArgs()
