@@ -92,3 +92,32 @@ def test_the_default_number_of_candidates_finds_all_beams_or_is_refused(backend,
             backend.beam_select(**call)
     with pytest.raises(TypeError):  # past the checks: there is no launch here
         backend.beam_select(**call, n=100)
+
+
+@pytest.mark.parametrize("penalty", [-2.0, -1.0, 0.0, 0.6, 1.0])
+def test_settled_means_that_no_beam_enters_any_more(backend, penalty):
+    """Against finish(), now or after any further steps of a beam (its score only falls)."""
+    R, W, T, steps = 400, 2, 9, 2
+    g = torch.Generator().manual_seed(3)
+
+    def search(live, at):
+        s = BeamSearch(backend, R, W, T, length_penalty=penalty)
+        s.steps = at
+        s.scores.copy_(live)
+        s.done_scores.copy_(done)
+        s.done_lengths.fill_(1)
+        return s
+
+    done = (-8 * torch.rand(R, W, generator=g)).sort(descending=True).values
+    live = -6 * torch.rand(R, W, generator=g)
+    if penalty == -1.0:
+        done[0], live[0] = torch.tensor([-1.0, -7.0]), torch.tensor([-3.0, -9.0])  # -3 counts -6 now
+    settled = search(live, steps).settled()
+    assert settled.any() and not settled.all()
+    for at in range(steps, T + 1):
+        got = search(live, at).finish()
+        for r in range(R):
+            if settled[r]:
+                assert [v for v, _ in got[r]] == done[r].tolist(), (r, at)
+    if penalty < 0:
+        assert not settled[0] or penalty != -1.0

@@ -117,8 +117,9 @@ class BeamSearch:
 
     def settled(self) -> torch.Tensor:
         """Whether each request's worst kept hypothesis is better than its best beam could become
-        (bool ``[R]`` on the device): every further token lowers a beam's log-probability."""
-        last = self.max_tokens if self.length_penalty > 0 else self.steps + 1
+        (bool ``[R]`` on the device): every further token lowers a beam's log-probability, and
+        its length counts for it with a positive penalty, against it with a negative one."""
+        last = self.max_tokens if self.length_penalty > 0 else max(1, self.steps)
         bound = self.scores.amax(1) / last ** self.length_penalty
         return self.done_scores[:, -1] >= bound
 
