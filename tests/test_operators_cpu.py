@@ -112,6 +112,7 @@ def test_settled_means_that_no_beam_enters_any_more(backend, penalty):
     live = -6 * torch.rand(R, W, generator=g)
     if penalty == -1.0:
         done[0], live[0] = torch.tensor([-1.0, -7.0]), torch.tensor([-3.0, -9.0])  # -3 counts -6 now
+    done[1], live[1] = torch.tensor([-0.1, -0.2]), torch.tensor([-5.0, -6.0])  # at any penalty here
     settled = search(live, steps).settled()
     assert settled.any() and not settled.all()
     for at in range(steps, T + 1):
@@ -119,5 +120,4 @@ def test_settled_means_that_no_beam_enters_any_more(backend, penalty):
         for r in range(R):
             if settled[r]:
                 assert [v for v, _ in got[r]] == done[r].tolist(), (r, at)
-    if penalty < 0:
-        assert not settled[0] or penalty != -1.0
+    assert settled[1] and not (penalty == -1.0 and settled[0])
