@@ -259,6 +259,8 @@ int vinfer_beam_select(const VinferBeamArgs* args, void* workspace, size_t works
  *    slot alone; any other parent must keep its own state (parents[parents[s]] == parents[s], as
  *    vinfer_beam_select lays beams out), else the slot is left alone and VINFER_ST_BAD_PARENT set.
  *  - Into another buffer (which must not overlap the source): every slot is copied, from any parent.
+ *  - Neither parents nor lengths lie in memory that is written, no two destinations share a byte, and
+ *    states copied in place share bytes of the same slot alone.
  *  - lengths (device int32 [slots]) with len_unit_bytes > 0 copies only the first lengths[s]
  *    positions (of len_unit_bytes each) of every run, with len_outer >= 0 only the first lengths[s]
  *    indices of that outer dimension; positions behind them are neither read nor written.

@@ -121,3 +121,66 @@ def test_settled_means_that_no_beam_enters_any_more(backend, penalty):
             if settled[r]:
                 assert [v for v, _ in got[r]] == done[r].tolist(), (r, at)
     assert settled[1] and not (penalty == -1.0 and settled[0])
+
+
+# ---- tensors that share memory -------------------------------------------------------------------
+def test_states_in_place_must_not_share_memory_across_slots():
+    """A slot read through one tensor and written through another: which comes first is not said."""
+    buf = torch.zeros(6, 8)
+    with pytest.raises(ValueError, match="state 1 overlaps state 0"):
+        DecodeStates([buf[:5], buf[1:]])                       # shifted by a slot
+    sq = torch.zeros(4, 4)
+    with pytest.raises(ValueError, match="state 1 overlaps state 0"):
+        DecodeStates([sq, sq.t()])                             # the slots of one are positions of the other
+    flat = torch.zeros(64)
+    with pytest.raises(ValueError, match="state 2 overlaps state 0"):
+        DecodeStates([flat[:32].view(4, 8), torch.zeros(4, 3), flat[28:60].view(4, 8)])
+    with pytest.raises(ValueError, match="state 1 overlaps state 0"):
+        DecodeStates([flat[:32].view(4, 8), flat[:16].view(4, 4)])  # other strides
+    # no shared element, or the same bytes of the same slot
+    kv = torch.zeros(4, 2, 3, 5)
+    DecodeStates([kv[:, 0], kv[:, 1]])
+    layers = torch.zeros(3, 2, 4, 5)
+    DecodeStates([layers[:, 0], layers[:, 1]], slot_dim=1)
+    packed = torch.zeros(4, 20)
+    DecodeStates([packed[:, :7], packed[:, 7:12].view(4, 5, 1), packed[:, 12:]])
+    DecodeStates([packed, packed[:, 3:9], packed])
+    last = torch.zeros(5, 2, 8)
+    DecodeStates([last[:, 0], last[:, 1]], slot_dim=1)
+
+
+def test_outputs_must_not_share_memory():
+    t, u = torch.zeros(4, 8), torch.zeros(4, 8)
+    buf = torch.zeros(5, 8)
+    with pytest.raises(ValueError, match="output 1 overlaps output 0"):
+        DecodeStates([t, u], out=[buf[:4], buf[1:]])
+    with pytest.raises(ValueError, match="output 0 overlaps a state"):
+        DecodeStates([buf[:4]], out=[buf[1:]])
+    # side by side in one buffer, states and outputs too
+    both = torch.zeros(4, 3, 8)
+    DecodeStates([both[:, 0]], out=[both[:, 2]])
+    DecodeStates([t, u], out=[both[:, 0], both[:, 1]])
+
+
+def test_reordering_refuses_what_it_would_write(backend):
+    """Parents and lengths that lie in the states are read while the states change."""
+    counts = torch.zeros(4, 3, dtype=torch.int32)
+    flat = counts.view(-1)
+    with pytest.raises(ValueError, match="parents must not lie in the states"):
+        backend.reorder_states(DecodeStates([torch.zeros(4, 2), counts]), flat[2:6])
+    st = DecodeStates([counts.view(4, 3, 1)], length_dim=1)
+    with pytest.raises(ValueError, match="lengths must not lie in the states"):
+        backend.reorder_states(st, torch.zeros(4, dtype=torch.int32), flat[8:])
+    out = torch.zeros(4, 3, dtype=torch.int32)
+    with pytest.raises(ValueError, match="parents must not lie in the states"):
+        backend.reorder_states(DecodeStates([counts], out=[out]), out.view(-1)[:4])
+
+
+def test_a_gradient_may_lie_between_the_logits(backend):
+    ids, lp = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3, 2)
+    buf = torch.zeros(3, 20)
+    for out in (buf[:, 9:19], buf[:, 5:15]):
+        with pytest.raises(ValueError, match="not overlap"):
+            backend.distill_step(buf[:, :10], ids, lp, out=out)
+    with pytest.raises(TypeError):  # past the checks: there is no launch here
+        backend.distill_step(buf[:, :10], ids, lp, out=buf[:, 10:])

@@ -324,9 +324,13 @@ class B200Sampler:
             raise ValueError("lengths and a length_dim of the states go together")
         if states.count == 0:
             return
+        at, held, nbytes = parents.data_ptr(), _ptr(lengths), 4 * states.slots
+        if states.writes_to(at, at + nbytes):
+            raise ValueError("parents must not lie in the states that are written")
+        if held is not None and states.writes_to(held, held + nbytes):
+            raise ValueError("lengths must not lie in the states that are written")
         self._call(self.lib.vinfer_reorder_states, "vinfer_reorder_states", states.array,
-                   states.count, parents.data_ptr(), states.slots, _ptr(lengths),
-                   self.status.data_ptr())
+                   states.count, at, states.slots, held, self.status.data_ptr())
 
     # ---- distillation ---------------------------------------------------------------------------
     def _distill_args(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,

@@ -10,6 +10,7 @@ is reproducible from ``(seed, position)`` alone, as in the reference.
 
 from __future__ import annotations
 
+import bisect
 import hashlib
 from collections.abc import Sequence
 from dataclasses import dataclass
@@ -281,7 +282,9 @@ class DecodeStates:
     ``[slots, heads, length, dim]``, recurrent states, token counts, in any strided layout
     without overlap). ``length_dim``, if given, is the dimension along which a call's ``lengths``
     say how many positions of a slot hold data. ``out`` are the tensors that receive the copies
-    (same shapes and types, any strides); without it slots are copied in place. The tensors are
+    (same shapes and types, any strides; they share no element with each other or a state);
+    without it slots are copied in place, and tensors may share bytes of the same slot alone. The
+    tensors are
     held and their addresses used by every call: they are not to be resized meanwhile. They
     play the role of vinfer's per-request state slots (``src/vinfer/state/pool.py:70-131``).
     """
@@ -319,9 +322,28 @@ class DecodeStates:
                 raise ValueError(f"output {i} is given twice")
             if t.numel():
                 found.append(_describe(i, t, u, sd, ld))
+        for i, j in _close_pairs(self.out):
+            if out is not None and _overlap(self.out[i], self.out[j]):
+                raise ValueError(f"output {j} overlaps output {i}")
+            if out is None and _overlap_across(self.out[i], self.out[j], slot_dim):
+                raise ValueError(f"state {j} overlaps state {i}")
+        # where slots are written: (first byte, behind the last), ascending, without overlap
+        self.written: list[list[int]] = []
+        for a, b in sorted((u.data_ptr(), u.data_ptr() + _extent(u)) for u in self.out if u.numel()):
+            if self.written and a <= self.written[-1][1]:
+                self.written[-1][1] = max(b, self.written[-1][1])
+            else:
+                self.written.append([a, b])
         self.count = len(found)
         self.in_place = all(d.src == d.dst for d in found)
         self.array = (_lib.State * max(1, self.count))(*found)
+
+    def writes_to(self, a: int, b: int) -> bool:
+        """Whether slots are written within the bytes [a, b)."""
+        if not self.written or b <= self.written[0][0] or a >= self.written[-1][1]:
+            return False
+        i = bisect.bisect_left(self.written, [b])  # the spans that begin below b
+        return i > 0 and self.written[i - 1][1] > a
 
     @staticmethod
     def _dim(t: torch.Tensor, dim: int, name: str) -> tuple[int, int]:
@@ -336,10 +358,82 @@ def _extent(t: torch.Tensor) -> int:
 
 
 def _overlap(t: torch.Tensor, u: torch.Tensor) -> bool:
-    if not t.numel():
+    """Whether two tensors share a byte (True also where finding out would take thousands of steps)."""
+    if not t.numel() or not u.numel():
         return False
     a, b = t.data_ptr(), u.data_ptr()
-    return a < b + _extent(u) and b < a + _extent(t)
+    if a >= b + _extent(u) or b >= a + _extent(t):
+        return False
+    return _meet(b - a, *_nested(t), *_nested(u))
+
+
+def _overlap_across(t: torch.Tensor, u: torch.Tensor, slot_dim: int) -> bool:
+    """Whether a slot of one tensor shares a byte with another slot of the other. (The same slot's bytes
+    are copied from the same place by both.)"""
+    if not _overlap(t, u):
+        return False
+    step = t.stride(slot_dim) * t.element_size()
+    if t.shape[slot_dim] > 1 and step != u.stride(slot_dim) * u.element_size():
+        return True
+    d = u.data_ptr() - t.data_ptr()
+    a, b = _nested(t.select(slot_dim, 0)), _nested(u.select(slot_dim, 0))
+    return any(_meet(d + k * step, *a, *b) or _meet(d - k * step, *a, *b)
+               for k in range(1, t.shape[slot_dim]))
+
+
+def _close_pairs(tensors: Sequence[torch.Tensor]) -> list[tuple[int, int]]:
+    """The pairs (i < j) of tensors whose extents overlap."""
+    spans = sorted((t.data_ptr(), t.data_ptr() + _extent(t), i) for i, t in enumerate(tensors)
+                   if t.numel())
+    pairs, open_ = [], []
+    for a, b, j in spans:
+        open_ = [(end, i) for end, i in open_ if end > a]
+        pairs += [(min(i, j), max(i, j)) for _, i in open_]
+        open_.append((b, j))
+    return sorted(pairs)
+
+
+def _nested(t: torch.Tensor) -> tuple[list[tuple[int, int]], int]:
+    """A tensor's dimensions (size, stride in bytes), outermost first, over its contiguous run of
+    bytes."""
+    run, dims = t.element_size(), []
+    for s, n in sorted((s * t.element_size(), n) for n, s in zip(t.shape, t.stride()) if n > 1 and s):
+        if not dims and s == run:
+            run *= n
+        elif dims and s == dims[-1][0] * dims[-1][1]:
+            dims[-1] = (dims[-1][0] * n, dims[-1][1])
+        else:
+            dims.append((n, s))
+    return dims[::-1], run
+
+
+def _meet(d: int, a: list[tuple[int, int]], ra: int, b: list[tuple[int, int]], rb: int) -> bool:
+    """Whether two tensors, the second's first byte d behind the first's, share a byte. Where strides
+    nest, no more than a few places of the outermost dimension can, each decided by what is inside."""
+    ea = ra + sum((n - 1) * s for n, s in a)
+    eb = rb + sum((n - 1) * s for n, s in b)
+    if d >= ea or -d >= eb:
+        return False
+    if not a and not b:
+        return True
+    if a and b and a[0][1] == b[0][1]:  # only the difference of the two places matters
+        (n, s), m = a[0], b[0][0]
+        ia, ib = ea - (n - 1) * s, eb - (m - 1) * s
+        lo, hi = max(-(n - 1), -((ib - 1 + d) // s)), min(m - 1, (ia - 1 - d) // s)
+        inside = (a[1:], ra, b[1:], rb)
+    elif a and (not b or a[0][1] > b[0][1]):
+        n, s = a[0]
+        ia = ea - (n - 1) * s
+        lo, hi = max(-(n - 1), -((d + eb - 1) // s)), min(0, (ia - 1 - d) // s)
+        inside = (a[1:], ra, b, rb)
+    else:
+        m, s = b[0]
+        ib = eb - (m - 1) * s
+        lo, hi = max(0, -((ib - 1 + d) // s)), min(m - 1, (ea - 1 - d) // s)
+        inside = (a, ra, b[1:], rb)
+    if hi - lo >= 4096:
+        return True
+    return any(_meet(d + k * s, *inside) for k in range(lo, hi + 1))
 
 
 def _describe(i: int, t: torch.Tensor, u: torch.Tensor, slot_dim: int,
