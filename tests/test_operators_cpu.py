@@ -11,7 +11,7 @@ from vinfer_b200 import _lib
 from vinfer_b200.beam import BeamSearch
 from vinfer_b200.build import build
 from vinfer_b200.kernels.sampler.b200 import B200Sampler
-from vinfer_b200.sampling import DecodeStates
+from vinfer_b200.sampling import BeamStep, DecodeStates
 
 
 @pytest.fixture(scope="module")
@@ -184,3 +184,18 @@ def test_a_gradient_may_lie_between_the_logits(backend):
             backend.distill_step(buf[:, :10], ids, lp, out=out)
     with pytest.raises(TypeError):  # past the checks: there is no launch here
         backend.distill_step(buf[:, :10], ids, lp, out=buf[:, 10:])
+
+
+def test_beam_outputs_are_six_tensors(backend):
+    """An output given twice would hold whichever was written last."""
+    scores = torch.zeros(2, 4)
+    for a, b in (("scores", "next_scores"), ("beams", "tokens"), ("parents", "next_tokens"),
+                 ("tokens", "parents")):
+        out = BeamStep.empty(2, 4, 4, "cpu")
+        setattr(out, a, getattr(out, b))
+        with pytest.raises(ValueError, match="given twice"):
+            backend.beam_select(torch.zeros(8, 10), scores, 4, out=out)
+    out = BeamStep.empty(2, 4, 4, "cpu")
+    out.next_scores = scores  # as documented
+    with pytest.raises(TypeError):  # past the checks: there is no launch here
+        backend.beam_select(torch.zeros(8, 10), scores, 4, out=out)

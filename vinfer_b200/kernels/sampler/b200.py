@@ -281,10 +281,12 @@ class B200Sampler:
         if out is None:
             out = BeamStep.empty(r, w, n, self.device)
         else:
-            for name, dt, m in (("scores", torch.float32, n), ("beams", torch.int32, n),
-                                ("tokens", torch.int32, n), ("next_scores", torch.float32, w),
-                                ("parents", torch.int32, w), ("next_tokens", torch.int32, w)):
-                self._vector(f"out.{name}", getattr(out, name), dt, r, m)
+            at = {self._vector(f"out.{name}", getattr(out, name), dt, r, m)
+                  for name, dt, m in (("scores", torch.float32, n), ("beams", torch.int32, n),
+                                      ("tokens", torch.int32, n), ("next_scores", torch.float32, w),
+                                      ("parents", torch.int32, w), ("next_tokens", torch.int32, w))}
+            if len(at) < 6 and r:
+                raise ValueError("an output is given twice")
         if stops:
             a.eos = self._vector("eos", eos, torch.int32, stops)
         if r == 0:
