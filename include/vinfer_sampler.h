@@ -293,9 +293,11 @@ int vinfer_reorder_states(const VinferState* states, int32_t n_states, const int
  *   loss[row] = weight * ( sum_j p_j (ln p_j - ln q_j)  [ + p_t (ln p_t - ln q_t) with tail ] )
  * tail == 0: the p_j are first divided by their sum. tail != 0: p_t = max(0, 1 - sum p_j) is matched
  * with q_t, the student's mass outside the list. The loss carries no factor temperature^2.
- * Entries with id < 0 are empty; an entry with log-probability -inf lists its token with mass 0; an
- * id listed twice has the sum of its masses. A row of weight 0 is not read: loss and gradient 0;
- * without tail, a list of no mass gives loss and gradient 0.
+ * Entries with id < 0 are empty; an entry with log-probability -inf lists its token with mass 0. The
+ * sum runs over entries: the masses of an id listed twice add up in all that depends on the logits, so
+ * that the gradient is that of one entry with their sum; the teacher's own p_j ln p_j stay apart, so
+ * that the loss is below that of the one entry by a constant. A row of weight 0 is not read: loss
+ * and gradient 0; without tail, a list of no mass gives loss and gradient 0.
  * An id >= vocab or a log-probability that is NaN or +inf sets VINFER_ST_BAD_LIST, logits without a
  * finite log-sum VINFER_ST_NONFINITE; the row's loss and gradient are then NaN.
  *  - vinfer_distill_loss: losses [rows]; row_stats (float [rows, 2], 8-byte aligned) and list_grads

@@ -9,6 +9,9 @@ set), on the device and in the layout taken here. For rows of student logits ``x
 * with ``tail`` the mass the list leaves over, ``p_t = 1 - sum_j p_j``, is matched with the
   student's mass outside the list: ``... + p_t (ln p_t - ln q_t)``.
 
+The sums run over entries: an id listed twice has the gradient of one entry with its masses' sum, and a
+loss that is lower by a constant (the teacher's ``p ln p`` are taken entry by entry).
+
 The log-probabilities are the teacher's at the same temperature. The reference trains nothing; the
 losses carry no factor ``T ** 2`` (a weight may).
 """
