@@ -13,8 +13,10 @@
 //     beams' scores closer than NEAR could be ordered by the rounding of their sums, so the sums of
 //     such beams (rare) are taken again in double before the order stands.
 //
-// What bounds it: reading the logits once, then the instructions of the exponentials (8 an element
-// with all overheads; the ex2 unit alone is half busy). Measured on one B200, us a step: 32
+// What bounds it: for many long rows reading the logits once; for fewer, no single unit: a step of 256 rows of
+// 151,936 bf16 has 48 % of the issue slots and 53 % of the ex2 unit busy, its 512 parts leave some SMs
+// with three CTAs beside others with four, and two rounds in registers do not cover all of a load's
+// latency (largest stall); launch and ramp take 3 us and picking 4 more. Measured on one B200, us a step: 32
 // requests of 16 beams, 248,320 float32 logits 98.1 (508 MB: 5.2 TB/s, 0.79 of the measured copy
 // bandwidth); 64 of 4, 151,936 bf16 29.0 (77.8 MB: 0.41); one of 4 10.0, most of it the two kernels'
 // latency. Selecting costs little because it is not sorting: a part of a row finds a bar that n of

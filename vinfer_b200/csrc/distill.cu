@@ -20,8 +20,8 @@
 // What bounds them: HBM, then the exponentials' instructions. Measured on one B200, in us, with the share
 // of the measured copy bandwidth: losses of 1,024 rows of 151,936 bf16 58.8 (0.81); of 256 rows 27; the
 // gradient alone of 1,024 rows 104 (6.0 TB/s, 0.91); loss and gradient in one call of 4,096 rows of
-// 151,936 bf16, 512 of them masked, 494 (0.72) against 591 by the three kernels, of 512 rows of 248,320
-// float32 with lists of 128 229 (0.68) against 307.
+// 151,936 bf16, 512 of them masked, 487 (0.73) against 591 by the three kernels, of 512 rows of 248,320
+// float32 with lists of 128 233 (0.67) against 307.
 #include "rows.cuh"
 
 #include <algorithm>
@@ -409,6 +409,8 @@ __global__ void __launch_bounds__(FW * 32) k_distill_finish(const DistP P) {
   if (lane == 0) P.loss[row] = loss * weight;
 }
 
+// CTAs an SM, us with 2 / 3 / 4 / 5: 256 rows of 151,936 bf16 28.0 / 28.0 / 28.9 / 28.4, 1,024 rows 104.4 / 104.5
+// / 104.9 / 106.1, 64 rows of 40,001 float32 7.6 / 7.8 / 7.0 / 7.2.
 template <typename T>
 __global__ void __launch_bounds__(NT, 3) k_distill_grad(const DistP P) {
   using VT = Vec<T>;
@@ -474,9 +476,11 @@ __global__ void __launch_bounds__(NT, 3) k_distill_grad(const DistP P) {
 // all), and hands out the gradient's terms. Two CTAs an SM, so that one streams while the other
 // solves.
 //
-// Measured for 4,096 rows of 151,936 bf16 (512 masked): 494 us; the same kernel without any
-// arithmetic 452, so it is the pipeline of copies that bounds it, at 5.2 TB/s of a mix of reads and
-// writes that a plain streaming kernel takes at 6.0. One CTA an SM with a ring twice as large 545; a
+// Measured for 4,096 rows of 151,936 bf16 (512 masked): 487 us (4.8 TB/s). The same kernel without any
+// arithmetic took 452 where it took 494, so it is the pipeline of copies that bounds it: nine of a
+// row's thirteen chunks cross from L2 twice, in a mix of reads and writes that a plain streaming kernel
+// takes at 6.0 TB/s. 512 rows of 248,320 float32 are eight turns of the 71 clusters of four that run at
+// once, the last a fifth full. Also against those 494: one CTA an SM with a ring twice as large 545; a
 // row whole in the shared memory of four CTAs, the next one summed before it is written, 894 (what
 // a slice waits for, the solution and the copies, takes longer than the slice); chunks of 8
 // vectors a thread 569; three or four CTAs an SM 606 (their slices no longer stay in L2).

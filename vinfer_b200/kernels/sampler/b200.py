@@ -316,7 +316,8 @@ class B200Sampler:
         slot, any shape: ``BeamStep.parents``). In place a moved slot's parent must keep its own
         state, as ``beam_select`` lays beams out; into ``out`` tensors any parent will do. With
         a ``length_dim``, only the first ``lengths[s]`` (int32) positions are copied. A parent
-        out of range, or one that moves itself, leaves the slot alone and sets a status bit."""
+        out of range, or one that moves itself, leaves the slot alone and sets a status bit.
+        Neither tensor may lie in the states that are written."""
         if states.device != self.device:
             raise ValueError(f"states are on {states.device}, backend on {self.device}")
         self._slot_values("parents", parents, states.slots)
