@@ -30,7 +30,7 @@ def make(dev, N, V, k, dtype, seed):
     return x.to(dtype), ids, lp, w
 
 
-# at most 148 clusters of two or 74 of four run at once: seven rows each at least
+# at most 148 clusters of two or 74 of four fit the SMs at once: seven rows each at least
 @pytest.mark.parametrize("N,V,k,dtype", [
     (560, 248320, 128, torch.float32), (530, 248319, 7, torch.float32),
     (1060, 120007, 20, torch.float32), (1040, 262144, 33, torch.bfloat16)],
@@ -63,4 +63,22 @@ def test_clusters_that_take_many_rows(backend, N, V, k, dtype):
         f, t = first_g[r:r + 64].double(), apart[r:r + 64].double()
         tol = 4 * rel * q + f.abs() * (torch.finfo(dtype).eps + 8 * rel) + 2.0**-125
         assert torch.all((f - t).abs() <= tol), (r, ((f - t).abs() - tol).max())
+    backend.check()
+
+
+@pytest.mark.parametrize("N,V,dtype,pad", [(530, 248320, torch.float32, 0), (1040, 120007, torch.float32, 3),
+                                           (1040, 262144, torch.bfloat16, 8),
+                                           (1200, 151936, torch.bfloat16, 0)],
+                         ids=["4 f32", "2 f32 ragged", "2 bf16", "1 bf16"])
+def test_the_gradient_in_the_logits_place(backend, N, V, dtype, pad):
+    """The same bits as out of place, whatever is written while other chunks of the row are read again."""
+    x, ids, lp, w = make(backend.device, N, V, 20, dtype, V + 1)
+    wide = torch.full((N, V + pad), -77.0, dtype=dtype, device=x.device)
+    wide[:, :V] = x  # of the same strides: a row's sum is added in an order that its alignment gives
+    want_l, want_g = backend.distill_step(wide[:, :V], ids, lp, w, temperature=2.0)
+    for _ in range(8):
+        wide[:, :V] = x
+        loss, grad = backend.distill_step(wide[:, :V], ids, lp, w, temperature=2.0, out=wide[:, :V])
+        assert torch.equal(loss, want_l) and torch.equal(grad, want_g)
+        assert (wide[:, V:] == -77).all()
     backend.check()

@@ -1016,8 +1016,8 @@ int launch_step(const DistP& P, cudaStream_t st) {
 // kernels, whose second read of short rows comes from L2 anyway. Measured (us, one pass against
 // three kernels, rows of 151,936 bf16): 31.2 / 24.4 at 32 rows, 33.5 / 43.4 at 148, 169 / 219 at
 // 1,200; 1,200 rows of 65,536 bf16 103 / 100, of 33,000 bf16 80 / 67, of 33,000 float32 86 / 104. Rows
-// that clusters take: 248,320 float32 (four CTAs, 74 clusters) 51.2 / 57.7 at 96, 78.7 / 80.2 at 148 (two
-// turns), 223 / 292 at 600; 120,007 float32 (two) 31.2 / 36.2 at 96; 262,144 bf16 (two) 39.8 / 40.6
+// that clusters take: 248,320 float32 (four CTAs, 71 clusters) 51.2 / 57.7 at 96, 78.7 / 80.2 at 148 (a
+// third turn), 223 / 292 at 600; 120,007 float32 (two) 31.2 / 36.2 at 96; 262,144 bf16 (two) 39.8 / 40.6
 // at 96, 67.2 / 66.2 at 200, 151 / 165 at 600.
 bool step_in_one(const DistP& P, int dtype) {
   const bool bf = dtype == VINFER_DTYPE_BF16;
