@@ -68,3 +68,18 @@ def test_distillation_of_large_logits(backend, N, V, tail, dtype):
         _, _, loss, grad, steps = run_all(backend, x, ids, lp, w, T, tail)
         for l, gr in [(loss, grad), *steps]:
             compare(x[sel], ids[sel], lp[sel], w[sel], T, tail, l[sel], gr[sel])
+
+
+@pytest.mark.parametrize("N,V", [(400, 501), (300, 40001)])
+def test_large_losses_are_rounded_once(backend, N, V):
+    """Listed tokens under a finite mask: losses of thousands, whose rounding is all that shows."""
+    g = torch.Generator().manual_seed(N)
+    k = 4
+    x = torch.randn(N, V, generator=g)
+    x[:, 100:] = -30000.0
+    ids = torch.stack([torch.randperm(V - 100, generator=g)[:k] + 100 for _ in range(N)]).int()
+    lp = torch.log_softmax(torch.randn(N, k, generator=g), 1) - 0.5
+    w = torch.rand(N, generator=g) * 1e-3 + 1e-3  # a mean's weights
+    _, _, loss, _, steps = run_all(backend, x, ids, lp, w, 1.0, True)
+    for l in [loss] + [l for l, _ in steps]:
+        compare(x, ids, lp, w, 1.0, True, l)

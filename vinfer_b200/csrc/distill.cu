@@ -351,12 +351,13 @@ __device__ __forceinline__ Stat list_grads(const DistP& P, const ListS& L, const
   return Stat{m, f * (float)((S.mass * S.rest - S.pt) / r)};
 }
 
-__device__ __forceinline__ float list_loss(const DistP& P, const ListS& L, const Solved& S) {
+// The row's loss, to be weighted before it is rounded.
+__device__ __forceinline__ double list_loss(const DistP& P, const ListS& L, const Solved& S) {
   const int lane = threadIdx.x & 31;
   if (lost(S)) {
     if (lane == 0 && P.status)
       atomicOr(P.status, (int)(S.bad ? VINFER_ST_BAD_LIST : VINFER_ST_NONFINITE));
-    return __int_as_float(0x7fffffff);
+    return (double)__int_as_float(0x7fffffff);
   }
   const double lse = log(S.total), lnorm = S.norm == 1 ? 0.0 : -log(S.norm);
   const double unit = P.scale_d * LN2_D;
@@ -367,7 +368,7 @@ __device__ __forceinline__ float list_loss(const DistP& P, const ListS& L, const
               (((double)L.l[j] - lnorm) - (((double)L.z[j] - S.ref) * unit - lse));
   loss = warp_sum(loss);
   if (S.pt > 0) loss += S.pt * (log(S.pt) - log(S.rest));
-  return (float)loss;
+  return loss;
 }
 
 constexpr int FW = 4;  // rows of a finishing CTA, one a warp
@@ -405,8 +406,8 @@ __global__ void __launch_bounds__(FW * 32) k_distill_finish(const DistP P) {
     const Stat st = list_grads(P, L, S, m, r, 1.f, P.listg + row * P.k);
     if (lane == 0) P.stat[row] = st;
   }
-  const float loss = list_loss(P, L, S);
-  if (lane == 0) P.loss[row] = loss * weight;
+  const double loss = list_loss(P, L, S);
+  if (lane == 0) P.loss[row] = (float)(loss * weight);
 }
 
 // CTAs an SM, us with 2 / 3 / 4 / 5: 256 rows of 151,936 bf16 28.0 / 28.0 / 28.9 / 28.4, 1,024 rows 104.4 / 104.5
@@ -790,8 +791,8 @@ __global__ void __launch_bounds__(STEP_T, STEP_CTAS) k_distill_step(const __grid
       }
       __syncwarp();
       if (lane == 0) bar_arrive(&B.solved);
-      const float loss = list_loss(P, B.list, sol);
-      if (rank == 0 && lane == 0) P.loss[row] = loss * weight;
+      const double loss = list_loss(P, B.list, sol);
+      if (rank == 0 && lane == 0) P.loss[row] = (float)(loss * weight);
       __syncwarp();
     }
   } else {  // ---- the warps that sum and write
